@@ -218,6 +218,195 @@ int qx_cuda_final_head_noalloc(const float *residual_dev, const float *norm_weig
                                uint32_t hidden, uint32_t vocab, float *logits_dev, uint32_t *argmax_dev, void *stream,
                                char *err, uint64_t err_len);
 
+/* ---- device operators ----------------------------------------------------
+ *
+ * The steps of a decode loop that runs drafted tokens over an INT8 K/V cache of
+ * the engine's layout: rotate and append (qx_cuda_rope_append), attend
+ * (qx_cuda_tree_attention), pick a token per drafted node
+ * (qx_cuda_pick_tokens, after qx_cuda_final_head_noalloc or a caller's own
+ * head), and shorten a cache that is full (qx_cuda_kv_evict).  No counterpart
+ * in the reference, which decodes one token at a time on the CPU.
+ *
+ * All of them queue their work on `stream` (cudaStream_t, NULL = default) and
+ * return without waiting.  Pointers are device pointers the caller owns, on
+ * one device, which need not be the current one.  Nothing is allocated: scratch comes from the
+ * caller (`workspace`), belongs to one call at a time and needs no initial
+ * value, so calls may be captured into CUDA graphs; graphs or streams that can
+ * run at the same time need a workspace each.  Lengths, slots and node counts
+ * are read on the device when the call runs, so a captured call follows them.
+ * What the host can check (sizes, strides, alignment, types, NULLs) is refused
+ * with a message before anything is queued.  What only the device can see is
+ * checked there: a sequence whose slot, length or node count does not fit the
+ * cache, or which writes to a slot that another sequence of the call also
+ * uses, is left out of the call (nothing is read or written for it) and a bit
+ * is set in *status (device uint32, may be NULL; bits are only ever added).  */
+#define QX_CUDA_F32  0u
+#define QX_CUDA_F16  1u
+#define QX_CUDA_BF16 2u
+
+#define QX_CUDA_STATUS_RANGE  0x1u   /* slot, length or nodes outside the cache */
+#define QX_CUDA_STATUS_SHARED 0x2u   /* a slot written by a call is also another sequence's */
+
+/* An INT8 cache: the codes of row r of layer l of slot s are the
+ * kv_heads * head_dim bytes at row s * slot_rows + l * layer_rows + r of k and
+ * v, its scales at that index of k_scales and v_scales (value = code * scale;
+ * one scale per row for all KV heads, src/qx_format.c:6343-6362).  k and v are
+ * 16-byte aligned; layer_rows >= ctx_tokens where there is more than one
+ * layer, and the slots of a cache do not overlap. */
+typedef struct qx_cuda_kv_cache {
+    int8_t *k, *v;
+    float *k_scales, *v_scales;
+    uint64_t slot_rows, layer_rows;
+    uint32_t slots, layers, ctx_tokens, kv_heads, head_dim, reserved;
+} qx_cuda_kv_cache;
+
+/* The cache of an engine for the operators: which = 0 its own
+ * (qx_cuda_prefill, qx_cuda_decode_step; one slot), 1 the sequence slots of
+ * qx_cuda_decode_batch (once that has been called).  The engine's own calls
+ * run on qx_cuda_stream(engine); order the operators after them.  The view
+ * ends with the engine. */
+int qx_cuda_kv_view(const qx_cuda_engine *engine, uint32_t which, qx_cuda_kv_cache *out, char *err, uint64_t err_len);
+
+/* The drafted tokens of a call: `seqs` sequences of up to `max_nodes` nodes.
+ * Sequence i has slot slots[i], lens[i] committed rows 0..lens[i]-1, and
+ * nodes[i] <= max_nodes drafted tokens (nodes NULL: max_nodes each) whose rows
+ * are lens[i] .. lens[i] + nodes[i] - 1. */
+typedef struct qx_cuda_drafts {
+    uint32_t seqs, max_nodes;
+    const int32_t *slots, *lens, *nodes;
+} qx_cuda_drafts;
+
+/* A [seqs][max_nodes][heads][head_dim] tensor; strides in elements, the last
+ * dimension contiguous.  Inputs may be broadcast (stride 0), outputs may not
+ * overlap themselves. */
+typedef struct qx_cuda_heads {
+    void *data;
+    uint64_t seq_stride, node_stride, head_stride;
+} qx_cuda_heads;
+
+/* How a head is rotated: pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * interleaved, of its first rotary_dim values (even, <= head_dim) turn by the
+ * angle position * inv_freq[i]; the rest passes through.  cos and sin are
+ * multiplied by amplitude (1 without YaRN scaling).  inv_freq is a device array of
+ * rotary_dim / 2 doubles. */
+typedef struct qx_cuda_rotary {
+    const double *inv_freq;
+    double amplitude;
+    uint32_t rotary_dim, interleaved;
+} qx_cuda_rotary;
+
+/* The frequencies of a context-extension scheme (host only, no device needed):
+ * inv_freq[rotary_dim / 2] doubles and the amplitude.
+ *   NONE   base^(-2i/rotary_dim)
+ *   LINEAR those / factor
+ *   NTK    base * factor^(rotary_dim / (rotary_dim - 2)) as the base
+ *   YARN   by parts: a ramp over i between the dimensions that turn `low` and
+ *          `high` times within original_ctx (1 and 32 are usual) blends LINEAR
+ *          into NONE; amplitude 0.1 ln(factor) + 1
+ *   BANDS  by wavelength: longer than original_ctx / low -> LINEAR, shorter
+ *          than original_ctx / high -> NONE, blended in between */
+#define QX_CUDA_ROPE_NONE   0u
+#define QX_CUDA_ROPE_LINEAR 1u
+#define QX_CUDA_ROPE_NTK    2u
+#define QX_CUDA_ROPE_YARN   3u
+#define QX_CUDA_ROPE_BANDS  4u
+int qx_cuda_rope_frequencies(uint32_t scheme, uint32_t rotary_dim, double base, double factor, double original_ctx,
+                             double low, double high, double *inv_freq, double *amplitude, char *err,
+                             uint64_t err_len);
+
+/* Rotate the drafted tokens' queries and keys and append keys and values to
+ * layer `layer` of the cache.  positions[seqs][max_nodes] (int32; NULL: node j
+ * of sequence i is at lens[i] + j) need not be distinct or increasing: nodes
+ * of one depth of a tree share a position.  Keys turn in double, are rounded
+ * to F32 and quantized by the cache's row rule (scale = largest finite
+ * magnitude / 127, 1 if that is 0; codes rounded half to even, non-finite
+ * values 0; src/qx_format.c:6343-6362); queries turn in F32 and are rounded
+ * to `dtype` (which q, q_out, k and v share).  q_out may be q itself (same
+ * pointer and strides).  q and q_out may both have data NULL (q_heads 0), or
+ * k and v (no append). */
+int qx_cuda_rope_append(const qx_cuda_kv_cache *cache, uint32_t layer, const qx_cuda_drafts *drafts,
+                        const qx_cuda_rotary *rotary, uint32_t dtype, uint32_t q_heads, const qx_cuda_heads *q,
+                        const qx_cuda_heads *q_out, const qx_cuda_heads *k, const qx_cuda_heads *v,
+                        const int32_t *positions, uint32_t *status, void *stream, char *err, uint64_t err_len);
+
+/* Attention of the drafted tokens over layer `layer` of the cache.  Node j of
+ * sequence i sees the committed rows and those tree rows whose bit is set in
+ * its mask: bit b of mask[(i * max_nodes + j) * words + b / 64], words =
+ * (max_nodes + 63) / 64, is tree row b (its own row too needs its bit); with
+ * mask NULL, rows 0..j (a chain: plain causal attention, and with max_nodes 1
+ * a decode step).  Query head h reads KV head h / (q_heads / kv_heads).
+ * Weights are softmax(scale * q.k) over what the node sees; a node that sees
+ * nothing gets zeros (and lse -infinity).  What a node does not see does not
+ * touch it, whatever it holds.  head_dim 64 or 128; q and out share `dtype`;
+ * scores, softmax and sums are held in F32.  The value scales of rows that
+ * are seen must not be negative; ones below 2^-90 count as 2^-90.
+ *   lse[seqs][max_nodes][q_heads] (F32, may be NULL): log of the softmax sum.
+ *   mass (F32, one value per row at the index of the row's scales, may be
+ *   NULL): adds, for each row, the weights that all nodes and heads of the
+ *   call gave it - what qx_cuda_kv_evict goes by.  Sequences of one call then
+ *   need distinct slots.
+ * Rows of out and lse past a sequence's nodes stay as they were.  Sequences
+ * may share a slot when mass is NULL.  The same call gives the same bits every
+ * time; how a sequence's rows are split over the GPU, and so its rounding,
+ * follows from the lengths of the whole call. */
+int qx_cuda_tree_attention(const qx_cuda_kv_cache *cache, uint32_t layer, const qx_cuda_drafts *drafts,
+                           uint32_t dtype, uint32_t q_heads, const qx_cuda_heads *q, const qx_cuda_heads *out,
+                           const uint64_t *mask, float scale, float *lse, float *mass, void *workspace,
+                           uint64_t workspace_bytes, uint32_t *status, void *stream, char *err, uint64_t err_len);
+
+/* Bytes of workspace (16-byte aligned) that qx_cuda_tree_attention needs for
+ * drafts of up to seqs x max_nodes on any B200 (host only). */
+int qx_cuda_tree_attention_workspace(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_heads,
+                                     uint32_t head_dim, uint32_t dtype, uint64_t *bytes, char *err, uint64_t err_len);
+
+/* Evict rows by accumulated attention weight, in every layer of `seqs`
+ * sequences: of a sequence's lens[i] rows keep the first `sink`, the last
+ * `recent`, and of those between the ones with the largest mass, up to
+ * `budget` rows in all (sink + recent <= budget), in their order; equal mass
+ * keeps the lower row, NaN counts as less than any number.  Sequences of at
+ * most `budget` rows keep all.  The kept rows' codes, scales and mass move to
+ * rows 0.. of slot dst_slots[i] (NULL: in place), the mass of the rows behind
+ * them up to lens[i] becomes 0, and other rows stay as they were.  A
+ * destination slot must be no other sequence's source or destination.
+ *   kept[layers][seqs][budget] (int32): the rows kept, -1 past the last;
+ *   all -1 for a sequence left out.
+ *   new_lens[seqs] (int32, not lens itself): min(lens[i], budget); lens[i] for
+ *   a sequence left out. */
+int qx_cuda_kv_evict(const qx_cuda_kv_cache *cache, uint32_t seqs, const int32_t *slots, const int32_t *dst_slots,
+                     const int32_t *lens, float *mass, uint32_t budget, uint32_t sink, uint32_t recent, int32_t *kept,
+                     int32_t *new_lens, uint32_t *status, void *stream, char *err, uint64_t err_len);
+
+/* Penalties for repeated tokens, biases and a grammar mask on `rows` rows of
+ * logits, and each row's greedy token.  Per row r and token t, in F32:
+ *   x = logits[t]; c = how often t is in history[r][0 .. history_lens[r])
+ *   c > 0: x = x > 0 ? x / repetition[r] : x * repetition[r],
+ *          x = x - frequency[r] * c, x = x - presence[r]
+ *   t in bias_ids[r][0 .. bias_lens[r]): x = x + its bias value (the last
+ *          entry's, where an id is listed twice)
+ *   bit t % 32 of allowed[r][t / 32] is 0: x = -infinity, whatever the logit
+ * out (may be NULL, may be logits) gets x rounded to dtype; picked[r] the
+ * lowest token of the largest x, or 0xFFFFFFFF when nothing finite is left or
+ * an x is NaN or +infinity.  Ids outside the vocabulary are ignored.  Any of
+ * history, bias_ids, allowed may be NULL; so may repetition (1), frequency (0),
+ * presence (0), history_lens (max_history each), bias_lens (max_bias each).
+ * Lengths below 0 count as 0, above the maximum as the maximum.  Strides are
+ * in elements (of uint32 for allowed).  max_history < 2^20, max_bias <= 4095,
+ * vocab <= 393216.  dtype is that of logits and out. */
+typedef struct qx_cuda_pick {
+    const void *logits;
+    void *out;
+    uint64_t logits_stride, out_stride;
+    uint32_t rows, vocab, dtype, max_history, max_bias, reserved;
+    const int32_t *history, *history_lens;
+    const float *repetition, *frequency, *presence;
+    const int32_t *bias_ids, *bias_lens;
+    const float *bias_values;
+    const uint32_t *allowed;
+    uint64_t history_stride, bias_stride, allowed_stride;
+    uint32_t *picked;
+} qx_cuda_pick;
+int qx_cuda_pick_tokens(const qx_cuda_pick *args, void *stream, char *err, uint64_t err_len);
+
 /* ---- persistent KV ---------------------------------------------------- */
 
 /* Write / read `count` positions of layer `layer` starting at `first`:

@@ -1260,6 +1260,29 @@ QX_API int qx_cuda_profile_get(const qx_cuda_engine* E, qx_cuda_profile* out) {
     return 1;
 }
 
+QX_API int qx_cuda_kv_view(const qx_cuda_engine* E, uint32_t which, qx_cuda_kv_cache* out, char* err, uint64_t n) {
+    if (!E || !out || which > 1) { set_err(err, n, "invalid cache view argument"); return 0; }
+    if (which == 1 && !E->batch.slot_mem) {
+        set_err(err, n, "the sequence slots exist from the first qx_cuda_decode_batch");
+        return 0;
+    }
+    qx_cuda_kv_cache c{};
+    const uint64_t C = E->dm.ctx, L = E->dm.layers;
+    c.k = which ? E->batch.slots.k : E->dev.kcache;
+    c.v = which ? E->batch.slots.v : E->dev.vcache;
+    c.k_scales = which ? E->batch.slots.ks : E->dev.kscale;
+    c.v_scales = which ? E->batch.slots.vs : E->dev.vscale;
+    c.slot_rows = L * C;
+    c.layer_rows = C;
+    c.slots = which ? QX_CUDA_MAX_SLOTS : 1;
+    c.layers = (uint32_t)L;
+    c.ctx_tokens = (uint32_t)C;
+    c.kv_heads = (uint32_t)E->dm.kv_heads;
+    c.head_dim = (uint32_t)E->dm.head_dim;
+    *out = c;
+    return 1;
+}
+
 QX_API void* qx_cuda_stream(const qx_cuda_engine* E) { return E ? (void*)E->stream : nullptr; }
 
 QX_API int qx_cuda_time_kernels(qx_cuda_engine* E, uint32_t token, uint32_t position, uint32_t steps, char* names,

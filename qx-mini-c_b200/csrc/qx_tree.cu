@@ -1,0 +1,741 @@
+// Attention of drafted tokens over the INT8 cache (qx_cuda_tree_attention).
+//
+// For a query row q (one node, one head) and cache row t with codes k_t, v_t
+// and scales ks_t, vs_t:
+//     s_t = scale ks_t (q . k_t),   o = sum_t e^(s_t) vs_t v_t / sum_t e^(s_t).
+// In base 2 and with the value scale inside the exponent,
+//     x_t = s_t log2(e) + log2(vs_t),   P_t = 2^(x_t - m + 14),   m = max x_t,
+//     o = sum_t P_t v_t / sum_t (P_t / vs_t):
+// what meets the codes v_t in the second product is one F16 number in
+// (0, 2^14] per (row, t) whatever the scales are, and the running maximum of
+// x_t is the only thing the accumulators are ever rescaled by.
+//
+// INT8 codes are exact in F16, so both products run on the tensor cores as F16
+// with F32 accumulation.  F16 and BF16 queries are one F16 term: a row is
+// multiplied by a power of two that puts its largest value in [2^13, 2^14)
+// (BF16 values more than 2^38 below it lose bits).  F32 queries, and P_t then too,
+// are two F16 terms (hi + the rest, 22 bits).  Everything else is F32.
+//
+// Work is cut into units (sequence, KV head, block of rows) and those into
+// tiles of 64 cache rows; the tiles of all units, laid end to end, are shared
+// out evenly over the CTAs.  A CTA that has all of a unit's tiles writes its
+// rows; parts of a unit go to the workspace as (m, sum, o) and
+// k_tree_join adds them in the order of their tiles.
+#include <cmath>
+
+#include "qx_ops.cuh"
+
+namespace {
+
+using namespace qx::ops;
+
+constexpr int kTreeThreads = 128, kTreeWarps = 4, kTile = 64;
+constexpr int kScanThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPBias = 14.f;            // P_t = 2^(x_t - m + 14): 2^-24 / 2^14 is the smallest step of an F16 P_t
+constexpr float kMinLogVs = -90.f;        // value scales below 2^-90 count as that: 2^14 2^90 times 65536 rows still fits the F32 sum
+
+struct Tensor {
+    void* p;
+    size_t seq, node, head;
+};
+
+struct TreeArgs {
+    Cache c;
+    Drafts d;
+    int layer, q_heads, group, block_rows, row_blocks;   // row_blocks: of max_nodes * group rows
+    Tensor q, out;
+    int wide;                                             // 16-byte accesses to q and out
+    const unsigned long long* mask;
+    int words;
+    float scale;
+    float* lse;                                           // caller's, or null
+    float* lse2;                                          // workspace: base-2 log sums, for the mass
+    float* mass;
+    float* parts;                                         // [2 * ctas][block_rows][head_dim + 2]
+    int ctas;
+    uint32_t* status;
+};
+
+// ---- which tiles are whose -----------------------------------------------------
+
+// A sequence's share of the work: units of `tiles` tiles each, `units` of them.
+struct SeqWork {
+    int tiles, units;
+};
+__device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool report) {
+    const int slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
+    if (!fits(a.c, a.d, slot, len, n)) {
+        if (report && a.status) atomicOr(a.status, QX_CUDA_STATUS_RANGE);
+        return {0, 0};
+    }
+    if (n == 0) return {0, 0};
+    return {(len + n + kTile - 1) / kTile, a.c.kv_heads * ((n * a.group + a.block_rows - 1) / a.block_rows)};
+}
+
+// Prefix sums of the sequences' tiles, held by the threads of a CTA: thread t
+// has the sequences [t * per, (t + 1) * per).
+struct Scan {
+    long long first, total;      // tiles before this thread's sequences, and in all
+    int s0, s1;
+};
+__device__ __forceinline__ Scan scan_sequences(const TreeArgs& a, long long* warp_sum, bool report) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
+    Scan r;
+    r.s0 = min(a.d.seqs, (int)threadIdx.x * per);
+    r.s1 = min(a.d.seqs, r.s0 + per);
+    long long mine = 0;
+    for (int s = r.s0; s < r.s1; ++s) {
+        const SeqWork k = seq_work(a, s, report);
+        mine += (long long)k.tiles * k.units;
+    }
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += t;
+    }
+    if (lane == 31) warp_sum[w] = inc;
+    __syncthreads();
+    long long base = 0, total = 0;
+    for (int i = 0; i < kScanThreads / 32; ++i) {
+        if (i < w) base += warp_sum[i];
+        total += warp_sum[i];
+    }
+    r.first = base + inc - mine;
+    r.total = total;
+    return r;
+}
+__device__ __forceinline__ long long share(long long total, int ctas, int c) { return total * c / ctas; }
+
+// ---- F16 operands --------------------------------------------------------------
+
+// Four INT8 codes as F16: b + 128 as the low byte of 0x64xx is 1024 + b + 128,
+// and subtracting 1152 is exact.
+__device__ __forceinline__ uint32_t sub1152(uint32_t x) {
+    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t low_pair(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t high_pair(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4342)); }
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The pair minus its F16 rounding, as F16.
+__device__ __forceinline__ uint32_t rest_half(float a, float b, uint32_t hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    return pack_half(a - f.x, b - f.y);
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <class T>
+__device__ __forceinline__ float load_q(const Tensor& q, size_t at) { return to_f32(((const T*)q.p)[at]); }
+
+// ---- one warp's 16 cache rows --------------------------------------------------
+
+// Rows 4 j .. 4 j + 3 of the 16 belong to the lanes with lane % 4 = j, in both
+// products: accumulator column 2 j + c of key tile h is row 4 j + 2 h + c.
+template <int HD>
+struct KvRegs {
+    uint4 k[2][HD / 64];       // key tile h, row lane / 4 of it: bytes 64 c + 16 j ..
+    uint32_t v[4][HD / 32];    // rows 4 j + i, dims (lane / 4) * HD / 8 ..
+    float ks[4], vs[4];
+};
+
+template <int HD>
+__device__ __forceinline__ void load_kv(const TreeArgs& a, size_t base_row, int row0, int last, int g, KvRegs<HD>& r) {
+    const int lane = threadIdx.x & 31, j = lane & 3, n = lane >> 2;
+    const size_t KV = (size_t)a.c.kv_heads * HD;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = min(row0 + 4 * (n >> 1) + 2 * h + (n & 1), last);
+        const int8_t* p = a.c.k + (base_row + row) * KV + (size_t)g * HD + 16 * j;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) r.k[h][c] = __ldg(reinterpret_cast<const uint4*>(p + 64 * c));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = min(row0 + 4 * j + i, last);
+        const int8_t* p = a.c.v + (base_row + row) * KV + (size_t)g * HD + (HD / 8) * n;
+        if (HD == 128) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+            r.v[i][0] = w.x, r.v[i][1] = w.y;
+            r.v[i][HD / 32 - 2] = w.z, r.v[i][HD / 32 - 1] = w.w;
+        } else {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+            r.v[i][0] = w.x, r.v[i][1] = w.y;
+        }
+        r.ks[i] = __ldg(a.c.ks + base_row + row);
+        r.vs[i] = __ldg(a.c.vs + base_row + row);
+    }
+}
+
+// q . k for 16 query rows (staged at qs) and the 16 cache rows: acc[h] is the
+// accumulator of key tile h.
+template <int HD, int NT>
+__device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qterm, const KvRegs<HD>& r, float (&acc)[2][4]) {
+    const int lane = threadIdx.x & 31, j = lane & 3, n = lane >> 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[h][i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) {
+        uint32_t b[2][8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t w[4] = {r.k[h][c].x, r.k[h][c].y, r.k[h][c].z, r.k[h][c].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t u = w[i] ^ 0x80808080u;
+                b[h][2 * i] = low_pair(u);
+                b[h][2 * i + 1] = high_pair(u);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const __half* q0 = qs + t * qterm + n * qstride + 64 * c + 16 * j;
+            uint32_t lo[8], hi[8];
+            *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(q0);
+            *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(q0 + 8);
+            *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride);
+            *reinterpret_cast<uint4*>(hi + 4) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride + 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t af[4] = {lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1]};
+                mma16816(acc[0], af, b[0][2 * i], b[0][2 * i + 1]);
+                mma16816(acc[1], af, b[1][2 * i], b[1][2 * i + 1]);
+            }
+        }
+    }
+}
+
+// Which of a query row's node's keys a thread may see: row t of the sequence.
+__device__ __forceinline__ bool sees(const TreeArgs& a, const unsigned long long* mrow, int node, int t, int len, int n) {
+    if (t < len) return true;
+    const int b = t - len;
+    if (b >= n) return false;
+    return mrow ? (mrow[b >> 6] >> (b & 63)) & 1ull : b <= node;
+}
+
+// Stage `rows` query rows (from row0 on, `have` of them real) as F16 terms and
+// the factor that undoes their power of two; whole CTA.
+template <class T, int HD, int NT>
+__device__ __forceinline__ void stage_queries(const TreeArgs& a, int s, int g, int row0, int rows, int have, __half* qs,
+                                              int qstride, int qterm, float* qfac) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    for (int r = w; r < rows; r += nw) {
+        float x[HD / 32];
+        float big = 0.f;
+        if (r < have) {
+            const int node = (row0 + r) / a.group, h = g * a.group + (row0 + r) % a.group;
+            const size_t at = s * a.q.seq + node * a.q.node + h * a.q.head;
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+                x[i] = load_q<T>(a.q, at + lane + 32 * i);
+                big = fmaxf(big, isfinite(x[i]) ? fabsf(x[i]) : 0.f);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) x[i] = 0.f;
+        }
+        for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
+        // exponent e with big in [2^e, 2^(e+1)): times 2^(13 - e), in two exact steps
+        const int e = big > 0.f ? ilogbf(big) : 0;
+        const int up = 13 - e, u0 = up / 2;
+        const float f0 = __uint_as_float((uint32_t)(127 + u0) << 23), f1 = __uint_as_float((uint32_t)(127 + up - u0) << 23);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+            const float y = x[i] * f0 * f1;
+            const __half hi = __float2half_rn(y);
+            qs[r * qstride + lane + 32 * i] = hi;
+            if (NT == 2) qs[qterm + r * qstride + lane + 32 * i] = __float2half_rn(y - __half2float(hi));
+        }
+        if (lane == 0) qfac[r] = ldexpf(a.scale * kLog2e, -up);
+    }
+}
+
+// ---- the kernel for small trees ------------------------------------------------
+
+// MT blocks of 16 query rows; each of the 4 warps takes 16 of a tile's 64
+// cache rows, straight from global memory into the registers of the products
+// (the next tile's while this one is computed), keeps its own m, sum and o,
+// and the four are joined when the unit's part ends.
+template <class T, int HD, int NT, int MT>
+__global__ void __launch_bounds__(kTreeThreads) k_tree_small(TreeArgs a) {
+    constexpr int BM = 16 * MT, QS = HD + 8, NV = HD / 8;
+    __shared__ __align__(16) __half qs[NT * BM * QS];
+    __shared__ float qfac[BM];
+    __shared__ float wm[kTreeWarps][16], wl[kTreeWarps][16];
+    __shared__ __align__(16) float wo[kTreeWarps][16][HD + 4];
+    __shared__ long long warp_sum[kScanThreads / 32];
+    __shared__ int at_seq;
+    __shared__ long long at_first;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
+    const Scan sc = scan_sequences(a, warp_sum, blockIdx.x == 0);
+    const long long begin = share(sc.total, a.ctas, blockIdx.x), end = share(sc.total, a.ctas, blockIdx.x + 1);
+    if (begin >= end) return;
+    {   // the sequence that holds tile `begin`
+        long long f = sc.first;
+        for (int s = sc.s0; s < sc.s1; ++s) {
+            const SeqWork k = seq_work(a, s, false);
+            const long long t = (long long)k.tiles * k.units;
+            if (begin >= f && begin < f + t) at_seq = s, at_first = f;
+            f += t;
+        }
+    }
+    __syncthreads();
+    int s = at_seq;
+    long long seq_first = at_first;
+    SeqWork k = seq_work(a, s, false);
+    long long pos = begin;
+    while (pos < end) {
+        while (pos >= seq_first + (long long)k.tiles * k.units) {
+            seq_first += (long long)k.tiles * k.units;
+            k = seq_work(a, ++s, false);
+        }
+        const int slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
+        const int unit = (int)((pos - seq_first) / k.tiles), tile0 = (int)((pos - seq_first) % k.tiles);
+        const long long unit_first = seq_first + (long long)unit * k.tiles;
+        const int tile1 = (int)min((long long)k.tiles, end - unit_first);
+        const int g = unit % a.c.kv_heads, row0 = unit / a.c.kv_heads * BM, have = min(BM, n * a.group - row0);
+        const size_t base_row = (size_t)slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
+        const int last = len + n - 1;
+        // in a chain no row of this block sees past its last node
+        const int limit = a.mask ? len + n : min(len + n, len + (row0 + have - 1) / a.group + 1);
+        KvRegs<HD> kv;
+        int r0 = tile0 * kTile + 16 * warp;
+        if (r0 < min(limit, tile1 * kTile)) load_kv<HD>(a, base_row, r0, last, g, kv);
+        stage_queries<T, HD, NT>(a, s, g, row0, BM, have, qs, QS, BM * QS, qfac);
+        __syncthreads();
+        float m[MT][2], l[MT][2], o[MT][NV][4], fac[MT][2];
+        const unsigned long long* mrow[MT][2];
+        int node[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = 16 * t + n8 + 8 * u;
+                m[t][u] = -INFINITY, l[t][u] = 0.f;
+                fac[t][u] = qfac[r];
+                node[t][u] = r < have ? (row0 + r) / a.group : -1;
+                mrow[t][u] = a.mask && r < have ? a.mask + ((size_t)s * a.d.max_nodes + node[t][u]) * a.words : nullptr;
+            }
+#pragma unroll
+            for (int d = 0; d < NV; ++d) o[t][d][0] = o[t][d][1] = o[t][d][2] = o[t][d][3] = 0.f;
+        }
+        for (; r0 < min(limit, tile1 * kTile); r0 += kTile) {
+            float ks[4], lv[4], iv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ks[i] = kv.ks[i];
+                lv[i] = fmaxf(__log2f(kv.vs[i]), kMinLogVs);
+                if (!(kv.vs[i] >= 0.f)) lv[i] = __int_as_float(0x7fc00000);
+                iv[i] = kv.vs[i] > 0x1p-90f ? __frcp_rn(kv.vs[i]) : 0x1p90f;
+            }
+            const bool edge = r0 + 16 > len;
+            uint32_t p[MT][NT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                float acc[2][4];
+                dot_keys<HD, NT>(qs + 16 * t * QS, QS, BM * QS, kv, acc);
+                // acc[h][2 u + c]: query row n8 + 8 u, cache row r0 + 4 j + 2 h + c
+                float x[2][4];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[u][i] = fmaf(acc[i >> 1][2 * u + (i & 1)] * fac[t][u], ks[i], lv[i]);
+                        if (edge && (node[t][u] < 0 || !sees(a, mrow[t][u], node[t][u], r0 + 4 * j + i, len, n)))
+                            x[u][i] = -INFINITY;
+                    }
+                float up[2];
+                bool grew = false;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float mx = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
+                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+                    up[u] = fmaxf(mx, m[t][u]);
+                    grew |= up[u] > m[t][u];
+                }
+                if (__any_sync(~0u, grew)) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float f = up[u] > m[t][u] ? exp2_fast(m[t][u] - up[u]) : 1.f;
+                        l[t][u] *= f;
+#pragma unroll
+                        for (int d = 0; d < NV; ++d) o[t][d][2 * u] *= f, o[t][d][2 * u + 1] *= f;
+                        m[t][u] = up[u];
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float ref = m[t][u] == -INFINITY ? 0.f : m[t][u] - kPBias;
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        e[i] = exp2_fast(x[u][i] - ref);
+                        l[t][u] = fmaf(x[u][i] == -INFINITY ? 0.f : e[i], x[u][i] == -INFINITY ? 0.f : iv[i], l[t][u]);
+                    }
+                    p[t][0][u] = pack_half(e[0], e[1]);
+                    p[t][0][2 + u] = pack_half(e[2], e[3]);
+                    if (NT == 2) {
+                        p[t][NT - 1][u] = rest_half(e[0], e[1], p[t][0][u]);
+                        p[t][NT - 1][2 + u] = rest_half(e[2], e[3], p[t][0][2 + u]);
+                    }
+                }
+            }
+            // values: dims (lane / 4) * NV + d of rows 4 j .. 4 j + 3 are column lane / 4 of value tile d
+#pragma unroll
+            for (int w = 0; w < HD / 32; ++w) {
+                const uint32_t v0 = kv.v[0][w] ^ 0x80808080u, v1 = kv.v[1][w] ^ 0x80808080u,
+                               v2 = kv.v[2][w] ^ 0x80808080u, v3 = kv.v[3][w] ^ 0x80808080u;
+                const uint32_t a0 = __byte_perm(v0, v1, 0x5140), a1 = __byte_perm(v0, v1, 0x7362);
+                const uint32_t c0 = __byte_perm(v2, v3, 0x5140), c1 = __byte_perm(v2, v3, 0x7362);
+                const uint32_t b0[4] = {low_pair(a0), high_pair(a0), low_pair(a1), high_pair(a1)};
+                const uint32_t b1[4] = {low_pair(c0), high_pair(c0), low_pair(c1), high_pair(c1)};
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int q = 0; q < NT; ++q) mma16816(o[t][4 * w + d], p[t][q], b0[d], b1[d]);
+            }
+            if (r0 + kTile < min(limit, tile1 * kTile)) load_kv<HD>(a, base_row, r0 + kTile, last, g, kv);
+        }
+        // join the four warps, block of 16 rows by block
+        const bool whole = tile0 == 0 && tile1 == k.tiles;
+        float* part = a.parts + (size_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * BM * (HD + 2);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                l[t][u] += __shfl_xor_sync(~0u, l[t][u], 1);
+                l[t][u] += __shfl_xor_sync(~0u, l[t][u], 2);
+                if (j == 0) wm[warp][n8 + 8 * u] = m[t][u], wl[warp][n8 + 8 * u] = l[t][u];
+                // columns 2 j, 2 j + 1 of value tile d are dims 2 j NV + d and (2 j + 1) NV + d
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int d = 0; d < NV; d += 4)
+                        *reinterpret_cast<float4*>(&wo[warp][n8 + 8 * u][(2 * j + c) * NV + d]) =
+                            make_float4(o[t][d][2 * u + c], o[t][d + 1][2 * u + c], o[t][d + 2][2 * u + c], o[t][d + 3][2 * u + c]);
+            }
+            __syncthreads();
+            for (int i = tid; i < 16 * (HD / 8); i += kTreeThreads) {
+                const int r = i / (HD / 8), d0 = i % (HD / 8) * 8, row = 16 * t + r;
+                if (row >= have) continue;
+                float mx = -INFINITY, sum = 0.f, y[8] = {};
+                for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm[w][r]);
+                for (int w = 0; w < kTreeWarps; ++w) {
+                    const float f = wm[w][r] == -INFINITY ? (wl[w][r] == 0.f ? 0.f : 1.f) : exp2_fast(wm[w][r] - mx);
+                    sum = fmaf(f, wl[w][r], sum);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = fmaf(f, wo[w][r][d0 + e], y[e]);
+                }
+                if (whole) {
+                    const int nd = (row0 + row) / a.group, h = g * a.group + (row0 + row) % a.group;
+                    T* dst = (T*)a.out.p + s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : y[e] / sum);
+                    if (d0 == 0) {
+                        const float lg = sum == 0.f ? -INFINITY : mx - kPBias + log2f(sum);
+                        const size_t li = ((size_t)s * a.d.max_nodes + nd) * a.q_heads + h;
+                        if (a.lse) a.lse[li] = lg * 0.69314718055994531f;
+                        if (a.lse2) a.lse2[li] = lg;
+                    }
+                } else {
+                    float* dst = part + (size_t)row * (HD + 2);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dst[2 + d0 + e] = y[e];
+                    if (d0 == 0) dst[0] = mx, dst[1] = sum;
+                }
+            }
+            __syncthreads();
+        }
+        pos = unit_first + tile1;
+    }
+}
+
+// Adds the parts of the units that several CTAs worked on.  grid: (unit of the
+// largest batch, group of rows).
+constexpr int kJoinRows = 4;
+template <class T, int HD>
+__global__ void __launch_bounds__(kScanThreads) k_tree_join(TreeArgs a) {
+    __shared__ long long warp_sum[kScanThreads / 32];
+    __shared__ long long at_first;
+    __shared__ int at_seq;
+    const int tid = threadIdx.x;
+    const int per_seq = a.c.kv_heads * a.row_blocks, s = blockIdx.x / per_seq, unit = blockIdx.x % per_seq;
+    const Scan sc = scan_sequences(a, warp_sum, false);
+    {
+        long long f = sc.first;
+        for (int i = sc.s0; i < sc.s1; ++i) {
+            if (i == s) at_first = f, at_seq = i;
+            const SeqWork k = seq_work(a, i, false);
+            f += (long long)k.tiles * k.units;
+        }
+    }
+    __syncthreads();
+    const SeqWork k = seq_work(a, s, false);
+    if (unit >= k.units) return;
+    const long long u0 = at_first + (long long)unit * k.tiles, u1 = u0 + k.tiles;
+    // the CTA whose share holds a tile: shares are total * c / ctas, rounded down
+    auto cta_of = [&](long long t) {
+        int c = (int)((t * a.ctas) / sc.total);
+        while (c > 0 && share(sc.total, a.ctas, c) > t) --c;
+        while (share(sc.total, a.ctas, c + 1) <= t) ++c;
+        return c;
+    };
+    const int c0 = cta_of(u0), c1 = cta_of(u1 - 1);
+    if (c0 == c1) return;                                 // written by the CTA that had all of it
+    const int n = a.d.count(s), g = unit % a.c.kv_heads, row0 = unit / a.c.kv_heads * a.block_rows;
+    const int have = min(a.block_rows, n * a.group - row0);
+    for (int i = tid; i < kJoinRows * HD / 4; i += kScanThreads) {
+        const int row = blockIdx.y * kJoinRows + i / (HD / 4), d0 = i % (HD / 4) * 4;
+        if (row >= have) continue;
+        const size_t step = (size_t)a.block_rows * (HD + 2);
+        // the first CTA's part begins the unit (slot 1), the others' are slot 0
+        auto part = [&](int c) { return a.parts + (size_t)(2 * c + (c == c0 ? 1 : 0)) * step + (size_t)row * (HD + 2); };
+        float mx = -INFINITY;
+        for (int c = c0; c <= c1; ++c)
+            if (share(sc.total, a.ctas, c) < share(sc.total, a.ctas, c + 1)) mx = fmaxf(mx, part(c)[0]);
+        float sum = 0.f, y[4] = {};
+        for (int c = c0; c <= c1; ++c) {
+            if (share(sc.total, a.ctas, c) >= share(sc.total, a.ctas, c + 1)) continue;
+            const float* p = part(c);
+            const float f = p[0] == -INFINITY ? (p[1] == 0.f ? 0.f : 1.f) : exp2_fast(p[0] - mx);
+            sum = fmaf(f, p[1], sum);
+            for (int e = 0; e < 4; ++e) y[e] = fmaf(f, p[2 + d0 + e], y[e]);
+        }
+        const int nd = (row0 + row) / a.group, h = g * a.group + (row0 + row) % a.group;
+        T* dst = (T*)a.out.p + s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
+        for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : y[e] / sum);
+        if (d0 == 0) {
+            const float lg = sum == 0.f ? -INFINITY : mx - kPBias + log2f(sum);
+            const size_t li = ((size_t)s * a.d.max_nodes + nd) * a.q_heads + h;
+            if (a.lse) a.lse[li] = lg * 0.69314718055994531f;
+            if (a.lse2) a.lse2[li] = lg;
+        }
+    }
+}
+
+// ---- what each cache row got ---------------------------------------------------
+
+// mass[t] += sum over the sequence's query rows of 2^(s_t - lse).  A warp owns
+// 16 cache rows of a tile and goes through all query rows of all KV heads, so
+// the sum has one order and no atomics.
+template <class T, int HD, int NT>
+__global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
+    constexpr int QS = HD + 8;
+    __shared__ __align__(16) __half qs[NT * 16 * QS];
+    __shared__ float qfac[16];
+    __shared__ long long warp_sum[kScanThreads / 32];
+    __shared__ int at_seq, clash;
+    __shared__ long long at_first;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
+    // shares here are of tiles alone, one "unit" a sequence
+    const int per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
+    const int s0 = min(a.d.seqs, tid * per), s1 = min(a.d.seqs, s0 + per);
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) mine += seq_work(a, s, false).tiles;
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += t;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    __syncthreads();
+    long long first = inc - mine, total = 0;
+    for (int i = 0; i < kScanThreads / 32; ++i) {
+        if (i < warp) first += warp_sum[i];
+        total += warp_sum[i];
+    }
+    for (long long at = blockIdx.x; at < total; at += gridDim.x) {
+        __syncthreads();
+        if (tid == 0) clash = 0;
+        long long f = first;
+        for (int s = s0; s < s1; ++s) {
+            const int t = seq_work(a, s, false).tiles;
+            if (at >= f && at < f + t) at_seq = s, at_first = f;
+            f += t;
+        }
+        __syncthreads();
+        const int s = at_seq, slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
+        for (int i = tid; i < a.d.seqs; i += kTreeThreads)
+            if (i != s && a.d.slots[i] == slot && seq_work(a, i, false).tiles) clash = 1;
+        const int r0 = (int)(at - at_first) * kTile + 16 * warp, last = len + n - 1;
+        const size_t base_row = (size_t)slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
+        float got[4] = {};
+        for (int g = 0; g < a.c.kv_heads; ++g) {
+            KvRegs<HD> kv;
+            load_kv<HD>(a, base_row, min(r0, last), last, g, kv);
+            for (int row0 = 0; row0 < n * a.group; row0 += 16) {
+                const int have = min(16, n * a.group - row0);
+                __syncthreads();
+                stage_queries<T, HD, NT>(a, s, g, row0, 16, have, qs, QS, 16 * QS, qfac);
+                __syncthreads();
+                float acc[2][4];
+                dot_keys<HD, NT>(qs, QS, 16 * QS, kv, acc);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int r = n8 + 8 * u;
+                    if (r >= have) continue;
+                    const int node = (row0 + r) / a.group, h = g * a.group + (row0 + r) % a.group;
+                    const size_t li = (size_t)s * a.d.max_nodes + node;
+                    const unsigned long long* mrow = a.mask ? a.mask + li * a.words : nullptr;
+                    const float lg = a.lse2[li * a.q_heads + h];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int t = r0 + 4 * j + i;
+                        if (t <= last && sees(a, mrow, node, t, len, n))
+                            got[i] += exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * qfac[r], kv.ks[i], -lg));
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (clash) {
+            if (tid == 0 && a.status) atomicOr(a.status, QX_CUDA_STATUS_SHARED);
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            got[i] += __shfl_xor_sync(~0u, got[i], 4);
+            got[i] += __shfl_xor_sync(~0u, got[i], 8);
+            got[i] += __shfl_xor_sync(~0u, got[i], 16);
+            const int t = r0 + 4 * j + i;
+            if (n8 == 0 && t <= last) a.mass[base_row + t] += got[i];
+        }
+    }
+}
+
+// ---- host side -----------------------------------------------------------------
+
+constexpr int kMaxCtas = 148 * 8;
+
+struct Plan {
+    int block_rows, row_blocks, mt;
+    uint64_t parts, lse2;            // bytes
+};
+Plan plan_of(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim) {
+    Plan p{};
+    const uint32_t group = q_heads / kv_heads;
+    p.mt = 1;
+    p.block_rows = 16 * p.mt;
+    p.row_blocks = (int)(((uint64_t)max_nodes * group + p.block_rows - 1) / p.block_rows);
+    p.parts = (uint64_t)2 * kMaxCtas * p.block_rows * (head_dim + 2) * 4;
+    p.lse2 = (uint64_t)seqs * max_nodes * q_heads * 4;
+    return p;
+}
+
+const char* check_shape(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t dtype) {
+    if (head_dim != 64 && head_dim != 128) return "tree attention needs head_dim 64 or 128";
+    if (!kv_heads || kv_heads > kMaxHeads || !q_heads || q_heads > kMaxHeads || q_heads % kv_heads)
+        return "q_heads must be a multiple of kv_heads, at most 1024";
+    if (dtype > QX_CUDA_BF16) return "unsupported element type";
+    return nullptr;
+}
+
+template <class T, int HD, int NT, int MT>
+cudaError_t run_small(TreeArgs& a, int sms, cudaStream_t st) {
+    int per = 0;
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_tree_small<T, HD, NT, MT>, kTreeThreads, 0);
+    if (e != cudaSuccess) return e;
+    a.ctas = sms * (per < 1 ? 1 : per);
+    if (a.ctas > kMaxCtas) a.ctas = kMaxCtas;
+    k_tree_small<T, HD, NT, MT><<<a.ctas, kTreeThreads, 0, st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)(a.d.seqs * a.c.kv_heads * a.row_blocks), (unsigned)((a.block_rows + kJoinRows - 1) / kJoinRows));
+    k_tree_join<T, HD><<<grid, kScanThreads, 0, st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !a.mass) return e;
+    k_tree_mass<T, HD, NT><<<sms * 4, kTreeThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <class T, int NT>
+cudaError_t run_tree(TreeArgs& a, int sms, cudaStream_t st) {
+    return a.c.head_dim == 128 ? run_small<T, 128, NT, 1>(a, sms, st) : run_small<T, 64, NT, 1>(a, sms, st);
+}
+
+}  // namespace
+
+QX_API int qx_cuda_tree_attention_workspace(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_heads,
+                                            uint32_t head_dim, uint32_t dtype, uint64_t* bytes, char* err, uint64_t n) {
+    if (!bytes) return refuse(err, n, "invalid workspace argument");
+    if (!seqs || seqs > kMaxSeqs || !max_nodes || max_nodes > kMaxNodes)
+        return refuse(err, n, "at least one and at most 4096 sequences and nodes");
+    if (const char* m = check_shape(q_heads, kv_heads, head_dim, dtype)) return refuse(err, n, m);
+    const Plan p = plan_of(seqs, max_nodes, q_heads, kv_heads, head_dim);
+    *bytes = (p.parts + p.lse2 + 255) / 256 * 256;
+    return 1;
+}
+
+QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer, const qx_cuda_drafts* drafts,
+                                  uint32_t dtype, uint32_t q_heads, const qx_cuda_heads* q, const qx_cuda_heads* out,
+                                  const uint64_t* mask, float scale, float* lse, float* mass, void* workspace,
+                                  uint64_t workspace_bytes, uint32_t* status, void* stream, char* err, uint64_t n) {
+    const char* m = check_cache(cache);
+    if (!m) m = check_drafts(drafts);
+    if (!m) m = check_shape(q_heads, cache->kv_heads, cache->head_dim, dtype);
+    if (!m) m = check_heads(q, drafts->seqs, drafts->max_nodes, q_heads, cache->head_dim, dtype, false);
+    if (!m) m = check_heads(out, drafts->seqs, drafts->max_nodes, q_heads, cache->head_dim, dtype, true);
+    if (m) return refuse(err, n, m);
+    if (layer >= cache->layers) return refuse(err, n, "layer outside the cache");
+    if (!std::isfinite(scale)) return refuse(err, n, "the score scale must be finite");
+    if (!aligned(mask, 8)) return refuse(err, n, "the mask must be 8-byte aligned");
+    if (!aligned(lse, 4) || !aligned(mass, 4) || !aligned(status, 4))
+        return refuse(err, n, "lse, mass and status must be 4-byte aligned");
+    const Plan p = plan_of(drafts->seqs, drafts->max_nodes, q_heads, cache->kv_heads, cache->head_dim);
+    const uint64_t need = (p.parts + p.lse2 + 255) / 256 * 256;
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+        return refuse(err, n, "the workspace is missing, misaligned or too small");
+    const uint64_t join = (uint64_t)drafts->seqs * cache->kv_heads * p.row_blocks;
+    if (join > 0x7fffffffull) return refuse(err, n, "more row blocks than a launch holds");
+    DeviceOf dev(cache->k, err, n);
+    if (!dev.ok) return 0;
+    TreeArgs a{};
+    a.c = cache_of(cache);
+    a.d = drafts_of(drafts);
+    a.layer = (int)layer;
+    a.q_heads = (int)q_heads;
+    a.group = (int)(q_heads / cache->kv_heads);
+    a.block_rows = p.block_rows;
+    a.row_blocks = p.row_blocks;
+    a.q = {q->data, (size_t)q->seq_stride, (size_t)q->node_stride, (size_t)q->head_stride};
+    a.out = {out->data, (size_t)out->seq_stride, (size_t)out->node_stride, (size_t)out->head_stride};
+    a.mask = (const unsigned long long*)mask;
+    a.words = (int)((drafts->max_nodes + 63) / 64);
+    a.scale = scale;
+    a.lse = lse;
+    a.mass = mass;
+    a.parts = (float*)workspace;
+    a.lse2 = mass ? (float*)((uint8_t*)workspace + p.parts) : nullptr;
+    a.status = status;
+    int id = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&id);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, id);
+    if (e != cudaSuccess) return finish(e, err, n);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == QX_CUDA_F32) e = run_tree<float, 2>(a, sms, st);
+    else if (dtype == QX_CUDA_F16) e = run_tree<__half, 1>(a, sms, st);
+    else e = run_tree<__nv_bfloat16, 1>(a, sms, st);
+    return finish(e, err, n);
+}
