@@ -3,12 +3,14 @@
 Tolerances (each derived where it is used): u(t) = finfo(t).eps / 2 is the
 largest relative error of one rounding to t.
 """
+import ctypes as C
 import math
 
 import numpy as np
 import pytest
 import torch
 
+import opsabi
 import qxlib
 import qxops
 
@@ -600,11 +602,11 @@ def test_pick_tokens_of_a_large_vocabulary_and_history():
 
 def test_pick_without_output():
     x = torch.randn(3, 777, device=DEV)
-    args = qxops._Pick(x.data_ptr(), None, 777, 0, 3, 777, 0, 0, 0, 0, *([None] * 9), 0, 0, 0, 0)
+    args = opsabi.Pick(x.data_ptr(), None, 777, 0, 3, 777, 0, 0, 0, 0, *([None] * 9), 0, 0, 0, 0)
     tok = torch.zeros(3, dtype=torch.int32, device=DEV)
     args.picked = tok.data_ptr()
-    import ctypes as C
-    qxops._call(qxops._cuda().qx_cuda_pick_tokens, C.byref(args), torch.cuda.current_stream().cuda_stream)
+    err = qxlib.err_buf()
+    assert opsabi.lib().qx_cuda_pick_tokens(C.byref(args), torch.cuda.current_stream().cuda_stream, err, len(err)), err.value
     assert torch.equal(tok.long(), x.argmax(-1))
 
 

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-import qxlib
+import opsabi
 import qxops
 
 BASE = 1 << 20            # a 16-byte aligned address that nobody reads
@@ -18,17 +18,17 @@ def cache(**over):
     c = dict(k=BASE, v=BASE, k_scales=BASE, v_scales=BASE, slot_rows=200, layer_rows=100, slots=3, layers=2, ctx_tokens=100,
              kv_heads=2, head_dim=64, reserved=0)
     c.update(over)
-    return qxops._Cache(*(c[f] for f, _ in qxops._Cache._fields_))
+    return opsabi.Cache(*(c[f] for f, _ in opsabi.Cache._fields_))
 
 
 def drafts(**over):
     d = dict(seqs=2, max_nodes=3, slots=BASE, lens=BASE, nodes=None)
     d.update(over)
-    return qxops._Drafts(*(d[f] for f, _ in qxops._Drafts._fields_))
+    return opsabi.Drafts(*(d[f] for f, _ in opsabi.Drafts._fields_))
 
 
 def heads(data=BASE, seq=3 * 4 * 64, node=4 * 64, head=64):
-    return qxops._Heads(data, seq, node, head)
+    return opsabi.Heads(data, seq, node, head)
 
 
 def said(fn, *args):
@@ -39,11 +39,11 @@ def said(fn, *args):
 
 def rope(c=None, layer=0, d=None, freq=BASE, amplitude=1.0, rd=64, dtype=0, qh=4, q=None, qo=None, k=None, v=None,
          positions=None, status=None, no_q=False, no_kv=False):
-    r = qxops._Rotary(freq, amplitude, rd, 0)
+    r = opsabi.Rotary(freq, amplitude, rd, 0)
     ref = lambda x: None if x is None else C.byref(x)  # noqa: E731
     q, qo = (None, None) if no_q else (q or heads(), qo or heads())
     k, v = (None, None) if no_kv else (k or heads(), v or heads())
-    return said(qxops._cuda().qx_cuda_rope_append, C.byref(c or cache()), layer, C.byref(d or drafts()), C.byref(r), dtype, qh,
+    return said(opsabi.lib().qx_cuda_rope_append, C.byref(c or cache()), layer, C.byref(d or drafts()), C.byref(r), dtype, qh,
                 ref(q), ref(qo), ref(k), ref(v), positions, status, None)
 
 
@@ -81,7 +81,7 @@ def test_rope_append_refusals(args, message):
 
 def tree(c=None, layer=0, d=None, dtype=0, qh=4, q=None, out=None, mask=None, scale=0.1, lse=None, mass=None, work=BASE,
          size=1 << 40, status=None):
-    return said(qxops._cuda().qx_cuda_tree_attention, C.byref(c or cache()), layer, C.byref(d or drafts()), dtype, qh,
+    return said(opsabi.lib().qx_cuda_tree_attention, C.byref(c or cache()), layer, C.byref(d or drafts()), dtype, qh,
                 C.byref(q or heads()), C.byref(out or heads()), mask, scale, lse, mass, work, size, status, None)
 
 
@@ -108,7 +108,7 @@ def test_tree_attention_refusals(args, message):
 
 def evict(c=None, seqs=2, slots=BASE, dst=None, lens=BASE, mass=BASE, budget=8, sink=2, recent=2, kept=BASE, new=BASE + 64,
           status=None):
-    return said(qxops._cuda().qx_cuda_kv_evict, C.byref(c or cache()), seqs, slots, dst, lens, mass, budget, sink, recent, kept,
+    return said(opsabi.lib().qx_cuda_kv_evict, C.byref(c or cache()), seqs, slots, dst, lens, mass, budget, sink, recent, kept,
                 new, status, None)
 
 
@@ -133,8 +133,8 @@ def pick(**over):
              reserved=0, history=BASE, history_lens=None, repetition=None, frequency=None, presence=None, bias_ids=None,
              bias_lens=None, bias_values=None, allowed=None, history_stride=4, bias_stride=4, allowed_stride=32, picked=BASE)
     p.update(over)
-    a = qxops._Pick(*(p[f] for f, _ in qxops._Pick._fields_))
-    return said(qxops._cuda().qx_cuda_pick_tokens, C.byref(a), None)
+    a = opsabi.Pick(*(p[f] for f, _ in opsabi.Pick._fields_))
+    return said(opsabi.lib().qx_cuda_pick_tokens, C.byref(a), None)
 
 
 @pytest.mark.parametrize("args,message", [
@@ -157,7 +157,7 @@ def test_pick_refusals(args, message):
 
 
 def test_workspace_sizes_and_refusals():
-    f = qxops._cuda().qx_cuda_tree_attention_workspace
+    f = opsabi.lib().qx_cuda_tree_attention_workspace
     b = C.c_uint64()
     assert said(f, 1, 1, 32, 4, 128, 0, C.byref(b))[0] == 1 and b.value > 0 and b.value % 16 == 0
     small = b.value
@@ -225,8 +225,7 @@ def test_python_handles_check_tensors():
     c = qxops.KvCache(kt, kt, st, st)
     assert (c.c.slot_rows, c.c.layer_rows) == (8, 16)
     for bad in (lambda: qxops.KvCache(k.float(), k, s, s), lambda: qxops.KvCache(k, k, s[..., :4], s),
-                lambda: qxops.KvCache(k[..., :32], k[..., :32], s, s), lambda: qxops.KvCache(k, k, st.transpose(0, 1)[:, :, ::2], s),
-                lambda: c.mass_ptr(torch.zeros(2, 3, 4))):
+                lambda: qxops.KvCache(k[..., :32], k[..., :32], s, s), lambda: qxops.KvCache(k, k, st.transpose(0, 1)[:, :, ::2], s)):
         with pytest.raises(ValueError):
             bad()
 
@@ -238,11 +237,11 @@ def test_host_memory_is_refused():
     one = torch.zeros(1, dtype=torch.int32)
     c = qxops.KvCache(k, k.clone(), s, s.clone())
     kept, new = torch.zeros(4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
-    ok, msg = said(qxops._cuda().qx_cuda_kv_evict, c.ref, 1, one.data_ptr(), None, one.data_ptr(), s.data_ptr(), 4, 0, 0,
+    ok, msg = said(opsabi.lib().qx_cuda_kv_evict, C.byref(c.c), 1, one.data_ptr(), None, one.data_ptr(), s.data_ptr(), 4, 0, 0,
                    kept.data_ptr(), new.data_ptr(), None, None)
     assert ok == 0 and msg
 
 
 def test_view_refusals():
-    ok, msg = said(qxops._cuda().qx_cuda_kv_view, None, 0, None)
+    ok, msg = said(opsabi.lib().qx_cuda_kv_view, None, 0, None)
     assert (ok, msg) == (0, "invalid cache view argument")
