@@ -246,6 +246,7 @@ int qx_cuda_final_head_noalloc(const float *residual_dev, const float *norm_weig
 
 #define QX_CUDA_STATUS_RANGE  0x1u   /* slot, length or nodes outside the cache */
 #define QX_CUDA_STATUS_SHARED 0x2u   /* a slot written by a call is also another sequence's */
+#define QX_CUDA_STATUS_TIMEOUT 0x4u  /* a kernel's internal wait ran out (2 s): outputs are incomplete */
 
 /* An INT8 cache: the codes of row r of layer l of slot s are the
  * kv_heads * head_dim bytes at row s * slot_rows + l * layer_rows + r of k and

@@ -1,144 +1,22 @@
-// Attention of drafted tokens over the INT8 cache (qx_cuda_tree_attention).
-//
-// For a query row q (one node, one head) and cache row t with codes k_t, v_t
-// and scales ks_t, vs_t:
-//     s_t = scale ks_t (q . k_t),   o = sum_t e^(s_t) vs_t v_t / sum_t e^(s_t).
-// In base 2 and with the value scale inside the exponent,
-//     x_t = s_t log2(e) + log2(vs_t),   P_t = 2^(x_t - m + 14),   m = max x_t,
-//     o = sum_t P_t v_t / sum_t (P_t / vs_t):
-// what meets the codes v_t in the second product is one F16 number in
-// (0, 2^14] per (row, t) whatever the scales are, and the running maximum of
-// x_t is the only thing the accumulators are ever rescaled by.
-//
-// INT8 codes are exact in F16, so both products run on the tensor cores as F16
-// with F32 accumulation.  F16 and BF16 queries are one F16 term: a row is
-// multiplied by a power of two that puts its largest value in [2^13, 2^14)
-// (BF16 values more than 2^38 below it lose bits).  F32 queries, and P_t then too,
-// are two F16 terms (hi + the rest, 22 bits).  Everything else is F32.
-//
-// Work is cut into units (sequence, KV head, block of rows) and those into
-// tiles of 64 cache rows; the tiles of all units, laid end to end, are shared
-// out evenly over the CTAs.  A CTA that has all of a unit's tiles writes its
-// rows; parts of a unit go to the workspace as (m, sum, o) and
-// k_tree_join adds them in the order of their tiles.
+// Attention of drafted tokens over the INT8 cache (qx_cuda_tree_attention):
+// the entry point, the kernel for small trees, the joining of parts, and the
+// weights each cache row got.  The mathematics and the cut of the work are in
+// qx_tree.cuh, the kernel for larger trees in qx_tree_tc.cu.
 #include <cmath>
 
-#include "qx_ops.cuh"
+#include "qx_tree.cuh"
 
 namespace {
 
 using namespace qx::ops;
 
-constexpr int kTreeThreads = 128, kTreeWarps = 4, kTile = 64;
-constexpr int kScanThreads = 128;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPBias = 14.f;            // P_t = 2^(x_t - m + 14): 2^-24 / 2^14 is the smallest step of an F16 P_t
-constexpr float kMinLogVs = -90.f;        // value scales below 2^-90 count as that: 2^14 2^90 times 65536 rows still fits the F32 sum
-
-struct Tensor {
-    void* p;
-    size_t seq, node, head;
-};
-
-struct TreeArgs {
-    Cache c;
-    Drafts d;
-    int layer, q_heads, group, block_rows, row_blocks;   // row_blocks: of max_nodes * group rows
-    Tensor q, out;
-    int wide;                                             // 16-byte accesses to q and out
-    const unsigned long long* mask;
-    int words;
-    float scale;
-    float* lse;                                           // caller's, or null
-    float* lse2;                                          // workspace: base-2 log sums, for the mass
-    float* mass;
-    float* parts;                                         // [2 * ctas][block_rows][head_dim + 2]
-    int ctas;
-    uint32_t* status;
-};
-
-// ---- which tiles are whose -----------------------------------------------------
-
-// A sequence's share of the work: units of `tiles` tiles each, `units` of them.
-struct SeqWork {
-    int tiles, units;
-};
-__device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool report) {
-    const int slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
-    if (!fits(a.c, a.d, slot, len, n)) {
-        if (report && a.status) atomicOr(a.status, QX_CUDA_STATUS_RANGE);
-        return {0, 0};
-    }
-    if (n == 0) return {0, 0};
-    return {(len + n + kTile - 1) / kTile, a.c.kv_heads * ((n * a.group + a.block_rows - 1) / a.block_rows)};
-}
-
-// Prefix sums of the sequences' tiles, held by the threads of a CTA: thread t
-// has the sequences [t * per, (t + 1) * per).
-struct Scan {
-    long long first, total;      // tiles before this thread's sequences, and in all
-    int s0, s1;
-};
-__device__ __forceinline__ Scan scan_sequences(const TreeArgs& a, long long* warp_sum, bool report) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
-    Scan r;
-    r.s0 = min(a.d.seqs, (int)threadIdx.x * per);
-    r.s1 = min(a.d.seqs, r.s0 + per);
-    long long mine = 0;
-    for (int s = r.s0; s < r.s1; ++s) {
-        const SeqWork k = seq_work(a, s, report);
-        mine += (long long)k.tiles * k.units;
-    }
-    long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(~0u, inc, o);
-        if (lane >= o) inc += t;
-    }
-    if (lane == 31) warp_sum[w] = inc;
-    __syncthreads();
-    long long base = 0, total = 0;
-    for (int i = 0; i < kScanThreads / 32; ++i) {
-        if (i < w) base += warp_sum[i];
-        total += warp_sum[i];
-    }
-    r.first = base + inc - mine;
-    r.total = total;
-    return r;
-}
-__device__ __forceinline__ long long share(long long total, int ctas, int c) { return total * c / ctas; }
-
-// ---- F16 operands --------------------------------------------------------------
-
-// Four INT8 codes as F16: b + 128 as the low byte of 0x64xx is 1024 + b + 128,
-// and subtracting 1152 is exact.
-__device__ __forceinline__ uint32_t sub1152(uint32_t x) {
-    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t low_pair(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4140)); }
-__device__ __forceinline__ uint32_t high_pair(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4342)); }
-
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-// The pair minus its F16 rounding, as F16.
-__device__ __forceinline__ uint32_t rest_half(float a, float b, uint32_t hi) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    return pack_half(a - f.x, b - f.y);
-}
+constexpr int kTreeThreads = 128, kTreeWarps = 4;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 template <class T>
@@ -223,14 +101,6 @@ __device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qter
     }
 }
 
-// Which of a query row's node's keys a thread may see: row t of the sequence.
-__device__ __forceinline__ bool sees(const TreeArgs& a, const unsigned long long* mrow, int node, int t, int len, int n) {
-    if (t < len) return true;
-    const int b = t - len;
-    if (b >= n) return false;
-    return mrow ? (mrow[b >> 6] >> (b & 63)) & 1ull : b <= node;
-}
-
 // Stage `rows` query rows (from row0 on, `have` of them real) as F16 terms and
 // the factor that undoes their power of two; whole CTA.
 template <class T, int HD, int NT>
@@ -253,157 +123,111 @@ __device__ __forceinline__ void stage_queries(const TreeArgs& a, int s, int g, i
             for (int i = 0; i < HD / 32; ++i) x[i] = 0.f;
         }
         for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
-        // exponent e with big in [2^e, 2^(e+1)): times 2^(13 - e), in two exact steps
-        const int e = big > 0.f ? ilogbf(big) : 0;
-        const int up = 13 - e, u0 = up / 2;
-        const float f0 = __uint_as_float((uint32_t)(127 + u0) << 23), f1 = __uint_as_float((uint32_t)(127 + up - u0) << 23);
+        const RowScale rs(big);
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
-            const float y = x[i] * f0 * f1;
+            const float y = x[i] * rs.f0 * rs.f1;
             const __half hi = __float2half_rn(y);
             qs[r * qstride + lane + 32 * i] = hi;
             if (NT == 2) qs[qterm + r * qstride + lane + 32 * i] = __float2half_rn(y - __half2float(hi));
         }
-        if (lane == 0) qfac[r] = ldexpf(a.scale * kLog2e, -up);
+        if (lane == 0) qfac[r] = rs.undo(a.scale);
     }
 }
 
 // ---- the kernel for small trees ------------------------------------------------
 
-// MT blocks of 16 query rows; each of the 4 warps takes 16 of a tile's 64
-// cache rows, straight from global memory into the registers of the products
-// (the next tile's while this one is computed), keeps its own m, sum and o,
-// and the four are joined when the unit's part ends.
-template <class T, int HD, int NT, int MT>
+// Blocks of 16 query rows; each of the 4 warps takes 16 of a tile's 64 cache
+// rows, straight from global memory into the registers of the products (the
+// next tile's while this one is computed), keeps its own m, sum and o, and the
+// four are joined when the unit's part ends.
+template <class T, int HD, int NT>
 __global__ void __launch_bounds__(kTreeThreads) k_tree_small(TreeArgs a) {
-    constexpr int BM = 16 * MT, QS = HD + 8, NV = HD / 8;
+    constexpr int BM = 16, QS = HD + 8, NV = HD / 8;
     __shared__ __align__(16) __half qs[NT * BM * QS];
     __shared__ float qfac[BM];
-    __shared__ float wm[kTreeWarps][16], wl[kTreeWarps][16];
-    __shared__ __align__(16) float wo[kTreeWarps][16][HD + 4];
-    __shared__ long long warp_sum[kScanThreads / 32];
-    __shared__ int at_seq;
-    __shared__ long long at_first;
+    __shared__ float wm[kTreeWarps][BM], wl[kTreeWarps][BM];
+    __shared__ __align__(16) float wo[kTreeWarps][BM][HD + 4];
+    __shared__ ScanShared scan;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
-    const Scan sc = scan_sequences(a, warp_sum, blockIdx.x == 0);
-    const long long begin = share(sc.total, a.ctas, blockIdx.x), end = share(sc.total, a.ctas, blockIdx.x + 1);
-    if (begin >= end) return;
-    {   // the sequence that holds tile `begin`
-        long long f = sc.first;
-        for (int s = sc.s0; s < sc.s1; ++s) {
-            const SeqWork k = seq_work(a, s, false);
-            const long long t = (long long)k.tiles * k.units;
-            if (begin >= f && begin < f + t) at_seq = s, at_first = f;
-            f += t;
-        }
-    }
-    __syncthreads();
-    int s = at_seq;
-    long long seq_first = at_first;
-    SeqWork k = seq_work(a, s, false);
-    long long pos = begin;
-    while (pos < end) {
-        while (pos >= seq_first + (long long)k.tiles * k.units) {
-            seq_first += (long long)k.tiles * k.units;
-            k = seq_work(a, ++s, false);
-        }
-        const int slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
-        const int unit = (int)((pos - seq_first) / k.tiles), tile0 = (int)((pos - seq_first) % k.tiles);
-        const long long unit_first = seq_first + (long long)unit * k.tiles;
-        const int tile1 = (int)min((long long)k.tiles, end - unit_first);
-        const int g = unit % a.c.kv_heads, row0 = unit / a.c.kv_heads * BM, have = min(BM, n * a.group - row0);
-        const size_t base_row = (size_t)slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
-        const int last = len + n - 1;
-        // in a chain no row of this block sees past its last node
-        const int limit = a.mask ? len + n : min(len + n, len + (row0 + have - 1) / a.group + 1);
+    Cursor cur;
+    if (!begin_share(a, scan, cur)) return;
+    Piece p;
+    while (cur.next(a, p)) {
+        const int last = p.len + p.n - 1, stop = p.tile1 * kTile;
         KvRegs<HD> kv;
-        int r0 = tile0 * kTile + 16 * warp;
-        if (r0 < min(limit, tile1 * kTile)) load_kv<HD>(a, base_row, r0, last, g, kv);
-        stage_queries<T, HD, NT>(a, s, g, row0, BM, have, qs, QS, BM * QS, qfac);
+        int r0 = p.tile0 * kTile + 16 * warp;
+        if (r0 < stop) load_kv<HD>(a, p.base_row, r0, last, p.g, kv);
+        stage_queries<T, HD, NT>(a, p.s, p.g, p.row0, BM, p.have, qs, QS, BM * QS, qfac);
         __syncthreads();
-        float m[MT][2], l[MT][2], o[MT][NV][4], fac[MT][2];
-        const unsigned long long* mrow[MT][2];
-        int node[MT][2];
+        float m[2], l[2], o[NV][4], fac[2];
+        const unsigned long long* mrow[2];
+        int node[2];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int r = 16 * t + n8 + 8 * u;
-                m[t][u] = -INFINITY, l[t][u] = 0.f;
-                fac[t][u] = qfac[r];
-                node[t][u] = r < have ? (row0 + r) / a.group : -1;
-                mrow[t][u] = a.mask && r < have ? a.mask + ((size_t)s * a.d.max_nodes + node[t][u]) * a.words : nullptr;
-            }
-#pragma unroll
-            for (int d = 0; d < NV; ++d) o[t][d][0] = o[t][d][1] = o[t][d][2] = o[t][d][3] = 0.f;
+        for (int u = 0; u < 2; ++u) {
+            const int r = n8 + 8 * u;
+            m[u] = -INFINITY, l[u] = 0.f;
+            fac[u] = qfac[r];
+            node[u] = r < p.have ? (p.row0 + r) / a.group : -1;
+            mrow[u] = a.mask && r < p.have ? a.mask + ((size_t)p.s * a.d.max_nodes + node[u]) * a.words : nullptr;
         }
-        for (; r0 < min(limit, tile1 * kTile); r0 += kTile) {
+#pragma unroll
+        for (int d = 0; d < NV; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+        for (; r0 < stop; r0 += kTile) {
             float ks[4], lv[4], iv[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                ks[i] = kv.ks[i];
-                lv[i] = fmaxf(__log2f(kv.vs[i]), kMinLogVs);
-                if (!(kv.vs[i] >= 0.f)) lv[i] = __int_as_float(0x7fc00000);
-                iv[i] = kv.vs[i] > 0x1p-90f ? __frcp_rn(kv.vs[i]) : 0x1p90f;
+            for (int i = 0; i < 4; ++i) ks[i] = kv.ks[i], lv[i] = log_vs(kv.vs[i]), iv[i] = inv_vs(kv.vs[i]);
+            const bool edge = r0 + 16 > p.len;
+            float acc[2][4];
+            dot_keys<HD, NT>(qs, QS, BM * QS, kv, acc);
+            // acc[h][2 u + c]: query row n8 + 8 u, cache row r0 + 4 j + 2 h + c
+            float x[2][4], up[2];
+            bool grew = false;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[u][i] = fmaf(acc[i >> 1][2 * u + (i & 1)] * fac[u], ks[i], lv[i]);
+                    if (edge && (node[u] < 0 || !sees(mrow[u], node[u], r0 + 4 * j + i, p.len, p.n))) x[u][i] = -INFINITY;
+                }
+                float mx = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
+                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+                up[u] = mx > m[u] + kSlack || m[u] == -INFINITY ? fmaxf(mx, m[u]) : m[u];
+                grew |= up[u] > m[u];
             }
-            const bool edge = r0 + 16 > len;
-            uint32_t p[MT][NT][4];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                float acc[2][4];
-                dot_keys<HD, NT>(qs + 16 * t * QS, QS, BM * QS, kv, acc);
-                // acc[h][2 u + c]: query row n8 + 8 u, cache row r0 + 4 j + 2 h + c
-                float x[2][4];
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[u][i] = fmaf(acc[i >> 1][2 * u + (i & 1)] * fac[t][u], ks[i], lv[i]);
-                        if (edge && (node[t][u] < 0 || !sees(a, mrow[t][u], node[t][u], r0 + 4 * j + i, len, n)))
-                            x[u][i] = -INFINITY;
-                    }
-                float up[2];
-                bool grew = false;
+            if (__any_sync(~0u, grew)) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    float mx = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
-                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-                    up[u] = fmaxf(mx, m[t][u]);
-                    grew |= up[u] > m[t][u];
+                    const float f = up[u] > m[u] ? exp2_fast(m[u] - up[u]) : 1.f;
+                    l[u] *= f;
+#pragma unroll
+                    for (int d = 0; d < NV; ++d) o[d][2 * u] *= f, o[d][2 * u + 1] *= f;
+                    m[u] = up[u];
                 }
-                if (__any_sync(~0u, grew)) {
+            }
+            uint32_t w[NT][4];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float f = up[u] > m[t][u] ? exp2_fast(m[t][u] - up[u]) : 1.f;
-                        l[t][u] *= f;
+            for (int u = 0; u < 2; ++u) {
+                const float ref = m[u] == -INFINITY ? 0.f : m[u] - kPBias;
+                float e[4];
 #pragma unroll
-                        for (int d = 0; d < NV; ++d) o[t][d][2 * u] *= f, o[t][d][2 * u + 1] *= f;
-                        m[t][u] = up[u];
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    e[i] = exp2_fast(x[u][i] - ref);
+                    l[u] = fmaf(e[i], iv[i], l[u]);
                 }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float ref = m[t][u] == -INFINITY ? 0.f : m[t][u] - kPBias;
-                    float e[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        e[i] = exp2_fast(x[u][i] - ref);
-                        l[t][u] = fmaf(x[u][i] == -INFINITY ? 0.f : e[i], x[u][i] == -INFINITY ? 0.f : iv[i], l[t][u]);
-                    }
-                    p[t][0][u] = pack_half(e[0], e[1]);
-                    p[t][0][2 + u] = pack_half(e[2], e[3]);
-                    if (NT == 2) {
-                        p[t][NT - 1][u] = rest_half(e[0], e[1], p[t][0][u]);
-                        p[t][NT - 1][2 + u] = rest_half(e[2], e[3], p[t][0][2 + u]);
-                    }
+                w[0][u] = pack_half(e[0], e[1]);
+                w[0][2 + u] = pack_half(e[2], e[3]);
+                if (NT == 2) {
+                    w[NT - 1][u] = rest_half(e[0], e[1], w[0][u]);
+                    w[NT - 1][2 + u] = rest_half(e[2], e[3], w[0][2 + u]);
                 }
             }
             // values: dims (lane / 4) * NV + d of rows 4 j .. 4 j + 3 are column lane / 4 of value tile d
 #pragma unroll
-            for (int w = 0; w < HD / 32; ++w) {
-                const uint32_t v0 = kv.v[0][w] ^ 0x80808080u, v1 = kv.v[1][w] ^ 0x80808080u,
-                               v2 = kv.v[2][w] ^ 0x80808080u, v3 = kv.v[3][w] ^ 0x80808080u;
+            for (int v = 0; v < HD / 32; ++v) {
+                const uint32_t v0 = kv.v[0][v] ^ 0x80808080u, v1 = kv.v[1][v] ^ 0x80808080u,
+                               v2 = kv.v[2][v] ^ 0x80808080u, v3 = kv.v[3][v] ^ 0x80808080u;
                 const uint32_t a0 = __byte_perm(v0, v1, 0x5140), a1 = __byte_perm(v0, v1, 0x7362);
                 const uint32_t c0 = __byte_perm(v2, v3, 0x5140), c1 = __byte_perm(v2, v3, 0x7362);
                 const uint32_t b0[4] = {low_pair(a0), high_pair(a0), low_pair(a1), high_pair(a1)};
@@ -411,63 +235,51 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_small(TreeArgs a) {
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
-                    for (int t = 0; t < MT; ++t)
-#pragma unroll
-                        for (int q = 0; q < NT; ++q) mma16816(o[t][4 * w + d], p[t][q], b0[d], b1[d]);
+                    for (int q = 0; q < NT; ++q) mma16816(o[4 * v + d], w[q], b0[d], b1[d]);
             }
-            if (r0 + kTile < min(limit, tile1 * kTile)) load_kv<HD>(a, base_row, r0 + kTile, last, g, kv);
+            if (r0 + kTile < stop) load_kv<HD>(a, p.base_row, r0 + kTile, last, p.g, kv);
         }
-        // join the four warps, block of 16 rows by block
-        const bool whole = tile0 == 0 && tile1 == k.tiles;
-        float* part = a.parts + (size_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * BM * (HD + 2);
+        // join the four warps
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
+        for (int u = 0; u < 2; ++u) {
+            l[u] += __shfl_xor_sync(~0u, l[u], 1);
+            l[u] += __shfl_xor_sync(~0u, l[u], 2);
+            if (j == 0) wm[warp][n8 + 8 * u] = m[u], wl[warp][n8 + 8 * u] = l[u];
+            // columns 2 j, 2 j + 1 of value tile d are dims 2 j NV + d and (2 j + 1) NV + d
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                l[t][u] += __shfl_xor_sync(~0u, l[t][u], 1);
-                l[t][u] += __shfl_xor_sync(~0u, l[t][u], 2);
-                if (j == 0) wm[warp][n8 + 8 * u] = m[t][u], wl[warp][n8 + 8 * u] = l[t][u];
-                // columns 2 j, 2 j + 1 of value tile d are dims 2 j NV + d and (2 j + 1) NV + d
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int d = 0; d < NV; d += 4)
-                        *reinterpret_cast<float4*>(&wo[warp][n8 + 8 * u][(2 * j + c) * NV + d]) =
-                            make_float4(o[t][d][2 * u + c], o[t][d + 1][2 * u + c], o[t][d + 2][2 * u + c], o[t][d + 3][2 * u + c]);
-            }
-            __syncthreads();
-            for (int i = tid; i < 16 * (HD / 8); i += kTreeThreads) {
-                const int r = i / (HD / 8), d0 = i % (HD / 8) * 8, row = 16 * t + r;
-                if (row >= have) continue;
-                float mx = -INFINITY, sum = 0.f, y[8] = {};
-                for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm[w][r]);
-                for (int w = 0; w < kTreeWarps; ++w) {
-                    const float f = wm[w][r] == -INFINITY ? (wl[w][r] == 0.f ? 0.f : 1.f) : exp2_fast(wm[w][r] - mx);
-                    sum = fmaf(f, wl[w][r], sum);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = fmaf(f, wo[w][r][d0 + e], y[e]);
-                }
-                if (whole) {
-                    const int nd = (row0 + row) / a.group, h = g * a.group + (row0 + row) % a.group;
-                    T* dst = (T*)a.out.p + s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : y[e] / sum);
-                    if (d0 == 0) {
-                        const float lg = sum == 0.f ? -INFINITY : mx - kPBias + log2f(sum);
-                        const size_t li = ((size_t)s * a.d.max_nodes + nd) * a.q_heads + h;
-                        if (a.lse) a.lse[li] = lg * 0.69314718055994531f;
-                        if (a.lse2) a.lse2[li] = lg;
-                    }
-                } else {
-                    float* dst = part + (size_t)row * (HD + 2);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[2 + d0 + e] = y[e];
-                    if (d0 == 0) dst[0] = mx, dst[1] = sum;
-                }
-            }
-            __syncthreads();
+                for (int d = 0; d < NV; d += 4)
+                    *reinterpret_cast<float4*>(&wo[warp][n8 + 8 * u][(2 * j + c) * NV + d]) =
+                        make_float4(o[d][2 * u + c], o[d + 1][2 * u + c], o[d + 2][2 * u + c], o[d + 3][2 * u + c]);
         }
-        pos = unit_first + tile1;
+        __syncthreads();
+        float* part = part_of(a, blockIdx.x, p.begins);
+        for (int i = tid; i < BM * (HD / 8); i += kTreeThreads) {
+            const int r = i / (HD / 8), d0 = i % (HD / 8) * 8;
+            if (r >= p.have) continue;
+            float mx = -INFINITY, sum = 0.f, y[8] = {};
+            for (int w = 0; w < kTreeWarps; ++w) mx = fmaxf(mx, wm[w][r]);
+            for (int w = 0; w < kTreeWarps; ++w) {
+                const float f = part_weight(wm[w][r], wl[w][r], mx);
+                sum = fmaf(f, wl[w][r], sum);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = fmaf(f, wo[w][r][d0 + e], y[e]);
+            }
+            if (p.whole) {
+                const int nd = (p.row0 + r) / a.group, h = p.g * a.group + (p.row0 + r) % a.group;
+                T* dst = (T*)a.out.p + p.s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : y[e] / sum);
+                if (d0 == 0) write_lse(a, p.s, nd, h, mx, sum);
+            } else {
+                float* dst = part + (size_t)r * (kPartHead + HD);
+                *reinterpret_cast<float4*>(dst + kPartHead + d0) = make_float4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<float4*>(dst + kPartHead + d0 + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                if (d0 == 0) dst[0] = mx, dst[1] = sum;
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -476,61 +288,63 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_small(TreeArgs a) {
 constexpr int kJoinRows = 4;
 template <class T, int HD>
 __global__ void __launch_bounds__(kScanThreads) k_tree_join(TreeArgs a) {
-    __shared__ long long warp_sum[kScanThreads / 32];
-    __shared__ long long at_first;
-    __shared__ int at_seq;
     const int tid = threadIdx.x;
     const int per_seq = a.c.kv_heads * a.row_blocks, s = blockIdx.x / per_seq, unit = blockIdx.x % per_seq;
-    const Scan sc = scan_sequences(a, warp_sum, false);
-    {
-        long long f = sc.first;
-        for (int i = sc.s0; i < sc.s1; ++i) {
-            if (i == s) at_first = f, at_seq = i;
-            const SeqWork k = seq_work(a, i, false);
-            f += (long long)k.tiles * k.units;
-        }
-    }
-    __syncthreads();
     const SeqWork k = seq_work(a, s, false);
-    if (unit >= k.units) return;
-    const long long u0 = at_first + (long long)unit * k.tiles, u1 = u0 + k.tiles;
-    // the CTA whose share holds a tile: shares are total * c / ctas, rounded down
+    const int n = a.d.count(s), g = unit % a.c.kv_heads, row0 = unit / a.c.kv_heads * a.block_rows;
+    const int have = min(a.block_rows, n * a.group - row0);
+    if (unit >= k.units || (int)blockIdx.y * kJoinRows >= have) return;
+    // tiles before sequence s, and in all
+    long long before = 0, total = 0;
+    {
+        const int lane = tid & 31, w = tid >> 5;
+        long long b = 0, t = 0;
+        for (int i = tid; i < a.d.seqs; i += kScanThreads) {
+            const long long all = seq_work(a, i, false).all();
+            t += all;
+            b += i < s ? all : 0;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            b += __shfl_xor_sync(~0u, b, o);
+            t += __shfl_xor_sync(~0u, t, o);
+        }
+        __shared__ long long sb[kScanThreads / 32], st[kScanThreads / 32];
+        if (lane == 0) sb[w] = b, st[w] = t;
+        __syncthreads();
+        for (int i = 0; i < kScanThreads / 32; ++i) before += sb[i], total += st[i];
+    }
+    const long long u0 = before + (long long)unit * k.tiles, u1 = u0 + k.tiles;
+    const int busy = busy_ctas(a, total);
+    // the CTA whose share holds a tile: shares are total * c / busy, rounded down, and none is empty
     auto cta_of = [&](long long t) {
-        int c = (int)((t * a.ctas) / sc.total);
-        while (c > 0 && share(sc.total, a.ctas, c) > t) --c;
-        while (share(sc.total, a.ctas, c + 1) <= t) ++c;
+        int c = (int)((t * busy) / total);
+        while (c > 0 && share(total, busy, c) > t) --c;
+        while (share(total, busy, c + 1) <= t) ++c;
         return c;
     };
     const int c0 = cta_of(u0), c1 = cta_of(u1 - 1);
     if (c0 == c1) return;                                 // written by the CTA that had all of it
-    const int n = a.d.count(s), g = unit % a.c.kv_heads, row0 = unit / a.c.kv_heads * a.block_rows;
-    const int have = min(a.block_rows, n * a.group - row0);
     for (int i = tid; i < kJoinRows * HD / 4; i += kScanThreads) {
         const int row = blockIdx.y * kJoinRows + i / (HD / 4), d0 = i % (HD / 4) * 4;
         if (row >= have) continue;
-        const size_t step = (size_t)a.block_rows * (HD + 2);
-        // the first CTA's part begins the unit (slot 1), the others' are slot 0
-        auto part = [&](int c) { return a.parts + (size_t)(2 * c + (c == c0 ? 1 : 0)) * step + (size_t)row * (HD + 2); };
+        auto part = [&](int c) { return part_of(a, c, c == c0) + (size_t)row * (kPartHead + HD); };
         float mx = -INFINITY;
-        for (int c = c0; c <= c1; ++c)
-            if (share(sc.total, a.ctas, c) < share(sc.total, a.ctas, c + 1)) mx = fmaxf(mx, part(c)[0]);
-        float sum = 0.f, y[4] = {};
+        for (int c = c0; c <= c1; ++c) mx = fmaxf(mx, part(c)[0]);
+        float sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int c = c0; c <= c1; ++c) {
-            if (share(sc.total, a.ctas, c) >= share(sc.total, a.ctas, c + 1)) continue;
             const float* p = part(c);
-            const float f = p[0] == -INFINITY ? (p[1] == 0.f ? 0.f : 1.f) : exp2_fast(p[0] - mx);
+            const float f = part_weight(p[0], p[1], mx);
+            const float4 v = *reinterpret_cast<const float4*>(p + kPartHead + d0);
             sum = fmaf(f, p[1], sum);
-            for (int e = 0; e < 4; ++e) y[e] = fmaf(f, p[2 + d0 + e], y[e]);
+            y = make_float4(fmaf(f, v.x, y.x), fmaf(f, v.y, y.y), fmaf(f, v.z, y.z), fmaf(f, v.w, y.w));
         }
         const int nd = (row0 + row) / a.group, h = g * a.group + (row0 + row) % a.group;
         T* dst = (T*)a.out.p + s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
-        for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : y[e] / sum);
-        if (d0 == 0) {
-            const float lg = sum == 0.f ? -INFINITY : mx - kPBias + log2f(sum);
-            const size_t li = ((size_t)s * a.d.max_nodes + nd) * a.q_heads + h;
-            if (a.lse) a.lse[li] = lg * 0.69314718055994531f;
-            if (a.lse2) a.lse2[li] = lg;
-        }
+        const float z[4] = {y.x, y.y, y.z, y.w};
+        for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : z[e] / sum);
+        if (d0 == 0) write_lse(a, s, nd, h, mx, sum);
     }
 }
 
@@ -603,7 +417,7 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int t = r0 + 4 * j + i;
-                        if (t <= last && sees(a, mrow, node, t, len, n))
+                        if (t <= last && sees(mrow, node, t, len, n))
                             got[i] += exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * qfac[r], kv.ks[i], -lg));
                     }
                 }
@@ -627,19 +441,18 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
 
 // ---- host side -----------------------------------------------------------------
 
-constexpr int kMaxCtas = 148 * 8;
-
 struct Plan {
-    int block_rows, row_blocks, mt;
+    bool tc;                         // blocks of 128 rows on tcgen05
+    int block_rows, row_blocks;
     uint64_t parts, lse2;            // bytes
 };
 Plan plan_of(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim) {
     Plan p{};
-    const uint32_t group = q_heads / kv_heads;
-    p.mt = 1;
-    p.block_rows = 16 * p.mt;
-    p.row_blocks = (int)(((uint64_t)max_nodes * group + p.block_rows - 1) / p.block_rows);
-    p.parts = (uint64_t)2 * kMaxCtas * p.block_rows * (head_dim + 2) * 4;
+    const uint64_t rows = (uint64_t)max_nodes * (q_heads / kv_heads);
+    p.tc = rows > 32;
+    p.block_rows = p.tc ? 128 : 16;
+    p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
+    p.parts = (uint64_t)2 * (p.tc ? kMaxCtas / 8 : kMaxCtas) * p.block_rows * (kPartHead + head_dim) * 4;
     p.lse2 = (uint64_t)seqs * max_nodes * q_heads * 4;
     return p;
 }
@@ -652,15 +465,20 @@ const char* check_shape(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, 
     return nullptr;
 }
 
-template <class T, int HD, int NT, int MT>
-cudaError_t run_small(TreeArgs& a, int sms, cudaStream_t st) {
-    int per = 0;
-    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_tree_small<T, HD, NT, MT>, kTreeThreads, 0);
-    if (e != cudaSuccess) return e;
-    a.ctas = sms * (per < 1 ? 1 : per);
-    if (a.ctas > kMaxCtas) a.ctas = kMaxCtas;
-    k_tree_small<T, HD, NT, MT><<<a.ctas, kTreeThreads, 0, st>>>(a);
-    e = cudaGetLastError();
+template <class T, int HD, int NT>
+cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t st) {
+    cudaError_t e;
+    if (tc) {
+        e = launch_tree_tc(a, type, sms, st);
+    } else {
+        int per = 0;
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_tree_small<T, HD, NT>, kTreeThreads, 0);
+        if (e != cudaSuccess) return e;
+        a.ctas = sms * (per < 1 ? 1 : per);
+        if (a.ctas > kMaxCtas) a.ctas = kMaxCtas;
+        k_tree_small<T, HD, NT><<<a.ctas, kTreeThreads, 0, st>>>(a);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)(a.d.seqs * a.c.kv_heads * a.row_blocks), (unsigned)((a.block_rows + kJoinRows - 1) / kJoinRows));
     k_tree_join<T, HD><<<grid, kScanThreads, 0, st>>>(a);
@@ -671,8 +489,8 @@ cudaError_t run_small(TreeArgs& a, int sms, cudaStream_t st) {
 }
 
 template <class T, int NT>
-cudaError_t run_tree(TreeArgs& a, int sms, cudaStream_t st) {
-    return a.c.head_dim == 128 ? run_small<T, 128, NT, 1>(a, sms, st) : run_small<T, 64, NT, 1>(a, sms, st);
+cudaError_t run_tree(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t st) {
+    return a.c.head_dim == 128 ? run_typed<T, 128, NT>(a, tc, type, sms, st) : run_typed<T, 64, NT>(a, tc, type, sms, st);
 }
 
 }  // namespace
@@ -729,13 +547,17 @@ QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer,
     a.parts = (float*)workspace;
     a.lse2 = mass ? (float*)((uint8_t*)workspace + p.parts) : nullptr;
     a.status = status;
+    const uint64_t step = 16 / elem_bytes(dtype);
+    a.wide = aligned(q->data, 16) && aligned(out->data, 16) && q->seq_stride % step == 0 && q->node_stride % step == 0 &&
+             q->head_stride % step == 0 && out->seq_stride % step == 0 && out->node_stride % step == 0 &&
+             out->head_stride % step == 0;
     int id = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&id);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, id);
     if (e != cudaSuccess) return finish(e, err, n);
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == QX_CUDA_F32) e = run_tree<float, 2>(a, sms, st);
-    else if (dtype == QX_CUDA_F16) e = run_tree<__half, 1>(a, sms, st);
-    else e = run_tree<__nv_bfloat16, 1>(a, sms, st);
+    if (dtype == QX_CUDA_F32) e = run_tree<float, 2>(a, p.tc, dtype, sms, st);
+    else if (dtype == QX_CUDA_F16) e = run_tree<__half, 1>(a, p.tc, dtype, sms, st);
+    else e = run_tree<__nv_bfloat16, 1>(a, p.tc, dtype, sms, st);
     return finish(e, err, n);
 }

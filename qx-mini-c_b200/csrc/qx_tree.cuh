@@ -1,0 +1,275 @@
+// What the kernels of qx_cuda_tree_attention share (qx_tree.cu, qx_tree_tc.cu):
+// the mathematics, how the work is cut and shared out, and F16 operands.
+//
+// For a query row q (one node, one head) and cache row t with codes k_t, v_t
+// and scales ks_t, vs_t:
+//     s_t = scale ks_t (q . k_t),   o = sum_t e^(s_t) vs_t v_t / sum_t e^(s_t).
+// In base 2 and with the value scale inside the exponent,
+//     x_t = s_t log2(e) + log2(vs_t),   P_t = 2^(x_t - m + 8),   m >= max x_t - 7,
+//     o = sum_t P_t v_t / sum_t (P_t / vs_t):
+// what meets the codes v_t in the second product is one F16 number in
+// (0, 2^15] per (row, t) whatever the scales are, and the running reference m
+// is the only thing the accumulators are ever rescaled by.
+//
+// INT8 codes are exact in F16, so both products run on the tensor cores as F16
+// with F32 accumulation.  F16 and BF16 queries are one F16 term: a row is
+// multiplied by a power of two that puts its largest value in [2^13, 2^14)
+// (BF16 values more than 2^38 below it lose bits).  F32 queries, and P_t then
+// too, are two F16 terms (hi + the rest, 22 bits).  Everything else is F32.
+//
+// Work is cut into units (sequence, KV head, block of rows) and those into
+// tiles of 64 cache rows; the tiles of all units, laid end to end, are shared
+// out evenly over the CTAs.  A CTA that has all of a unit's tiles writes its
+// rows; parts of a unit go to the workspace as (m, sum, o) and k_tree_join
+// adds them in the order of their tiles.
+#pragma once
+#include "qx_ops.cuh"
+
+namespace qx {
+namespace ops {
+
+constexpr int kTile = 64;                 // cache rows
+constexpr int kScanThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kPBias = 8.f;
+constexpr float kSlack = 7.f;             // how far x_t may pass the reference: P_t <= 2^15, and F16 ends at 2^16
+constexpr float kMinLogVs = -90.f;        // value scales below 2^-90 count as that: 2^15 2^90 times 65536 rows still fits the F32 sum
+constexpr int kPartHead = 4;              // floats of a part's row before its o: m, sum, two unused (16-byte rows)
+constexpr int kMaxCtas = 148 * 8;
+
+struct Tensor {
+    void* p;
+    size_t seq, node, head;
+};
+
+struct TreeArgs {
+    Cache c;
+    Drafts d;
+    int layer, q_heads, group, block_rows, row_blocks;   // row_blocks: of max_nodes * group rows
+    Tensor q, out;
+    int wide;                                             // q and out allow 16-byte accesses
+    const unsigned long long* mask;
+    int words;
+    float scale;
+    float* lse;                                           // caller's, or null
+    float* lse2;                                          // workspace: base-2 log sums, for the mass
+    float* mass;
+    float* parts;                                         // [2 * ctas][block_rows][kPartHead + head_dim]
+    int ctas;
+    uint32_t* status;
+};
+
+// The tensor-core kernel for blocks of 128 query rows (qx_tree_tc.cu).
+// type: QX_CUDA_F32, F16 or BF16; sets a.ctas.
+cudaError_t launch_tree_tc(TreeArgs& a, uint32_t type, int sms, cudaStream_t st);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- which tiles are whose -----------------------------------------------------
+
+// A sequence's share of the work: `units` units of `tiles` tiles each.
+struct SeqWork {
+    int tiles, units;
+    __device__ __forceinline__ long long all() const { return (long long)tiles * units; }
+};
+__device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool report) {
+    const int slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
+    if (!fits(a.c, a.d, slot, len, n)) {
+        if (report && a.status) atomicOr(a.status, QX_CUDA_STATUS_RANGE);
+        return {0, 0};
+    }
+    if (n == 0) return {0, 0};
+    return {(len + n + kTile - 1) / kTile, a.c.kv_heads * ((n * a.group + a.block_rows - 1) / a.block_rows)};
+}
+
+// CTAs that get work: never more than there are tiles.
+__device__ __forceinline__ int busy_ctas(const TreeArgs& a, long long total) { return (int)min((long long)a.ctas, total); }
+__device__ __forceinline__ long long share(long long total, int ctas, int c) { return total * c / ctas; }
+
+// Shared memory of a CTA's look at the sequences.
+struct ScanShared {
+    long long warp_sum[kScanThreads / 32], at_first, total;
+    int at_seq;
+};
+// The sequence that holds tile `want(total)` and the tiles before it, in
+// sh; whole CTA, the first 128 threads hold the sequences.  Returns the tiles
+// of all sequences.
+template <class Want>
+__device__ __forceinline__ long long scan_sequences(const TreeArgs& a, ScanShared& sh, bool report, Want want) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
+    const bool scans = threadIdx.x < kScanThreads;
+    const int s0 = scans ? min(a.d.seqs, (int)threadIdx.x * per) : 0, s1 = scans ? min(a.d.seqs, s0 + per) : 0;
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) mine += seq_work(a, s, report).all();
+    long long inc = mine;
+    if (scans) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(~0u, inc, o);
+            if (lane >= o) inc += t;
+        }
+        if (lane == 31) sh.warp_sum[w] = inc;
+    }
+    __syncthreads();
+    long long first = inc - mine, total = 0;
+    for (int i = 0; i < kScanThreads / 32; ++i) {
+        if (i < w) first += sh.warp_sum[i];
+        total += sh.warp_sum[i];
+    }
+    const long long at = want(total);
+    for (int s = s0; s < s1; ++s) {
+        const long long t = seq_work(a, s, false).all();
+        if (at >= first && at < first + t) sh.at_seq = s, sh.at_first = first;
+        first += t;
+    }
+    __syncthreads();
+    return total;
+}
+
+// One unit's tiles that a CTA has.
+struct Piece {
+    int s, slot, len, n, g, row0, have;    // rows row0 .. row0 + have of KV head g
+    int tile0, tile1;                      // tiles; none (tile1 <= tile0) where no row of the block sees them
+    bool begins, whole;
+    size_t base_row;
+};
+struct Cursor {
+    long long pos, end, seq_first;
+    int s;
+    SeqWork k;
+    __device__ __forceinline__ bool next(const TreeArgs& a, Piece& p) {
+        if (pos >= end) return false;
+        while (pos >= seq_first + k.all()) {
+            seq_first += k.all();
+            k = seq_work(a, ++s, false);
+        }
+        const int unit = (int)((pos - seq_first) / k.tiles);
+        const long long first = seq_first + (long long)unit * k.tiles;
+        p.s = s;
+        p.slot = a.d.slots[s], p.len = a.d.lens[s], p.n = a.d.count(s);
+        p.g = unit % a.c.kv_heads;
+        p.row0 = unit / a.c.kv_heads * a.block_rows;
+        p.have = min(a.block_rows, p.n * a.group - p.row0);
+        p.tile0 = (int)(pos - first);
+        p.tile1 = (int)min((long long)k.tiles, end - first);
+        p.begins = p.tile0 == 0;
+        p.whole = p.begins && p.tile1 == k.tiles;
+        p.base_row = (size_t)p.slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
+        pos = first + p.tile1;
+        // in a chain no row of the block sees past its last node
+        const int limit = a.mask ? p.len + p.n : min(p.len + p.n, p.len + (p.row0 + p.have - 1) / a.group + 1);
+        p.tile1 = min(p.tile1, (limit + kTile - 1) / kTile);
+        return true;
+    }
+};
+// This CTA's cursor; false where it has nothing to do.
+__device__ __forceinline__ bool begin_share(const TreeArgs& a, ScanShared& sh, Cursor& c) {
+    const long long total = scan_sequences(a, sh, blockIdx.x == 0, [&](long long t) {
+        const int busy = busy_ctas(a, t);
+        return (int)blockIdx.x < busy ? share(t, busy, blockIdx.x) : -1ll;
+    });
+    const int busy = busy_ctas(a, total);
+    if ((int)blockIdx.x >= busy) return false;
+    c.pos = share(total, busy, blockIdx.x);
+    c.end = share(total, busy, blockIdx.x + 1);
+    c.s = sh.at_seq;
+    c.seq_first = sh.at_first;
+    c.k = seq_work(a, c.s, false);
+    return true;
+}
+// Where the part of a piece goes: a CTA has at most one that ends a unit
+// begun elsewhere, and one that begins a unit.
+__device__ __forceinline__ float* part_of(const TreeArgs& a, int cta, bool begins) {
+    return a.parts + (size_t)(2 * cta + (begins ? 1 : 0)) * a.block_rows * (kPartHead + a.c.head_dim);
+}
+
+// ---- parts -----------------------------------------------------------------------
+
+// The factor of a part whose reference is m when parts are joined at mx; a
+// part that saw nothing has none, and one that met a NaN keeps it.
+__device__ __forceinline__ float part_weight(float m, float l, float mx) {
+    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2_fast(m - mx);
+}
+__device__ __forceinline__ void write_lse(const TreeArgs& a, int s, int node, int h, float m, float sum) {
+    const float lg = sum == 0.f ? -INFINITY : m - kPBias + log2f(sum);
+    const size_t li = ((size_t)s * a.d.max_nodes + node) * a.q_heads + h;
+    if (a.lse) a.lse[li] = lg * 0.69314718055994531f;
+    if (a.lse2) a.lse2[li] = lg;
+}
+
+// ---- operands ------------------------------------------------------------------
+
+// Four INT8 codes as F16: b + 128 as the low byte of 0x64xx is 1024 + b + 128,
+// and subtracting 1152 is exact.  `biased` holds b + 128 (b ^ 0x80).
+__device__ __forceinline__ uint32_t sub1152(uint32_t x) {
+    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t low_pair(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t high_pair(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4342)); }
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The pair minus its F16 rounding, as F16.
+__device__ __forceinline__ uint32_t rest_half(float a, float b, uint32_t hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    return pack_half(a - f.x, b - f.y);
+}
+// The power of two 2^up that puts `big` (the largest finite magnitude of a
+// row) in [2^13, 2^14), as two factors that are normal numbers.
+struct RowScale {
+    int up;
+    float f0, f1;
+    __device__ __forceinline__ explicit RowScale(float big) {
+        up = 13 - (big > 0.f ? ilogbf(big) : 0);
+        const int u0 = up / 2;
+        f0 = __uint_as_float((uint32_t)(127 + u0) << 23);
+        f1 = __uint_as_float((uint32_t)(127 + up - u0) << 23);
+    }
+    // what turns the integer dot product of scaled queries and codes into a base-2 score, but for ks_t
+    __device__ __forceinline__ float undo(float scale) const { return ldexpf(scale * kLog2e, -up); }
+};
+
+// log2(vs) for the exponent, and 1 / vs for the sum of weights.
+__device__ __forceinline__ float log_vs(float vs) {
+    return vs >= 0.f ? fmaxf(__log2f(vs), kMinLogVs) : __int_as_float(0x7fc00000);
+}
+__device__ __forceinline__ float inv_vs(float vs) { return vs > 0x1p-90f ? __frcp_rn(vs) : 0x1p90f; }
+
+// ---- visibility ----------------------------------------------------------------
+
+// Whether a node sees row t of its sequence (mrow: its mask words, or null).
+__device__ __forceinline__ bool sees(const unsigned long long* mrow, int node, int t, int len, int n) {
+    if (t < len) return true;
+    const int b = t - len;
+    if (b >= n) return false;
+    return mrow ? (mrow[b >> 6] >> (b & 63)) & 1ull : b <= node;
+}
+// The same for the 64 rows from t0 on, as bits.
+__device__ __forceinline__ unsigned long long sees64(const unsigned long long* mrow, int words, int node, int t0, int len,
+                                                     int n) {
+    const unsigned long long all = ~0ull;
+    auto first = [&](int c) { return c <= 0 ? 0ull : c >= 64 ? all : (1ull << c) - 1ull; };   // bits 0 .. c - 1
+    if (!mrow) return first(min(len + n, len + node + 1) - t0);
+    unsigned long long w;
+    if (t0 >= len) {
+        const int b = t0 - len, i = b >> 6, sh = b & 63;
+        w = i < words ? mrow[i] >> sh : 0ull;
+        if (sh && i + 1 < words) w |= mrow[i + 1] << (64 - sh);
+    } else {
+        const int c = len - t0;
+        w = c >= 64 ? all : first(c) | mrow[0] << c;
+    }
+    return w & first(len + n - t0);
+}
+#endif  // __CUDACC__
+
+}  // namespace ops
+}  // namespace qx

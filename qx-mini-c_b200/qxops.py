@@ -23,6 +23,7 @@ except ImportError as e:
 
 STATUS_RANGE = 0x1        # a sequence's slot, length or nodes lie outside the cache
 STATUS_SHARED = 0x2       # a slot written by a call is also another sequence's
+STATUS_TIMEOUT = 0x4      # a kernel's internal wait ran out: outputs are incomplete
 
 ROPE_SCHEMES = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
