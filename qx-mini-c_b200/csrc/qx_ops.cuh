@@ -150,6 +150,11 @@ inline Cache cache_of(const qx_cuda_kv_cache* c) {
             (int)c->layers, (int)c->ctx_tokens, (int)c->kv_heads, (int)c->head_dim};
 }
 
+// Rows from the first to the end of the last.
+inline size_t cache_rows(const Cache& c) {
+    return (size_t)(c.slots - 1) * c.slot_rows + (size_t)(c.layers - 1) * c.layer_rows + (size_t)c.ctx;
+}
+
 struct Drafts {
     int seqs, max_nodes;
     const int *slots, *lens, *nodes;

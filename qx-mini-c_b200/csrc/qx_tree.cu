@@ -142,18 +142,18 @@ __device__ __forceinline__ void stage_queries(const TreeArgs& a, int s, int g, i
 // next tile's while this one is computed), keeps its own m, sum and o, and the
 // four are joined when the unit's part ends.
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(kTreeThreads) k_tree_small(TreeArgs a) {
+__global__ void __launch_bounds__(kTreeThreads) k_tree_small(const __grid_constant__ TreeArgs a) {
     constexpr int BM = 16, QS = HD + 8, NV = HD / 8;
     __shared__ __align__(16) __half qs[NT * BM * QS];
     __shared__ float qfac[BM];
     __shared__ float wm[kTreeWarps][BM], wl[kTreeWarps][BM];
     __shared__ __align__(16) float wo[kTreeWarps][BM][HD + 4];
-    __shared__ ScanShared scan;
+    __shared__ PieceList list;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
-    Cursor cur;
-    if (!begin_share(a, scan, cur)) return;
-    Piece p;
-    while (cur.next(a, p)) {
+    int batch = 0, at = 0;
+    list_pieces(a, list, 0);
+    while (at < list.count) {
+        const Piece p = list.piece[at];
         const int last = p.len + p.n - 1, stop = p.tile1 * kTile;
         KvRegs<HD> kv;
         int r0 = p.tile0 * kTile + 16 * warp;
@@ -280,72 +280,45 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_small(TreeArgs a) {
             }
         }
         __syncthreads();
+        if (++at == list.count && list.more) {
+            __syncthreads();                             // everyone has read the counts
+            list_pieces(a, list, ++batch);
+            at = 0;
+        }
     }
 }
 
-// Adds the parts of the units that several CTAs worked on.  grid: (unit of the
-// largest batch, group of rows).
-constexpr int kJoinRows = 4;
+// Adds the parts of the units that several CTAs worked on, by the records
+// they left.  grid: (CTA of the kernel before, group of rows).
+constexpr int kJoinThreads = 128;
 template <class T, int HD>
-__global__ void __launch_bounds__(kScanThreads) k_tree_join(TreeArgs a) {
-    const int tid = threadIdx.x;
-    const int per_seq = a.c.kv_heads * a.row_blocks, s = blockIdx.x / per_seq, unit = blockIdx.x % per_seq;
-    const SeqWork k = seq_work(a, s, false);
-    const int n = a.d.count(s), g = unit % a.c.kv_heads, row0 = unit / a.c.kv_heads * a.block_rows;
-    const int have = min(a.block_rows, n * a.group - row0);
-    if (unit >= k.units || (int)blockIdx.y * kJoinRows >= have) return;
-    // tiles before sequence s, and in all
-    long long before = 0, total = 0;
-    {
-        const int lane = tid & 31, w = tid >> 5;
-        long long b = 0, t = 0;
-        for (int i = tid; i < a.d.seqs; i += kScanThreads) {
-            const long long all = seq_work(a, i, false).all();
-            t += all;
-            b += i < s ? all : 0;
-        }
+__global__ void __launch_bounds__(kJoinThreads) k_tree_join(const __grid_constant__ TreeArgs a) {
+    constexpr int kRows = kJoinThreads / (HD / 4);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before still runs
+    const Join j = a.joins[blockIdx.x];
+    const int row = blockIdx.y * kRows + threadIdx.x / (HD / 4), d0 = threadIdx.x % (HD / 4) * 4;
+    if (row >= (j.parts ? j.have : 0)) return;
+    // the first part begins the unit, the others are what their CTAs began with
+    auto part = [&](int i) { return part_of(a, blockIdx.x - 1 + i, i == 0) + (size_t)row * (kPartHead + HD); };
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < j.parts; ++i) mx = fmaxf(mx, part(i)[0]);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < j.parts; ++i) {
+        const float* p = part(i);
+        const float2 ml = *reinterpret_cast<const float2*>(p);
+        const float4 v = *reinterpret_cast<const float4*>(p + kPartHead + d0);
+        const float f = part_weight(ml.x, ml.y, mx);
+        sum = fmaf(f, ml.y, sum);
+        y = make_float4(fmaf(f, v.x, y.x), fmaf(f, v.y, y.y), fmaf(f, v.z, y.z), fmaf(f, v.w, y.w));
+    }
+    const int nd = (j.row0 + row) / a.group, h = j.g * a.group + (j.row0 + row) % a.group;
+    T* dst = (T*)a.out.p + j.s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
+    const float z[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            b += __shfl_xor_sync(~0u, b, o);
-            t += __shfl_xor_sync(~0u, t, o);
-        }
-        __shared__ long long sb[kScanThreads / 32], st[kScanThreads / 32];
-        if (lane == 0) sb[w] = b, st[w] = t;
-        __syncthreads();
-        for (int i = 0; i < kScanThreads / 32; ++i) before += sb[i], total += st[i];
-    }
-    const long long u0 = before + (long long)unit * k.tiles, u1 = u0 + k.tiles;
-    const int busy = busy_ctas(a, total);
-    // the CTA whose share holds a tile: shares are total * c / busy, rounded down, and none is empty
-    auto cta_of = [&](long long t) {
-        int c = (int)((t * busy) / total);
-        while (c > 0 && share(total, busy, c) > t) --c;
-        while (share(total, busy, c + 1) <= t) ++c;
-        return c;
-    };
-    const int c0 = cta_of(u0), c1 = cta_of(u1 - 1);
-    if (c0 == c1) return;                                 // written by the CTA that had all of it
-    for (int i = tid; i < kJoinRows * HD / 4; i += kScanThreads) {
-        const int row = blockIdx.y * kJoinRows + i / (HD / 4), d0 = i % (HD / 4) * 4;
-        if (row >= have) continue;
-        auto part = [&](int c) { return part_of(a, c, c == c0) + (size_t)row * (kPartHead + HD); };
-        float mx = -INFINITY;
-        for (int c = c0; c <= c1; ++c) mx = fmaxf(mx, part(c)[0]);
-        float sum = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = c0; c <= c1; ++c) {
-            const float* p = part(c);
-            const float f = part_weight(p[0], p[1], mx);
-            const float4 v = *reinterpret_cast<const float4*>(p + kPartHead + d0);
-            sum = fmaf(f, p[1], sum);
-            y = make_float4(fmaf(f, v.x, y.x), fmaf(f, v.y, y.y), fmaf(f, v.z, y.z), fmaf(f, v.w, y.w));
-        }
-        const int nd = (row0 + row) / a.group, h = g * a.group + (row0 + row) % a.group;
-        T* dst = (T*)a.out.p + s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
-        const float z[4] = {y.x, y.y, y.z, y.w};
-        for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : z[e] / sum);
-        if (d0 == 0) write_lse(a, s, nd, h, mx, sum);
-    }
+    for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : z[e] / sum);
+    if (d0 == 0) write_lse(a, j.s, nd, h, mx, sum);
 }
 
 // ---- what each cache row got ---------------------------------------------------
@@ -358,32 +331,30 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
     constexpr int QS = HD + 8;
     __shared__ __align__(16) __half qs[NT * 16 * QS];
     __shared__ float qfac[16];
-    __shared__ long long warp_sum[kScanThreads / 32];
-    __shared__ int at_seq, clash;
-    __shared__ long long at_first;
+    __shared__ int warp_sum[kScanThreads / 32], at_seq, at_first, clash;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
     // shares here are of tiles alone, one "unit" a sequence
     const int per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
     const int s0 = min(a.d.seqs, tid * per), s1 = min(a.d.seqs, s0 + per);
-    long long mine = 0;
+    int mine = 0;
     for (int s = s0; s < s1; ++s) mine += seq_work(a, s, false).tiles;
-    long long inc = mine;
+    int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(~0u, inc, o);
+        const int t = __shfl_up_sync(~0u, inc, o);
         if (lane >= o) inc += t;
     }
     if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
-    long long first = inc - mine, total = 0;
+    int first = inc - mine, total = 0;
     for (int i = 0; i < kScanThreads / 32; ++i) {
         if (i < warp) first += warp_sum[i];
         total += warp_sum[i];
     }
-    for (long long at = blockIdx.x; at < total; at += gridDim.x) {
+    for (int at = blockIdx.x; at < total; at += gridDim.x) {
         __syncthreads();
         if (tid == 0) clash = 0;
-        long long f = first;
+        int f = first;
         for (int s = s0; s < s1; ++s) {
             const int t = seq_work(a, s, false).tiles;
             if (at >= f && at < f + t) at_seq = s, at_first = f;
@@ -393,7 +364,7 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
         const int s = at_seq, slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
         for (int i = tid; i < a.d.seqs; i += kTreeThreads)
             if (i != s && a.d.slots[i] == slot && seq_work(a, i, false).tiles) clash = 1;
-        const int r0 = (int)(at - at_first) * kTile + 16 * warp, last = len + n - 1;
+        const int r0 = (at - at_first) * kTile + 16 * warp, last = len + n - 1;
         const size_t base_row = (size_t)slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
         float got[4] = {};
         for (int g = 0; g < a.c.kv_heads; ++g) {
@@ -444,7 +415,8 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
 struct Plan {
     bool tc;                         // blocks of 128 rows on tcgen05
     int block_rows, row_blocks;
-    uint64_t parts, lse2;            // bytes
+    uint64_t parts, joins, lse2;     // bytes of workspace
+    uint64_t all() const { return (parts + joins + lse2 + 255) / 256 * 256; }
 };
 Plan plan_of(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim) {
     Plan p{};
@@ -453,6 +425,7 @@ Plan plan_of(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_he
     p.block_rows = p.tc ? 128 : 16;
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
     p.parts = (uint64_t)2 * (p.tc ? kMaxCtas / 8 : kMaxCtas) * p.block_rows * (kPartHead + head_dim) * 4;
+    p.joins = (uint64_t)(kMaxCtas * sizeof(Join) + 255) / 256 * 256;
     p.lse2 = (uint64_t)seqs * max_nodes * q_heads * 4;
     return p;
 }
@@ -480,9 +453,17 @@ cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)(a.d.seqs * a.c.kv_heads * a.row_blocks), (unsigned)((a.block_rows + kJoinRows - 1) / kJoinRows));
-    k_tree_join<T, HD><<<grid, kScanThreads, 0, st>>>(a);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    constexpr int kRows = kJoinThreads / (HD / 4);
+    cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)(a.block_rows / kRows));
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_tree_join<T, HD>, a);
     if (e != cudaSuccess || !a.mass) return e;
     k_tree_mass<T, HD, NT><<<sms * 4, kTreeThreads, 0, st>>>(a);
     return cudaGetLastError();
@@ -502,7 +483,7 @@ QX_API int qx_cuda_tree_attention_workspace(uint32_t seqs, uint32_t max_nodes, u
         return refuse(err, n, "at least one and at most 4096 sequences and nodes");
     if (const char* m = check_shape(q_heads, kv_heads, head_dim, dtype)) return refuse(err, n, m);
     const Plan p = plan_of(seqs, max_nodes, q_heads, kv_heads, head_dim);
-    *bytes = (p.parts + p.lse2 + 255) / 256 * 256;
+    *bytes = p.all();
     return 1;
 }
 
@@ -522,11 +503,12 @@ QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer,
     if (!aligned(lse, 4) || !aligned(mass, 4) || !aligned(status, 4))
         return refuse(err, n, "lse, mass and status must be 4-byte aligned");
     const Plan p = plan_of(drafts->seqs, drafts->max_nodes, q_heads, cache->kv_heads, cache->head_dim);
-    const uint64_t need = (p.parts + p.lse2 + 255) / 256 * 256;
-    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < p.all())
         return refuse(err, n, "the workspace is missing, misaligned or too small");
-    const uint64_t join = (uint64_t)drafts->seqs * cache->kv_heads * p.row_blocks;
-    if (join > 0x7fffffffull) return refuse(err, n, "more row blocks than a launch holds");
+    const uint64_t tiles = ((uint64_t)cache->ctx_tokens + kTile - 1) / kTile;
+    if ((uint64_t)drafts->seqs * cache->kv_heads * p.row_blocks * tiles > 0x7fffffffull)
+        return refuse(err, n, "more rows and cache than one call can take");
+    if (cache_rows(cache_of(cache)) > 0x7fffffffull - kTile) return refuse(err, n, "the cache has more rows than the operator supports");
     DeviceOf dev(cache->k, err, n);
     if (!dev.ok) return 0;
     TreeArgs a{};
@@ -545,7 +527,8 @@ QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer,
     a.lse = lse;
     a.mass = mass;
     a.parts = (float*)workspace;
-    a.lse2 = mass ? (float*)((uint8_t*)workspace + p.parts) : nullptr;
+    a.joins = (Join*)((uint8_t*)workspace + p.parts);
+    a.lse2 = mass ? (float*)((uint8_t*)workspace + p.parts + p.joins) : nullptr;
     a.status = status;
     const uint64_t step = 16 / elem_bytes(dtype);
     a.wide = aligned(q->data, 16) && aligned(out->data, 16) && q->seq_stride % step == 0 && q->node_stride % step == 0 &&

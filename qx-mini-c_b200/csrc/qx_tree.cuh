@@ -42,6 +42,11 @@ struct Tensor {
     size_t seq, node, head;
 };
 
+// Parts to join: those of CTAs c - 1 .. c - 1 + parts - 1 (none: nothing to do), c the record's index.
+struct Join {
+    int parts, s, g, row0, have;
+};
+
 struct TreeArgs {
     Cache c;
     Drafts d;
@@ -55,6 +60,7 @@ struct TreeArgs {
     float* lse2;                                          // workspace: base-2 log sums, for the mass
     float* mass;
     float* parts;                                         // [2 * ctas][block_rows][kPartHead + head_dim]
+    Join* joins;                                          // [ctas]
     int ctas;
     uint32_t* status;
 };
@@ -72,10 +78,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 // ---- which tiles are whose -----------------------------------------------------
 
-// A sequence's share of the work: `units` units of `tiles` tiles each.
+// A sequence's share of the work: `units` units of `tiles` tiles each.  (The
+// host refuses calls whose tiles could pass 2^31.)
 struct SeqWork {
     int tiles, units;
-    __device__ __forceinline__ long long all() const { return (long long)tiles * units; }
+    __device__ __forceinline__ int all() const { return tiles * units; }
 };
 __device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool report) {
     const int slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
@@ -87,100 +94,126 @@ __device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool repor
     return {(len + n + kTile - 1) / kTile, a.c.kv_heads * ((n * a.group + a.block_rows - 1) / a.block_rows)};
 }
 
-// CTAs that get work: never more than there are tiles.
-__device__ __forceinline__ int busy_ctas(const TreeArgs& a, long long total) { return (int)min((long long)a.ctas, total); }
-__device__ __forceinline__ long long share(long long total, int ctas, int c) { return total * c / ctas; }
-
-// Shared memory of a CTA's look at the sequences.
-struct ScanShared {
-    long long warp_sum[kScanThreads / 32], at_first, total;
-    int at_seq;
+// The tiles of all units laid end to end, cut into shares that differ by one
+// tile at most; never more CTAs than tiles.
+struct Shares {
+    int busy, each, extra;
+    __device__ __forceinline__ Shares(const TreeArgs& a, int total) {
+        busy = min(a.ctas, total);
+        each = busy ? total / busy : 0;
+        extra = busy ? total - each * busy : 0;
+    }
+    __device__ __forceinline__ int begin(int c) const { return each * c + min(c, extra); }
+    // the CTA that has tile t
+    __device__ __forceinline__ int of(int t) const {
+        const int longer = extra * (each + 1);
+        return t < longer ? t / (each + 1) : extra + (t - longer) / each;
+    }
 };
-// The sequence that holds tile `want(total)` and the tiles before it, in
-// sh; whole CTA, the first 128 threads hold the sequences.  Returns the tiles
-// of all sequences.
-template <class Want>
-__device__ __forceinline__ long long scan_sequences(const TreeArgs& a, ScanShared& sh, bool report, Want want) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
-    const bool scans = threadIdx.x < kScanThreads;
-    const int s0 = scans ? min(a.d.seqs, (int)threadIdx.x * per) : 0, s1 = scans ? min(a.d.seqs, s0 + per) : 0;
-    long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += seq_work(a, s, report).all();
-    long long inc = mine;
-    if (scans) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long t = __shfl_up_sync(~0u, inc, o);
-            if (lane >= o) inc += t;
-        }
-        if (lane == 31) sh.warp_sum[w] = inc;
-    }
-    __syncthreads();
-    long long first = inc - mine, total = 0;
-    for (int i = 0; i < kScanThreads / 32; ++i) {
-        if (i < w) first += sh.warp_sum[i];
-        total += sh.warp_sum[i];
-    }
-    const long long at = want(total);
-    for (int s = s0; s < s1; ++s) {
-        const long long t = seq_work(a, s, false).all();
-        if (at >= first && at < first + t) sh.at_seq = s, sh.at_first = first;
-        first += t;
-    }
-    __syncthreads();
-    return total;
-}
 
 // One unit's tiles that a CTA has.
 struct Piece {
-    int s, slot, len, n, g, row0, have;    // rows row0 .. row0 + have of KV head g
+    size_t base_row;                       // the sequence's row 0 in the layer
+    int s, len, n, g, row0, have;          // query rows row0 .. row0 + have of KV head g
     int tile0, tile1;                      // tiles; none (tile1 <= tile0) where no row of the block sees them
-    bool begins, whole;
-    size_t base_row;
+    int begins, whole;
 };
-struct Cursor {
-    long long pos, end, seq_first;
-    int s;
-    SeqWork k;
-    __device__ __forceinline__ bool next(const TreeArgs& a, Piece& p) {
-        if (pos >= end) return false;
-        while (pos >= seq_first + k.all()) {
-            seq_first += k.all();
-            k = seq_work(a, ++s, false);
-        }
-        const int unit = (int)((pos - seq_first) / k.tiles);
-        const long long first = seq_first + (long long)unit * k.tiles;
-        p.s = s;
-        p.slot = a.d.slots[s], p.len = a.d.lens[s], p.n = a.d.count(s);
-        p.g = unit % a.c.kv_heads;
-        p.row0 = unit / a.c.kv_heads * a.block_rows;
-        p.have = min(a.block_rows, p.n * a.group - p.row0);
-        p.tile0 = (int)(pos - first);
-        p.tile1 = (int)min((long long)k.tiles, end - first);
-        p.begins = p.tile0 == 0;
-        p.whole = p.begins && p.tile1 == k.tiles;
-        p.base_row = (size_t)p.slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
-        pos = first + p.tile1;
-        // in a chain no row of the block sees past its last node
-        const int limit = a.mask ? p.len + p.n : min(p.len + p.n, p.len + (p.row0 + p.have - 1) / a.group + 1);
-        p.tile1 = min(p.tile1, (limit + kTile - 1) / kTile);
-        return true;
+// The pieces of a CTA, kList at a time: every thread of the first 128 looks at
+// its own sequences and writes down those units of theirs that the CTA's share
+// of the tiles meets, so that no one follows a chain of loads.
+constexpr int kList = 32;
+struct PieceList {
+    Piece piece[kList];
+    int tile_sum[kScanThreads / 32], unit_sum[kScanThreads / 32], first_unit;
+    int count, more;
+};
+// Fills the list with pieces batch * kList and on; whole CTA, and it must be
+// done with the pieces before.  The first batch also writes the CTA's join
+// record.  (Not inlined: instruction fetch is what kernels with several roles
+// run short of.)
+static __device__ __noinline__ void list_pieces(const TreeArgs& a, PieceList& sh, int batch) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
+    const bool scans = threadIdx.x < kScanThreads;
+    const int s0 = scans ? min(a.d.seqs, (int)threadIdx.x * per) : 0, s1 = scans ? min(a.d.seqs, s0 + per) : 0;
+    int tiles = 0, units = 0;
+    SeqWork one{0, 0};                                    // kept where a thread has one sequence
+    for (int s = s0; s < s1; ++s) {
+        one = seq_work(a, s, blockIdx.x == 0 && batch == 0);
+        tiles += one.all();
+        units += one.units;
     }
-};
-// This CTA's cursor; false where it has nothing to do.
-__device__ __forceinline__ bool begin_share(const TreeArgs& a, ScanShared& sh, Cursor& c) {
-    const long long total = scan_sequences(a, sh, blockIdx.x == 0, [&](long long t) {
-        const int busy = busy_ctas(a, t);
-        return (int)blockIdx.x < busy ? share(t, busy, blockIdx.x) : -1ll;
-    });
-    const int busy = busy_ctas(a, total);
-    if ((int)blockIdx.x >= busy) return false;
-    c.pos = share(total, busy, blockIdx.x);
-    c.end = share(total, busy, blockIdx.x + 1);
-    c.s = sh.at_seq;
-    c.seq_first = sh.at_first;
-    c.k = seq_work(a, c.s, false);
-    return true;
+    auto work = [&](int s) { return per == 1 ? one : seq_work(a, s, false); };
+    int tl = tiles, un = units;
+    if (scans) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(~0u, tl, o), u = __shfl_up_sync(~0u, un, o);
+            if (lane >= o) tl += t, un += u;
+        }
+        if (lane == 31) sh.tile_sum[w] = tl, sh.unit_sum[w] = un;
+    }
+    if (threadIdx.x == 0) {
+        sh.count = sh.more = 0;
+        if (batch == 0) a.joins[blockIdx.x].parts = 0;
+    }
+    __syncthreads();
+    int first = tl - tiles, unit0 = un - units, total = 0;
+#pragma unroll
+    for (int i = 0; i < kScanThreads / 32; ++i) {
+        if (i < w) first += sh.tile_sum[i], unit0 += sh.unit_sum[i];
+        total += sh.tile_sum[i];
+    }
+    const Shares cut(a, total);
+    const int c = blockIdx.x, begin = c < cut.busy ? cut.begin(c) : 0, end = c < cut.busy ? cut.begin(c + 1) : 0;
+    const bool meets = begin < end && first < end && first + tiles > begin;
+    if (meets && begin >= first) {                        // the unit that holds the share's first tile
+        int f = first, u = unit0;
+        for (int s = s0; s < s1; ++s) {
+            const SeqWork k = work(s);
+            if (begin >= f && begin < f + k.all()) sh.first_unit = u + (begin - f) / k.tiles;
+            f += k.all();
+            u += k.units;
+        }
+    }
+    __syncthreads();
+    if (meets)
+        for (int s = s0; s < s1; ++s) {
+            const SeqWork k = work(s);
+            if (k.units && first < end && first + k.all() > begin) {
+                const int u0 = begin > first ? (begin - first) / k.tiles : 0;
+                const int u1 = end < first + k.all() ? (end - first + k.tiles - 1) / k.tiles : k.units;
+                for (int u = u0; u < u1; ++u) {
+                    const int at = unit0 + u - sh.first_unit - batch * kList;
+                    if (at < 0) continue;
+                    if (at >= kList) {
+                        sh.more = 1;
+                        break;
+                    }
+                    const int f = first + u * k.tiles;
+                    Piece& p = sh.piece[at];
+                    p.s = s;
+                    p.len = a.d.lens[s], p.n = a.d.count(s);
+                    p.g = u % a.c.kv_heads;
+                    p.row0 = u / a.c.kv_heads * a.block_rows;
+                    p.have = min(a.block_rows, p.n * a.group - p.row0);
+                    p.tile0 = max(begin, f) - f;
+                    p.tile1 = min(k.tiles, end - f);
+                    p.begins = p.tile0 == 0;
+                    p.whole = p.begins && p.tile1 == k.tiles;
+                    p.base_row = (size_t)a.d.slots[s] * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
+                    // of the CTAs that share a unit, the second sees to its joining
+                    if (at == 0 && batch == 0 && !p.begins && cut.begin(c - 1) <= f)
+                        a.joins[c] = {cut.of(f + k.tiles - 1) - c + 2, s, p.g, p.row0, p.have};
+                    // in a chain no row of the block sees past its last node
+                    const int limit = a.mask ? p.len + p.n : min(p.len + p.n, p.len + (p.row0 + p.have - 1) / a.group + 1);
+                    p.tile1 = min(p.tile1, (limit + kTile - 1) / kTile);
+                    atomicAdd(&sh.count, 1);
+                }
+            }
+            first += k.all();
+            unit0 += k.units;
+        }
+    __syncthreads();
 }
 // Where the part of a piece goes: a CTA has at most one that ends a unit
 // begun elsewhere, and one that begins a unit.

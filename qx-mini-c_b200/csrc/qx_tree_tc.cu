@@ -3,20 +3,23 @@
 // rows, one persistent CTA per SM.
 //
 // Roles, by warp:
-//   0-3, 4-7   two softmax groups, which take a piece's tiles in turn; a thread
-//              has one query row (TMEM lane), and each group its own scores,
-//              reference, sum and output accumulator
-//   8-11       bring the cache: INT8 codes from global memory into registers
-//              two tiles ahead, to F16 in shared memory, and the per-row
-//              constants of the scores; also the query block of each piece
-//   12         issues the MMAs: S = Q K^T (128 x 64), then O += P V with P read
-//              from TMEM, where it overwrites the S it came from
-// S of one group is computed while the other group is in its softmax.
+//   0-3, 4-7   two softmax groups, which take the tiles in turn; a thread has
+//              one query row (TMEM lane), and each group its own reference,
+//              sum and output accumulator.  Both bring the query blocks, too
+//   8          issues the MMAs: S = Q K^T (128 x 64), then O += P V with P read
+//              from TMEM, where it overwrites the S it came from; whichever
+//              has its operands, S up to four tiles ahead of O
+//   9-11       bring the cache: INT8 codes by TMA some tiles ahead, then to F16
+//              operands and the per-row constants of the scores
 //
-// Shared memory operands are in the no-swizzle core-matrix layout: 8 rows x 16
-// bytes each, [row / 8][dim / 8][row % 8].  That one layout is K-major for
-// K (rows = N, dims = K) and for Q, and MN-major for V (dims = N, rows = K), so
-// nothing is transposed.
+// F16 operands are in the no-swizzle core-matrix layout: 8 rows x 16 bytes
+// each, [row / 8][dim / 8][row % 8].  That one layout is K-major for K (rows =
+// N, dims = K) and for Q, and MN-major for V (dims = N, rows = K), so nothing is
+// transposed.  The codes arrive in TMA's 128-byte (64 dims: 64-byte) swizzle,
+// from which eight rows of one 16-byte chunk, what a quarter-warp reads and
+// writes at a time, lie in different banks.
+#include <cuda.h>
+
 #include <cmath>
 
 #include "qx_tree.cuh"
@@ -25,19 +28,27 @@ namespace qx {
 namespace ops {
 namespace {
 
-constexpr int kRows = 128, kGroup = 128, kBring = 128, kTcThreads = 2 * kGroup + kBring + 32;
-constexpr int kStages = 4, kAhead = 2;
+constexpr int kRows = 128, kGroup = 128, kBring = 96, kTcThreads = 2 * kGroup + 32 + kBring;
+constexpr int kKs = 2, kVs = 4;            // operand tiles: K goes once S is computed, V stays through the softmax
+constexpr int kScores = 4;                 // S buffers
+constexpr int kFacs = 8;                   // pieces whose row factors may be in use (queries run at most 6 ahead)
 
 template <int HD, int NT>
 struct Shape {
     static constexpr int kTileBytes = kTile * HD * 2;          // K or V of a tile
     static constexpr int kQBytes = kRows * HD * 2;             // one term of Q
-    static constexpr int kSmem = NT * kQBytes + kStages * 2 * kTileBytes + 128;
-    static constexpr int kTmem = HD == 128 ? 512 : 256;        // S of both groups, then O of both (a power of two)
+    static constexpr int kQs = NT == 1 ? 2 : 1;                // query blocks
+    static constexpr int kRawBytes = kTile * HD;               // codes of K or V of a tile
+    static constexpr int kAhead = NT == 1 ? 3 : 2;             // tiles of codes on their way
+    static constexpr int kQAt = kAhead * 2 * kRawBytes, kKvAt = kQAt + kQs * NT * kQBytes;
+    static constexpr int kSmem = kKvAt + (kKs + kVs) * kTileBytes + 1024;
+    static constexpr int kO = kScores * kTile;                 // TMEM column of group 0's output
+    static constexpr int kTmem = 512;                          // 256 + 2 HD, to a power of two
 };
 
 struct Bars {
-    unsigned long long full[kStages], empty[kStages], s_ready[2], p_ready[2], o_done[2], q_full, q_free, both, o_free;
+    unsigned long long raw[4], raw_free[4], k_full[kKs], k_free[kKs], v_full[kVs], v_free[kVs], s_ready[kScores], p_ready[kScores], o_done[2], q_full[2], q_free[2],
+        both, o_free;
 };
 struct alignas(16) Columns {
     float ks[kTile], lv[kTile], iv[kTile];
@@ -50,28 +61,43 @@ __device__ __forceinline__ void bar_init(unsigned long long* b, unsigned count) 
 __device__ __forceinline__ void bar_arrive(unsigned long long* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
 }
+__device__ __forceinline__ bool bar_try(unsigned long long* b, unsigned parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(smem_addr(b)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool bar_test(unsigned long long* b, unsigned parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(smem_addr(b)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
 // Bounded wait for a phase (2 s; a healthy one takes microseconds).  Gives up
-// at once where another role has.
-__device__ __forceinline__ bool bar_wait(unsigned long long* b, unsigned parity, volatile int* gave_up) {
+// soon after another role has, unless it is for work of its own in flight.
+__device__ __noinline__ bool bar_wait_slow(unsigned long long* b, unsigned parity, volatile int* gave_up, bool own) {
     unsigned long long t0 = 0;
-    for (unsigned i = 0;; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-            : "=r"(done)
-            : "r"(smem_addr(b)), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((i & 255u) == 255u) {
+    for (unsigned i = 1;; ++i) {
+        if (bar_try(b, parity)) return true;
+        if ((i & 255u) == 0u) {
             unsigned long long t;
             asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
             if (!t0) t0 = t;
-            if (*gave_up || t - t0 > 2000000000ull) {
+            if ((*gave_up && !own) || t - t0 > 2000000000ull) {
                 *gave_up = 1;
                 return false;
             }
         }
     }
+}
+__device__ __forceinline__ bool bar_wait(unsigned long long* b, unsigned parity, volatile int* gave_up, bool own = false) {
+    return bar_try(b, parity) || bar_wait_slow(b, parity, gave_up, own);
 }
 
 __device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -129,6 +155,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* r) {
         : "memory");
 }
 
+// After the wait for a load: what reads the registers stays behind it.
+template <int N>
+__device__ __forceinline__ void loaded(float2 (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(x[i].x), "+f"(x[i].y));
+}
+
 // Two F32 operations an instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 r;
@@ -155,166 +188,144 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // ---- bringing the cache --------------------------------------------------------
 
-// The tiles of a CTA, one after another over its pieces.
-struct TileCursor {
-    Cursor c;
-    Piece p;
-    int tile;
-    bool more;
-    __device__ __forceinline__ void find(const TreeArgs& a) {
-        do more = c.next(a, p);
-        while (more && p.tile1 <= p.tile0);
-        tile = p.tile0;
-    }
-    __device__ __forceinline__ void next(const TreeArgs& a) {
-        if (++tile >= p.tile1) find(a);
-    }
-};
-
-// A bringing thread's share of a tile's bytes.  Eight lanes take eight rows of
-// one 16-byte chunk (their F16 stores then fill 128 consecutive bytes), the
-// four groups of eight lanes four chunks.
-template <int HD>
-struct Raw {
-    static constexpr int kLoads = kTile * HD / 16 / kBring;    // of K, and of V
-    uint4 k[kLoads], v[kLoads];
-    float ks, vs;
-};
-template <int HD>
-__device__ __forceinline__ void where(int bt, int i, int& row, int& chunk) {
-    const int w = bt >> 5, lane = bt & 31, slot = w + 4 * i;   // warp-wide accesses: [chunk / 4][row / 8]
-    row = (slot & 7) * 8 + (lane & 7);
-    chunk = (slot >> 3) * 4 + (lane >> 3);
-}
-template <int HD>
-__device__ __forceinline__ void load_raw(const TreeArgs& a, const TileCursor& t, int bt, Raw<HD>& r) {
-    const int last = t.p.len + t.p.n - 1, row0 = t.tile * kTile;
-    const size_t KV = (size_t)a.c.kv_heads * HD;
-#pragma unroll
-    for (int i = 0; i < Raw<HD>::kLoads; ++i) {
-        int row, chunk;
-        where<HD>(bt, i, row, chunk);
-        const size_t at = (t.p.base_row + min(row0 + row, last)) * KV + (size_t)t.p.g * HD + 16 * chunk;
-        r.k[i] = __ldg(reinterpret_cast<const uint4*>(a.c.k + at));
-        r.v[i] = __ldg(reinterpret_cast<const uint4*>(a.c.v + at));
-    }
-    if (bt < kTile) {
-        const size_t row = t.p.base_row + min(row0 + bt, last);
-        r.ks = __ldg(a.c.ks + row);
-        r.vs = __ldg(a.c.vs + row);
-    }
-}
 // 16 codes as F16: two 16-byte units of an operand tile.
 __device__ __forceinline__ void widen(const uint4& w, uint8_t* to) {
     const uint32_t c[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
     *reinterpret_cast<uint4*>(to) = make_uint4(low_pair(c[0]), high_pair(c[0]), low_pair(c[1]), high_pair(c[1]));
     *reinterpret_cast<uint4*>(to + 128) = make_uint4(low_pair(c[2]), high_pair(c[2]), low_pair(c[3]), high_pair(c[3]));
 }
+// A tile's codes of K or V to F16, by the three bringing warps: a warp takes
+// eight rows of four 16-byte chunks at a time, all its reads before its writes.
+// `first`: the warp that has one unit more than the others.
 template <int HD>
-__device__ __forceinline__ void store_raw(const Raw<HD>& r, int bt, uint8_t* kt, uint8_t* vt, Columns& col) {
+__device__ __forceinline__ void widen_tile(const uint8_t* raw, int bt, int first, uint8_t* to) {
+    constexpr int kUnits = kTile / 8 * (HD / 64), kMine = (kUnits + 2) / 3;
+    const int lane = bt & 31, r8 = lane & 7, c4 = lane >> 3, w0 = (bt >> 5) == first ? 0 : (bt >> 5) == 1 ? 1 : 2;
+    uint4 w[kMine];
 #pragma unroll
-    for (int i = 0; i < Raw<HD>::kLoads; ++i) {
-        int row, chunk;
-        where<HD>(bt, i, row, chunk);
-        const int o = (row >> 3) * (HD / 8 * 128) + 2 * chunk * 128 + (row & 7) * 16;
-        widen(r.k[i], kt + o);
-        widen(r.v[i], vt + o);
+    for (int i = 0; i < kMine; ++i) {
+        const int u = 3 * i + w0;
+        if (u < kUnits) {
+            const int rows = u / (HD / 64), chunk = u % (HD / 64) * 4 + c4;
+            const int swizzled = HD == 128 ? chunk ^ r8 : chunk ^ (r8 >> 1);
+            w[i] = *reinterpret_cast<const uint4*>(raw + (rows * 8 + r8) * HD + swizzled * 16);
+        }
     }
-    if (bt < kTile) {
-        col.ks[bt] = r.ks;
-        col.lv[bt] = log_vs(r.vs);
-        col.iv[bt] = inv_vs(r.vs);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int u = 3 * i + w0;
+        if (u < kUnits) widen(w[i], to + u / (HD / 64) * (HD / 8 * 128) + (u % (HD / 64) * 4 + c4) * 256 + r8 * 16);
     }
 }
+__device__ __forceinline__ void tma_tile(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
 
-// Query row bt of a piece: F16 terms into the operand, the undoing factor to fac.
+// The query block of a piece as F16 terms, and the factors that undo the rows'
+// powers of two; both softmax groups, two neighbouring lanes to a row, which
+// take its units of eight values in turn.
 template <class T, int HD, int NT>
-__device__ __forceinline__ void stage_row(const TreeArgs& a, const Piece& p, int bt, uint8_t* qt, float* fac) {
-    constexpr int V = 16 / sizeof(T), U = 8;
-    const int r = p.row0 + bt;
-    const bool real = bt < p.have;
+__device__ __noinline__ void stage_queries(const TreeArgs& a, const Piece& p, int tid, uint8_t* qt, float* fac) {
+    constexpr int V = 16 / sizeof(T), kSteps = HD / 16, kPacks = 8 / V;
+    const int row = tid >> 1, half = tid & 1, r = p.row0 + row;
+    const bool real = row < p.have;
     const T* src = (const T*)a.q.p + p.s * a.q.seq + (real ? r / a.group : 0) * a.q.node +
-                   (size_t)(p.g * a.group + (real ? r % a.group : 0)) * a.q.head;
-    auto read = [&](int i) {
-        Pack<T, V> x;
-        if (a.wide) {
-            x = *reinterpret_cast<const Pack<T, V>*>(src + i);
-        } else {
+                   (size_t)(p.g * a.group + (real ? r % a.group : 0)) * a.q.head + half * 8;
+    Pack<T, V> x[kSteps][kPacks];
 #pragma unroll
-            for (int u = 0; u < V; ++u) x.v[u] = src[i + u];
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+#pragma unroll
+            for (int u = 0; u < V; ++u) x[i][k].v[u] = from_f32<T>(0.f);
+            if (real && a.wide) x[i][k] = *reinterpret_cast<const Pack<T, V>*>(src + 16 * i + V * k);
         }
-        return x;
-    };
+    if (real && !a.wide)
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+                for (int u = 0; u < V; ++u) x[i][k].v[u] = src[16 * i + V * k + u];
     float big = 0.f;
-    if (real)
-        for (int i = 0; i < HD; i += U * V) {
-            Pack<T, V> x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (i + u * V < HD) x[u] = read(i + u * V);
+    for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (i + u * V < HD)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float y = to_f32(x[u].v[e]);
-                        big = fmaxf(big, isfinite(y) ? fabsf(y) : 0.f);
-                    }
+        for (int e = 0; e < 8; ++e) {
+            const float y = to_f32(x[i][e / V].v[e % V]);
+            big = fmaxf(big, isfinite(y) ? fabsf(y) : 0.f);
         }
+    big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
     const RowScale rs(big);
-    uint8_t* to = qt + (bt >> 3) * (HD / 8 * 128) + (bt & 7) * 16;
-#pragma unroll 2
-    for (int d = 0; d < HD; d += 8) {
+    uint8_t* to = qt + (row >> 3) * (HD / 8 * 128) + (row & 7) * 16 + half * 128;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e += V) {
-            if (real) {
-                const Pack<T, V> x = read(d + e);
-#pragma unroll
-                for (int u = 0; u < V; ++u) y[e + u] = to_f32(x.v[u]) * rs.f0 * rs.f1;
-            } else {
-#pragma unroll
-                for (int u = 0; u < V; ++u) y[e + u] = 0.f;
-            }
-        }
+        for (int e = 0; e < 8; ++e) y[e] = to_f32(x[i][e / V].v[e % V]) * rs.f0 * rs.f1;
         const uint4 hi = make_uint4(pack_half(y[0], y[1]), pack_half(y[2], y[3]), pack_half(y[4], y[5]), pack_half(y[6], y[7]));
-        *reinterpret_cast<uint4*>(to + d / 8 * 128) = hi;
+        *reinterpret_cast<uint4*>(to + i * 256) = hi;
         if (NT == 2)
-            *reinterpret_cast<uint4*>(to + Shape<HD, NT>::kQBytes + d / 8 * 128) =
+            *reinterpret_cast<uint4*>(to + Shape<HD, NT>::kQBytes + i * 256) =
                 make_uint4(rest_half(y[0], y[1], hi.x), rest_half(y[2], y[3], hi.y), rest_half(y[4], y[5], hi.z),
                            rest_half(y[6], y[7], hi.w));
     }
-    fac[bt] = rs.undo(a.scale);
+    if (half == 0) fac[row] = rs.undo(a.scale);
 }
+
+// A place in the list: the pieces that have tiles, tile by tile.
+struct At {
+    int piece, tile, end;
+    __device__ __forceinline__ explicit At(const PieceList& l) : piece(-1), tile(0), end(0) { next(l); }
+    __device__ __forceinline__ void next(const PieceList& l) {
+        ++tile;
+        while (tile >= end && piece < l.count) {
+            if (++piece < l.count) tile = l.piece[piece].tile0, end = l.piece[piece].tile1;
+        }
+    }
+    __device__ __forceinline__ bool more(const PieceList& l) const { return piece < l.count; }
+};
 
 // ---- the kernel ----------------------------------------------------------------
 
+struct Maps {
+    CUtensorMap k, v;
+};
+
+// Tiles count through all lists: tile t is softmax group t % 2's, its S in
+// buffer t % 4, its operands in stages t % 2 (K) and t % 4 (V, and the columns'
+// constants).  Pieces (those with tiles) likewise.
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(TreeArgs a) {
+__global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant__ TreeArgs a, const __grid_constant__ Maps maps) {
     using S = Shape<HD, NT>;
     extern __shared__ uint8_t dyn[];
     __shared__ Bars bars;
-    __shared__ Columns cols[kStages];
-    __shared__ float fac_s[2][kRows], m_s[2][2][kRows], l_s[2][2][kRows];
-    __shared__ ScanShared scan;
+    __shared__ Columns cols[kVs];
+    __shared__ float fac_s[kFacs][kRows], m_s[2][2][kRows], l_s[2][2][kRows];
+    __shared__ PieceList list;
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
-    uint8_t* q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 127) & ~(uintptr_t)127);
-    uint8_t* kv_s = q_s + NT * S::kQBytes;                       // [stage][K, V]
+    uint8_t* raw_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);   // [ahead][K, V]
+    uint8_t* q_s = raw_s + S::kQAt;                              // [block][term]
+    uint8_t* k_s = raw_s + S::kKvAt;                             // [stage]
+    uint8_t* v_s = k_s + kKs * S::kTileBytes;                    // [stage]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    Cursor cur;
-    if (!begin_share(a, scan, cur)) return;                      // whole CTA
-    if (warp == 12) {
+    list_pieces(a, list, 0);
+    if (!list.count) return;                                     // whole CTA
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_s)), "n"(S::kTmem)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
         gave_up = 0;
-        for (int i = 0; i < kStages; ++i) bar_init(&bars.full[i], kBring), bar_init(&bars.empty[i], 1);
-        for (int w = 0; w < 2; ++w) bar_init(&bars.s_ready[w], 1), bar_init(&bars.p_ready[w], kGroup), bar_init(&bars.o_done[w], 1);
-        bar_init(&bars.q_full, kBring);
-        bar_init(&bars.q_free, 1);
+        for (int i = 0; i < 4; ++i) bar_init(&bars.raw[i], 1), bar_init(&bars.raw_free[i], kBring);
+        for (int i = 0; i < kKs; ++i) bar_init(&bars.k_full[i], kBring), bar_init(&bars.k_free[i], 1);
+        for (int i = 0; i < kVs; ++i) bar_init(&bars.v_full[i], kBring), bar_init(&bars.v_free[i], 1);
+        for (int i = 0; i < kScores; ++i) bar_init(&bars.s_ready[i], 1), bar_init(&bars.p_ready[i], kGroup);
+        for (int i = 0; i < 2; ++i) bar_init(&bars.o_done[i], 1), bar_init(&bars.q_full[i], 2 * kGroup), bar_init(&bars.q_free[i], 1);
         bar_init(&bars.both, 2 * kGroup);
         bar_init(&bars.o_free, 2 * kGroup);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -323,281 +334,398 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(TreeArgs a) {
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_s;
-    // columns: S of group w at 64 w (P over it), O of group w at 128 + HD w
-    if (warp < 8) {
-        // ---- softmax ----
-        const int w = warp >> 2, row = tid & 127;
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + 64 * w, to = tmem + lanes + 128 + HD * w;
-        unsigned tiles = 0, mine = 0, pieces = 0;                // tiles before this piece, of this group, pieces with tiles
-        Piece p;
-        bool ok = true;
-        while (ok && cur.next(a, p)) {
-            const int nt = max(0, p.tile1 - p.tile0);
-            float m = -INFINITY;
-            float2 l2 = make_float2(0.f, 0.f);
-            const bool real = row < p.have;
-            const int node = real ? (p.row0 + row) / a.group : 0;
-            const unsigned long long* mrow = a.mask ? a.mask + ((size_t)p.s * a.d.max_nodes + node) * a.words : nullptr;
-            float fac = 0.f;
-            for (int j = w; j < nt; j += 2) {
-                const unsigned t = tiles + j, st = t % kStages;
-                ok = bar_wait(&bars.full[st], (t / kStages) & 1, &gave_up) && bar_wait(&bars.s_ready[w], mine & 1, &gave_up);
-                ok = __all_sync(~0u, ok);                        // and the warp is one again for what follows
-                if (!ok) break;
-                fence_after();
-                if (j == w) fac = fac_s[pieces & 1][row];
-                float2 x[32];
-                tmem_ld32(ts, reinterpret_cast<uint32_t*>(x));
-                tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(x + 16));
-                wait_ld();
-                const Columns& col = cols[st];
-                const float2 fac2 = make_float2(fac, fac);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float4 k = *reinterpret_cast<const float4*>(&col.ks[2 * i]), v = *reinterpret_cast<const float4*>(&col.lv[2 * i]);
-                    x[i] = fma2(mul2(x[i], fac2), make_float2(k.x, k.y), make_float2(v.x, v.y));
-                    x[i + 1] = fma2(mul2(x[i + 1], fac2), make_float2(k.z, k.w), make_float2(v.z, v.w));
-                }
-                const int t0 = (p.tile0 + j) * kTile;
-                if (t0 + kTile > p.len) {
-                    const unsigned long long see = real ? sees64(mrow, a.words, node, t0, p.len, p.n) : 0ull;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (!(see >> (2 * i) & 1ull)) x[i].x = -INFINITY;
-                        if (!(see >> (2 * i + 1) & 1ull)) x[i].y = -INFINITY;
-                    }
-                }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], fmaxf(x[i].x, x[i].y));
-                const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const bool raise = big > m + kSlack || (m == -INFINITY && big > -INFINITY);
-                if (__any_sync(~0u, raise)) {
-                    const float f = raise ? exp2_fast(m - big) : 1.f;
-                    if (raise) m = big;
-                    l2 = mul2(l2, make_float2(f, f));
-                    if (j != w) {                                // an accumulator to rescale, once its last product is in
-                        ok = bar_wait(&bars.o_done[w], (mine - 1) & 1, &gave_up);
-                        ok = __all_sync(~0u, ok);
-                        if (!ok) break;
-                        fence_after();
-                        for (int c = 0; c < HD; c += 16) {
-                            float2 o[8];
-                            tmem_ld16(to + c, reinterpret_cast<uint32_t*>(o));
-                            wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] = mul2(o[i], make_float2(f, f));
-                            tmem_st16(to + c, reinterpret_cast<const uint32_t*>(o));
-                        }
-                    }
-                }
-                const float up = kPBias - (m == -INFINITY ? 0.f : m);
-                const float2 up2 = make_float2(up, up);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t ph[16], pl[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float4 iv = *reinterpret_cast<const float4*>(&col.iv[32 * h + 2 * i]);
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            float2 e = add2(x[16 * h + i + u], up2);
-                            e.x = exp2_fast(e.x);
-                            e.y = exp2_fast(e.y);
-                            l2 = fma2(e, u ? make_float2(iv.z, iv.w) : make_float2(iv.x, iv.y), l2);
-                            ph[i + u] = pack_half(e.x, e.y);
-                            if (NT == 2) pl[i + u] = rest_half(e.x, e.y, ph[i + u]);
-                        }
-                    }
-                    tmem_st16(ts + 16 * h, ph);
-                    if (NT == 2) tmem_st16(ts + 32 + 16 * h, pl);
-                }
-                wait_st();
-                fence_before();
-                bar_arrive(&bars.p_ready[w]);
-                ++mine;
-            }
-            if (!ok) break;
-            // both groups' references and sums, then half of the dims each
-            const int by = pieces & 1;
-            float* part = part_of(a, blockIdx.x, p.begins) + (size_t)row * (kPartHead + HD);
-            if (nt > 0) {
-                m_s[by][w][row] = m;
-                l_s[by][w][row] = l2.x + l2.y;
-                if (w < nt) ok = bar_wait(&bars.o_done[w], (mine - 1) & 1, &gave_up);
-                bar_arrive(&bars.both);
-                ok = bar_wait(&bars.both, pieces & 1, &gave_up) && ok;
+    unsigned t = 0, pc = 0;                                      // tiles and pieces of the lists before
+    for (int batch = 0;; ++batch) {
+        const int count = list.count;
+        if (warp < 8) {
+            // ---- softmax ----
+            const int w = warp >> 2, row = tid & 127;
+            const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), to = lanes + S::kO + HD * w;
+            bool ok = !gave_up;
+            unsigned qc = pc;                                    // query blocks staged
+            At q_at(list);
+            auto stage = [&]() {
+                if (!q_at.more(list)) return;
+                const unsigned b = qc % S::kQs, use = qc / S::kQs;
+                if (use) ok = bar_wait(&bars.q_free[b], (use - 1) & 1, &gave_up) && ok;
                 ok = __all_sync(~0u, ok);
+                if (!ok) return;
+                stage_queries<T, HD, NT>(a, list.piece[q_at.piece], tid, q_s + b * NT * S::kQBytes, fac_s[qc % kFacs]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bar_arrive(&bars.q_full[b]);
+                ++qc;
+                q_at.tile = q_at.end - 1;                        // on to the next piece with tiles
+                q_at.next(list);
+            };
+            stage();
+            for (int i = 0; ok && i < count; ++i) {
+                const Piece& p = list.piece[i];
+                if (S::kQs == 2 && p.tile1 > p.tile0) stage();   // the next piece's, before this one's tiles
                 if (!ok) break;
-                fence_after();
-                const float ma = m_s[by][0][row], mb = m_s[by][1][row], la = l_s[by][0][row], lb = l_s[by][1][row];
-                const float top = fmaxf(ma, mb);
-                const float fa = part_weight(ma, la, top), fb = nt > 1 ? part_weight(mb, lb, top) : 0.f;
-                const float sum = fmaf(fa, la, fb * lb);
-                const float by_sum = p.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
-                const float2 a2 = make_float2(fa * by_sum, fa * by_sum), b2 = make_float2(fb * by_sum, fb * by_sum);
-                const int h = p.g * a.group + (p.row0 + row) % a.group;
-                T* dst = (T*)a.out.p + p.s * a.out.seq + node * a.out.node + h * a.out.head;
-                for (int c = w * (HD / 2); c < (w + 1) * (HD / 2); c += 16) {
-                    float2 oa[8], ob[8];
-                    tmem_ld16(tmem + lanes + 128 + c, reinterpret_cast<uint32_t*>(oa));
-                    if (nt > 1) tmem_ld16(tmem + lanes + 128 + HD + c, reinterpret_cast<uint32_t*>(ob));
+                const int nt = max(0, p.tile1 - p.tile0), j0 = (w ^ t) & 1;
+                const int node = row < p.have ? (p.row0 + row) / a.group : -1;
+                float m = -INFINITY, fac = 0.f;
+                float2 l2 = make_float2(0.f, 0.f);
+                for (int j = j0; j < nt; j += 2) {
+                    const unsigned tt = t + j, st = tt % kVs;
+                    const uint32_t ts = lanes + kTile * (tt % kScores);
+                    ok = (j != j0 || bar_wait(&bars.q_full[pc % S::kQs], (pc / S::kQs) & 1, &gave_up)) &&
+                         bar_wait(&bars.v_full[st], (tt / kVs) & 1, &gave_up) &&
+                         bar_wait(&bars.s_ready[tt % kScores], (tt / kScores) & 1, &gave_up);
+                    ok = __all_sync(~0u, ok);                    // and the warp is one again for what follows
+                    if (!ok) break;
+                    fence_after();
+                    if (j == j0) fac = fac_s[pc % kFacs][row];
+                    float2 x[32];
+                    tmem_ld32(ts, reinterpret_cast<uint32_t*>(x));
+                    tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(x + 16));
+                    const Columns& col = cols[st];
+                    const float2 fac2 = make_float2(fac, fac);
                     wait_ld();
+                    loaded(x);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        oa[i] = mul2(oa[i], a2);
-                        if (nt > 1) oa[i] = fma2(ob[i], b2, oa[i]);
+                    for (int c = 0; c < 32; c += 2) {
+                        const float4 k = *reinterpret_cast<const float4*>(&col.ks[2 * c]), v = *reinterpret_cast<const float4*>(&col.lv[2 * c]);
+                        x[c] = fma2(mul2(x[c], fac2), make_float2(k.x, k.y), make_float2(v.x, v.y));
+                        x[c + 1] = fma2(mul2(x[c + 1], fac2), make_float2(k.z, k.w), make_float2(v.z, v.w));
                     }
-                    if (!real) continue;
-                    if (!p.whole) {
+                    const int t0 = (p.tile0 + j) * kTile;
+                    if (t0 + kTile > p.len) {
+                        const unsigned long long see =
+                            node < 0 ? 0ull
+                                     : sees64(a.mask ? a.mask + ((size_t)p.s * a.d.max_nodes + node) * a.words : nullptr, a.words, node,
+                                              t0, p.len, p.n);
+                        const uint32_t lo = (uint32_t)see, hi = (uint32_t)(see >> 32);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            *reinterpret_cast<float4*>(part + kPartHead + c + 4 * i) =
-                                make_float4(oa[2 * i].x, oa[2 * i].y, oa[2 * i + 1].x, oa[2 * i + 1].y);
-                    } else {
-                        constexpr int V = 16 / sizeof(T);
-                        const float* y = reinterpret_cast<const float*>(oa);
+                        for (int c = 0; c < 32; ++c) {
+                            const uint32_t bits = c < 16 ? lo : hi;
+                            if (!(bits >> (2 * (c & 15)) & 1u)) x[c].x = -INFINITY;
+                            if (!(bits >> (2 * (c & 15) + 1) & 1u)) x[c].y = -INFINITY;
+                        }
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < 16; i += V) {
-                            Pack<T, V> z;
+                    for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], fmaxf(x[c].x, x[c].y));
+                    const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const bool raise = big > m + kSlack || (m == -INFINITY && big > -INFINITY);
+                    if (__any_sync(~0u, raise)) {
+                        const float f = raise ? exp2_fast(m - big) : 1.f;
+                        if (raise) m = big;
+                        l2 = mul2(l2, make_float2(f, f));
+                        if (j != j0) {                           // an accumulator to rescale, once its last product is in
+                            ok = bar_wait(&bars.o_done[w], ((tt - 2) >> 1) & 1, &gave_up);
+                            ok = __all_sync(~0u, ok);
+                            if (!ok) break;
+                            fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < HD; c += 16) {
+                                float2 o[8];
+                                tmem_ld16(to + c, reinterpret_cast<uint32_t*>(o));
+                                wait_ld();
+                                loaded(o);
 #pragma unroll
-                            for (int u = 0; u < V; ++u) z.v[u] = from_f32<T>(y[i + u]);
-                            if (a.wide) {
-                                *reinterpret_cast<Pack<T, V>*>(dst + c + i) = z;
-                            } else {
-#pragma unroll
-                                for (int u = 0; u < V; ++u) dst[c + i + u] = z.v[u];
+                                for (int e = 0; e < 8; ++e) o[e] = mul2(o[e], make_float2(f, f));
+                                tmem_st16(to + c, reinterpret_cast<const uint32_t*>(o));
                             }
                         }
                     }
-                }
-                if (real && w == 0) {
-                    if (p.whole) write_lse(a, p.s, node, h, top, sum);
-                    else part[0] = top, part[1] = sum;
-                }
-                fence_before();
-                bar_arrive(&bars.o_free);
-                ++pieces;
-            } else if (real) {                                   // no row of the block sees these tiles
-                for (int c = w * (HD / 2); c < (w + 1) * (HD / 2); c += 4)
-                    *reinterpret_cast<float4*>(part + kPartHead + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (w == 0) part[0] = -INFINITY, part[1] = 0.f;
-            }
-            tiles += nt;
-        }
-    } else if (warp < 12) {
-        // ---- bring the cache ----
-        const int bt = tid - 2 * kGroup;
-        TileCursor ld, cv;
-        ld.c = cv.c = cur;
-        ld.find(a);
-        cv.find(a);
-        Raw<HD> raw[kAhead];
+                    const float up = kPBias - (m == -INFINITY ? 0.f : m);
+                    const float2 up2 = make_float2(up, up);
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d)
-            if (ld.more) load_raw<HD>(a, ld, bt, raw[d]), ld.next(a);
-        unsigned t = 0, pieces = 0;
-        bool ok = true, fresh = true;
-        while (ok && cv.more) {
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t ph[16], pl[16];
 #pragma unroll
-            for (int d = 0; d < kAhead; ++d) {
-                if (!ok || !cv.more) break;
-                if (fresh) {
-                    if (pieces) ok = bar_wait(&bars.q_free, (pieces - 1) & 1, &gave_up);
-                    if (!ok) break;
-                    stage_row<T, HD, NT>(a, cv.p, bt, q_s, fac_s[pieces & 1]);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    bar_arrive(&bars.q_full);
-                    ++pieces;
+                        for (int c = 0; c < 16; c += 2) {
+                            const float4 iv = *reinterpret_cast<const float4*>(&col.iv[32 * h + 2 * c]);
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                float2 e = add2(x[16 * h + c + u], up2);
+                                e.x = exp2_fast(e.x);
+                                e.y = exp2_fast(e.y);
+                                l2 = fma2(e, u ? make_float2(iv.z, iv.w) : make_float2(iv.x, iv.y), l2);
+                                ph[c + u] = pack_half(e.x, e.y);
+                                if (NT == 2) pl[c + u] = rest_half(e.x, e.y, ph[c + u]);
+                            }
+                        }
+                        tmem_st16(ts + 16 * h, ph);
+                        if (NT == 2) tmem_st16(ts + 32 + 16 * h, pl);
+                    }
+                    wait_st();
+                    fence_before();
+                    bar_arrive(&bars.p_ready[tt % kScores]);
                 }
-                const unsigned st = t % kStages, use = t / kStages;
-                if (use) ok = bar_wait(&bars.empty[st], (use - 1) & 1, &gave_up);
                 if (!ok) break;
-                uint8_t* kt = kv_s + (size_t)st * 2 * S::kTileBytes;
-                store_raw<HD>(raw[d], bt, kt, kt + S::kTileBytes, cols[st]);
+                if (S::kQs == 1 && nt > 0) stage();              // one block: once this piece's scores are all computed
+                if (!ok) break;
+                // both groups' references and sums, then half of the dims each
+                float* part = part_of(a, blockIdx.x, p.begins) + (size_t)row * (kPartHead + HD);
+                if (nt > 0) {
+                    const int by = pc & 1;
+                    m_s[by][w][row] = m;
+                    l_s[by][w][row] = l2.x + l2.y;
+                    if (j0 < nt) {                               // this group's last tile
+                        const unsigned last = t + nt - 1 - ((nt - 1 - j0) & 1);
+                        ok = bar_wait(&bars.o_done[w], (last >> 1) & 1, &gave_up);
+                    }
+                    bar_arrive(&bars.both);
+                    ok = bar_wait(&bars.both, pc & 1, &gave_up) && ok;
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                    fence_after();
+                    const float ma = m_s[by][0][row], mb = m_s[by][1][row], la = l_s[by][0][row], lb = l_s[by][1][row];
+                    const float top = fmaxf(ma, mb);
+                    // a group without a tile has m -infinity and sum 0: factor 0, and its O is not read
+                    const bool has_a = nt > 1 || (t & 1) == 0, has_b = nt > 1 || (t & 1) == 1;
+                    const float fa = part_weight(ma, la, top), fb = part_weight(mb, lb, top);
+                    const float sum = fmaf(fa, la, fb * lb);
+                    const float by_sum = p.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+                    const float2 a2 = make_float2(fa * by_sum, fa * by_sum), b2 = make_float2(fb * by_sum, fb * by_sum);
+                    const int h = p.g * a.group + (p.row0 + row) % a.group;
+                    T* dst = (T*)a.out.p + p.s * a.out.seq + node * a.out.node + h * a.out.head;
+#pragma unroll 1
+                    for (int c = w * (HD / 2); c < (w + 1) * (HD / 2); c += 16) {
+                        float2 oa[8] = {}, ob[8] = {};
+                        if (has_a) tmem_ld16(lanes + S::kO + c, reinterpret_cast<uint32_t*>(oa));
+                        if (has_b) tmem_ld16(lanes + S::kO + HD + c, reinterpret_cast<uint32_t*>(ob));
+                        wait_ld();
+                        loaded(oa);
+                        loaded(ob);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) oa[e] = fma2(ob[e], b2, mul2(oa[e], a2));
+                        if (node < 0) continue;
+                        if (!p.whole) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                *reinterpret_cast<float4*>(part + kPartHead + c + 4 * e) =
+                                    make_float4(oa[2 * e].x, oa[2 * e].y, oa[2 * e + 1].x, oa[2 * e + 1].y);
+                        } else {
+                            constexpr int V = 16 / sizeof(T);
+                            const float* y = reinterpret_cast<const float*>(oa);
+#pragma unroll
+                            for (int e = 0; e < 16; e += V) {
+                                Pack<T, V> z;
+#pragma unroll
+                                for (int u = 0; u < V; ++u) z.v[u] = from_f32<T>(y[e + u]);
+                                if (a.wide) {
+                                    *reinterpret_cast<Pack<T, V>*>(dst + c + e) = z;
+                                } else {
+#pragma unroll
+                                    for (int u = 0; u < V; ++u) dst[c + e + u] = z.v[u];
+                                }
+                            }
+                        }
+                    }
+                    if (node >= 0 && w == 0) {
+                        if (p.whole) write_lse(a, p.s, node, h, top, sum);
+                        else part[0] = top, part[1] = sum;
+                    }
+                    fence_before();
+                    bar_arrive(&bars.o_free);
+                    ++pc;
+                } else if (node >= 0) {                          // no row of the block sees these tiles
+#pragma unroll 1
+                    for (int c = w * (HD / 2); c < (w + 1) * (HD / 2); c += 4)
+                        *reinterpret_cast<float4*>(part + kPartHead + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (w == 0) part[0] = -INFINITY, part[1] = 0.f;
+                }
+                t += nt;
+            }
+        } else if (warp > 8) {
+            // ---- bring the cache ----
+            const int bt = tid - 2 * kGroup - 32;
+            const uint32_t raw_a = smem_addr(raw_s);
+            bool ok = !gave_up;
+            unsigned sent = t;                                   // by the first thread: tiles asked for
+            At to_send(list), here(list), soon(list);
+            auto send = [&]() {
+                if (!to_send.more(list)) return;
+                const Piece& p = list.piece[to_send.piece];
+                const unsigned slot = sent % S::kAhead;
+                const uint32_t bar = smem_addr(&bars.raw[slot]), to = raw_a + slot * 2 * S::kRawBytes;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * S::kRawBytes) : "memory");
+                const int y = (int)p.base_row + to_send.tile * kTile;
+                tma_tile(to, &maps.k, p.g * HD, y, bar);
+                tma_tile(to + S::kRawBytes, &maps.v, p.g * HD, y, bar);
+                ++sent;
+                to_send.next(list);
+            };
+            if (bt == 0)
+                for (int d = 0; d < S::kAhead; ++d) send();
+            // the scales of row bt, a tile ahead
+            auto scales = [&](const At& x) {
+                if (bt >= kTile || !x.more(list)) return make_float2(0.f, 0.f);
+                const Piece& p = list.piece[x.piece];
+                const size_t r = p.base_row + min(x.tile * kTile + bt, p.len + p.n - 1);
+                return make_float2(__ldg(a.c.ks + r), __ldg(a.c.vs + r));
+            };
+            float2 sc = scales(soon);
+            soon.next(list);
+            for (; ok && here.more(list); here.next(list)) {
+                const unsigned ks = t % kKs, vs = t % kVs, slot = t % S::kAhead;
+                const uint8_t* raw = raw_s + slot * 2 * S::kRawBytes;
+                ok = bar_wait(&bars.raw[slot], (t / S::kAhead) & 1, &gave_up);
+                if (ok && t >= kKs) ok = bar_wait(&bars.k_free[ks], (t / kKs - 1) & 1, &gave_up);
+                ok = __all_sync(~0u, ok);
+                if (!ok) break;
+                widen_tile<HD>(raw, bt, 0, k_s + ks * S::kTileBytes);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(&bars.full[st]);
+                bar_arrive(&bars.k_full[ks]);
+                const float2 now = sc;
+                sc = scales(soon);
+                soon.next(list);
+                if (t >= kVs) ok = bar_wait(&bars.v_free[vs], (t / kVs - 1) & 1, &gave_up);
+                ok = __all_sync(~0u, ok);
+                if (!ok) break;
+                if (bt < kTile) {
+                    cols[vs].ks[bt] = now.x;
+                    cols[vs].lv[bt] = log_vs(now.y);
+                    cols[vs].iv[bt] = inv_vs(now.y);
+                }
+                widen_tile<HD>(raw + S::kRawBytes, bt, 2, v_s + vs * S::kTileBytes);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bar_arrive(&bars.v_full[vs]);
+                bar_arrive(&bars.raw_free[slot]);
+                if (bt == 0) {                                   // once all three warps have read the codes
+                    ok = bar_wait(&bars.raw_free[slot], (t / S::kAhead) & 1, &gave_up);
+                    if (ok) send();
+                }
                 ++t;
-                fresh = cv.tile + 1 >= cv.p.tile1;
-                cv.next(a);
-                if (ld.more) load_raw<HD>(a, ld, bt, raw[d]), ld.next(a);
+            }
+            // copies of this CTA still on their way, if a wait gave up
+            if (bt == 0)
+                for (; t < sent; ++t) bar_wait(&bars.raw[t % S::kAhead], (t / S::kAhead) & 1, &gave_up, true);
+        } else if (lane == 0) {
+            // ---- issue the products ----
+            const uint32_t qa = smem_addr(q_s), ka = smem_addr(k_s), va = smem_addr(v_s);
+            constexpr uint32_t kGroupStride = HD / 8 * 128;       // eight rows
+            constexpr uint32_t id_s = idesc_f16(kRows, kTile, false), id_o = idesc_f16(kRows, HD, true);
+            bool ok = !gave_up;
+            At qk(list), pv(list);
+            const unsigned t0 = t;
+            unsigned to = t, pq = pc;                            // tile of the second product; piece of the first
+            unsigned idle = 0;
+            unsigned long long since = 0;
+            while (pv.more(list)) {
+                if (to < t) {
+                    const Piece& p = list.piece[pv.piece];
+                    const unsigned vs = to % kVs, sb = to % kScores;
+                    if (bar_test(&bars.p_ready[sb], (to / kScores) & 1) &&
+                        (pv.tile != p.tile0 || !pc || bar_test(&bars.o_free, (pc - 1) & 1)) &&
+                        bar_test(&bars.v_full[vs], (to / kVs) & 1)) {                 // O of tile `to`
+                        fence_after();
+                        const uint32_t vt = va + vs * S::kTileBytes, d = tmem + S::kO + HD * (to & 1), ap = tmem + kTile * sb;
+                        const uint32_t add = pv.tile - p.tile0 >= 2;
+#pragma unroll
+                        for (int q = 0; q < NT; ++q)
+#pragma unroll
+                            for (int k = 0; k < kTile / 16; ++k)
+                                mma_ts(d, ap + 32 * q + 8 * k, umma_desc(vt + k * 2 * kGroupStride, kGroupStride, 128), id_o,
+                                       add | (q + k > 0));
+                        mma_commit(&bars.v_free[vs]);
+                        mma_commit(&bars.o_done[to & 1]);
+                        if (pv.tile == p.tile1 - 1) ++pc;
+                        ++to;
+                        pv.next(list);
+                        idle = 0;
+                        continue;
+                    }
+                }
+                if (qk.more(list) && t - to < kScores) {
+                    const Piece& p = list.piece[qk.piece];
+                    const unsigned ks = t % kKs, b = pq % S::kQs;
+                    if (bar_test(&bars.k_full[ks], (t / kKs) & 1) &&
+                        (qk.tile != p.tile0 || bar_test(&bars.q_full[b], (pq / S::kQs) & 1))) {   // S of tile t
+                        fence_after();
+                        const uint32_t kt = ka + ks * S::kTileBytes, qb = qa + b * NT * S::kQBytes, d = tmem + kTile * (t % kScores);
+#pragma unroll
+                        for (int q = 0; q < NT; ++q)
+#pragma unroll
+                            for (int k = 0; k < HD / 16; ++k)
+                                mma_ss(d, umma_desc(qb + q * S::kQBytes + k * 256, 128, kGroupStride),
+                                       umma_desc(kt + k * 256, 128, kGroupStride), id_s, q + k > 0);
+                        mma_commit(&bars.s_ready[t % kScores]);
+                        mma_commit(&bars.k_free[ks]);
+                        if (qk.tile == p.tile1 - 1) mma_commit(&bars.q_free[b]), ++pq;
+                        ++t;
+                        qk.next(list);
+                        idle = 0;
+                        continue;
+                    }
+                }
+                if ((++idle & 1023u) == 0) {                     // as bounded as the other roles' waits
+                    unsigned long long now;
+                    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+                    if (idle == 1024u) since = now;
+                    if (*(volatile int*)&gave_up || now - since > 2000000000ull) {
+                        *(volatile int*)&gave_up = 1;
+                        ok = false;
+                        break;
+                    }
+                }
+            }
+            // the last products are in before TMEM goes (the softmax groups have waited for them, unless a wait gave up)
+            if (!ok) {
+                for (unsigned i = t > t0 + kScores ? t - kScores : t0; i < t; ++i)
+                    bar_wait(&bars.s_ready[i % kScores], (i / kScores) & 1, &gave_up, true);
+                for (unsigned i = to > t0 + 2 ? to - 2 : t0; i < to; ++i) bar_wait(&bars.o_done[i & 1], (i >> 1) & 1, &gave_up, true);
             }
         }
-    } else if (lane == 0) {
-        // ---- issue the products ----
-        const uint32_t qa = smem_addr(q_s), kva = smem_addr(kv_s);
-        constexpr uint32_t kGroupStride = HD / 8 * 128;           // eight rows
-        constexpr uint32_t id_s = idesc_f16(kRows, kTile, false), id_o = idesc_f16(kRows, HD, true);
-        unsigned t = 0, mine[2] = {0, 0}, pieces = 0;
-        Piece p;
-        bool ok = true;
-        while (ok && cur.next(a, p)) {
-            const int nt = max(0, p.tile1 - p.tile0);
-            if (!nt) continue;
-            ok = bar_wait(&bars.q_full, pieces & 1, &gave_up);
-            bool fresh_o = true;
-            for (int j = 0; ok && j <= nt; ++j) {
-                if (j < nt) {                                    // S of tile j
-                    const unsigned st = (t + j) % kStages;
-                    ok = bar_wait(&bars.full[st], ((t + j) / kStages) & 1, &gave_up);
-                    if (!ok) break;
-                    fence_after();
-                    const uint32_t kt = kva + st * 2 * S::kTileBytes, d = tmem + 64 * (j & 1);
-#pragma unroll
-                    for (int q = 0; q < NT; ++q)
-#pragma unroll
-                        for (int k = 0; k < HD / 16; ++k)
-                            mma_ss(d, umma_desc(qa + q * S::kQBytes + k * 256, 128, kGroupStride),
-                                   umma_desc(kt + k * 256, 128, kGroupStride), id_s, q + k > 0);
-                    mma_commit(&bars.s_ready[j & 1]);
-                    if (j == nt - 1) mma_commit(&bars.q_free);
-                }
-                if (j > 0) {                                     // O of tile j - 1
-                    const int w = (j - 1) & 1;
-                    const unsigned st = (t + j - 1) % kStages;
-                    if (fresh_o && pieces) ok = bar_wait(&bars.o_free, (pieces - 1) & 1, &gave_up);
-                    fresh_o = false;
-                    ok = ok && bar_wait(&bars.p_ready[w], mine[w] & 1, &gave_up);
-                    if (!ok) break;
-                    ++mine[w];
-                    fence_after();
-                    const uint32_t vt = kva + st * 2 * S::kTileBytes + S::kTileBytes, d = tmem + 128 + HD * w, ap = tmem + 64 * w;
-#pragma unroll
-                    for (int q = 0; q < NT; ++q)
-#pragma unroll
-                        for (int k = 0; k < kTile / 16; ++k)
-                            mma_ts(d, ap + 32 * q + 8 * k, umma_desc(vt + k * 2 * kGroupStride, kGroupStride, 128), id_o,
-                                   j - 1 >= 2 || q + k > 0);
-                    mma_commit(&bars.empty[st]);
-                    mma_commit(&bars.o_done[w]);
-                }
-            }
-            t += nt;
-            ++pieces;
-        }
-        // the last products are in before TMEM goes (the softmax groups waited for them, unless a wait gave up)
-        if (!ok)
-            for (int w = 0; w < 2; ++w)
-                if (mine[w]) bar_wait(&bars.o_done[w], (mine[w] - 1) & 1, &gave_up);
+        __syncwarp();
+        __syncthreads();                                         // every role is done with the list
+        const bool again = !gave_up && list.more;
+        __syncthreads();                                         // and has seen whether there is another
+        if (!again) break;
+        list_pieces(a, list, batch + 1);
     }
-    __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
     if (tid == 0 && gave_up && a.status) atomicOr(a.status, QX_CUDA_STATUS_TIMEOUT);
-    if (warp == 12) {
+    if (warp == 8) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmem) : "memory");
     }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return fn;
+}
+
+// The whole cache as rows of codes; boxes of 64 rows of one KV head.  Rows past
+// the last are filled with zeros, so a tile may run over the end.
+cudaError_t cache_maps(const Cache& c, Maps& m) {
+    const EncodeTiled encode = encoder();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t row = (cuuint64_t)c.kv_heads * c.head_dim;
+    const cuuint64_t dims[2] = {row, (cuuint64_t)cache_rows(c)}, strides[1] = {row};
+    const cuuint32_t box[2] = {(cuuint32_t)c.head_dim, (cuuint32_t)kTile}, steps[2] = {1, 1};
+    const CUtensorMapSwizzle sw = c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    for (int i = 0; i < 2; ++i)
+        if (encode(i ? &m.v : &m.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i ? c.v : c.k, dims, strides, box, steps,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    return cudaSuccess;
 }
 
 template <class T, int HD, int NT>
 cudaError_t run(TreeArgs& a, int sms, cudaStream_t st) {
     a.ctas = sms < kMaxCtas / 8 ? sms : kMaxCtas / 8;
-    const cudaError_t e = cudaFuncSetAttribute((const void*)k_tree_tc<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               Shape<HD, NT>::kSmem);
+    Maps maps;
+    cudaError_t e = cache_maps(a.c, maps);
     if (e != cudaSuccess) return e;
-    k_tree_tc<T, HD, NT><<<a.ctas, kTcThreads, Shape<HD, NT>::kSmem, st>>>(a);
+    e = cudaFuncSetAttribute((const void*)k_tree_tc<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD, NT>::kSmem);
+    if (e != cudaSuccess) return e;
+    k_tree_tc<T, HD, NT><<<a.ctas, kTcThreads, Shape<HD, NT>::kSmem, st>>>(a, maps);
     return cudaGetLastError();
 }
 
