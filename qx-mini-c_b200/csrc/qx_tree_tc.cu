@@ -9,8 +9,9 @@
 //   8          issues the MMAs: S = Q K^T (128 x 64), then O += P V with P read
 //              from TMEM, where it overwrites the S it came from; whichever
 //              has its operands, S up to four tiles ahead of O
-//   9-11       bring the cache: INT8 codes by TMA some tiles ahead, then to F16
-//              operands and the per-row constants of the scores
+//   9, 10      turn the INT8 codes into F16 operands
+//   11         asks for the codes, by TMA some tiles ahead, and makes the per-row
+//              constants of the scores
 //
 // F16 operands are in the no-swizzle core-matrix layout: 8 rows x 16 bytes
 // each, [row / 8][dim / 8][row % 8].  That one layout is K-major for K (rows =
@@ -28,7 +29,7 @@ namespace qx {
 namespace ops {
 namespace {
 
-constexpr int kRows = 128, kGroup = 128, kBring = 96, kTcThreads = 2 * kGroup + 32 + kBring;
+constexpr int kRows = 128, kGroup = 128, kTeam = 64, kTcThreads = 2 * kGroup + 128;
 constexpr int kKs = 2, kVs = 4;            // operand tiles: K goes once S is computed, V stays through the softmax
 constexpr int kScores = 4;                 // S buffers
 constexpr int kFacs = 8;                   // pieces whose row factors may be in use (queries run at most 6 ahead)
@@ -47,7 +48,7 @@ struct Shape {
 };
 
 struct Bars {
-    unsigned long long raw[4], raw_free[4], k_full[kKs], k_free[kKs], v_full[kVs], v_free[kVs], s_ready[kScores], p_ready[kScores], o_done[2], q_full[2], q_free[2],
+    unsigned long long raw[4], raw_free[4], k_full[kKs], k_free[kKs], v_full[kVs], v_free[kVs], c_full[kVs], s_ready[kScores], p_ready[kScores], o_done[2], q_full[2], q_free[2],
         both, o_free;
 };
 struct alignas(16) Columns {
@@ -194,27 +195,24 @@ __device__ __forceinline__ void widen(const uint4& w, uint8_t* to) {
     *reinterpret_cast<uint4*>(to) = make_uint4(low_pair(c[0]), high_pair(c[0]), low_pair(c[1]), high_pair(c[1]));
     *reinterpret_cast<uint4*>(to + 128) = make_uint4(low_pair(c[2]), high_pair(c[2]), low_pair(c[3]), high_pair(c[3]));
 }
-// A tile's codes of K or V to F16, by the three bringing warps: a warp takes
-// eight rows of four 16-byte chunks at a time, all its reads before its writes.
-// `first`: the warp that has one unit more than the others.
+// A tile's codes of K or V to F16, by two warps: a warp takes eight rows of four
+// 16-byte chunks at a time, four such units' reads before their writes.
 template <int HD>
-__device__ __forceinline__ void widen_tile(const uint8_t* raw, int bt, int first, uint8_t* to) {
-    constexpr int kUnits = kTile / 8 * (HD / 64), kMine = (kUnits + 2) / 3;
-    const int lane = bt & 31, r8 = lane & 7, c4 = lane >> 3, w0 = (bt >> 5) == first ? 0 : (bt >> 5) == 1 ? 1 : 2;
-    uint4 w[kMine];
+__device__ __forceinline__ void widen_tile(const uint8_t* raw, int bt, uint8_t* to) {
+    constexpr int kUnits = kTile / 8 * (HD / 64), kBatch = 4;
+    const int lane = bt & 31, r8 = lane & 7, c4 = lane >> 3, w = bt >> 5;
+    // unit 2 i + w: with 128 dims chunks 4 w .. 4 w + 3 of rows 8 i .., with 64 rows 8 (2 i + w) ..
+    const int chunk = (HD == 128 ? 4 * w : 0) + c4, row0 = HD == 128 ? 0 : 8 * w;
+    constexpr int kStep = HD == 128 ? 8 : 16;                  // rows from one of a warp's units to the next
+    raw += (row0 + r8) * HD + (HD == 128 ? chunk ^ r8 : chunk ^ (r8 >> 1)) * 16;
+    to += row0 / 8 * (HD / 8 * 128) + chunk * 256 + r8 * 16;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        const int u = 3 * i + w0;
-        if (u < kUnits) {
-            const int rows = u / (HD / 64), chunk = u % (HD / 64) * 4 + c4;
-            const int swizzled = HD == 128 ? chunk ^ r8 : chunk ^ (r8 >> 1);
-            w[i] = *reinterpret_cast<const uint4*>(raw + (rows * 8 + r8) * HD + swizzled * 16);
-        }
-    }
+    for (int i = 0; i < kUnits / 2; i += kBatch) {
+        uint4 x[kBatch];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        const int u = 3 * i + w0;
-        if (u < kUnits) widen(w[i], to + u / (HD / 64) * (HD / 8 * 128) + (u % (HD / 64) * 4 + c4) * 256 + r8 * 16);
+        for (int k = 0; k < kBatch; ++k) x[k] = *reinterpret_cast<const uint4*>(raw + (i + k) * kStep * HD);
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) widen(x[k], to + (i + k) * (kStep / 8) * (HD / 8 * 128));
     }
 }
 __device__ __forceinline__ void tma_tile(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -321,9 +319,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
     }
     if (tid == 0) {
         gave_up = 0;
-        for (int i = 0; i < 4; ++i) bar_init(&bars.raw[i], 1), bar_init(&bars.raw_free[i], kBring);
-        for (int i = 0; i < kKs; ++i) bar_init(&bars.k_full[i], kBring), bar_init(&bars.k_free[i], 1);
-        for (int i = 0; i < kVs; ++i) bar_init(&bars.v_full[i], kBring), bar_init(&bars.v_free[i], 1);
+        for (int i = 0; i < 4; ++i) bar_init(&bars.raw[i], 1), bar_init(&bars.raw_free[i], kTeam);
+        for (int i = 0; i < kKs; ++i) bar_init(&bars.k_full[i], kTeam), bar_init(&bars.k_free[i], 1);
+        for (int i = 0; i < kVs; ++i) bar_init(&bars.v_full[i], kTeam), bar_init(&bars.v_free[i], 1), bar_init(&bars.c_full[i], 32);
         for (int i = 0; i < kScores; ++i) bar_init(&bars.s_ready[i], 1), bar_init(&bars.p_ready[i], kGroup);
         for (int i = 0; i < 2; ++i) bar_init(&bars.o_done[i], 1), bar_init(&bars.q_full[i], 2 * kGroup), bar_init(&bars.q_free[i], 1);
         bar_init(&bars.both, 2 * kGroup);
@@ -370,7 +368,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                     const unsigned tt = t + j, st = tt % kVs;
                     const uint32_t ts = lanes + kTile * (tt % kScores);
                     ok = (j != j0 || bar_wait(&bars.q_full[pc % S::kQs], (pc / S::kQs) & 1, &gave_up)) &&
-                         bar_wait(&bars.v_full[st], (tt / kVs) & 1, &gave_up) &&
+                         bar_wait(&bars.c_full[st], (tt / kVs) & 1, &gave_up) &&
                          bar_wait(&bars.s_ready[tt % kScores], (tt / kScores) & 1, &gave_up);
                     ok = __all_sync(~0u, ok);                    // and the warp is one again for what follows
                     if (!ok) break;
@@ -530,129 +528,147 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                 }
                 t += nt;
             }
-        } else if (warp > 8) {
-            // ---- bring the cache ----
+        } else if (warp == 9 || warp == 10) {
+            // ---- widen the codes ----
             const int bt = tid - 2 * kGroup - 32;
-            const uint32_t raw_a = smem_addr(raw_s);
             bool ok = !gave_up;
-            unsigned sent = t;                                   // by the first thread: tiles asked for
-            At to_send(list), here(list), soon(list);
-            auto send = [&]() {
-                if (!to_send.more(list)) return;
-                const Piece& p = list.piece[to_send.piece];
-                const unsigned slot = sent % S::kAhead;
-                const uint32_t bar = smem_addr(&bars.raw[slot]), to = raw_a + slot * 2 * S::kRawBytes;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * S::kRawBytes) : "memory");
-                const int y = (int)p.base_row + to_send.tile * kTile;
-                tma_tile(to, &maps.k, p.g * HD, y, bar);
-                tma_tile(to + S::kRawBytes, &maps.v, p.g * HD, y, bar);
-                ++sent;
-                to_send.next(list);
-            };
-            if (bt == 0)
-                for (int d = 0; d < S::kAhead; ++d) send();
-            // the scales of row bt, a tile ahead
-            auto scales = [&](const At& x) {
-                if (bt >= kTile || !x.more(list)) return make_float2(0.f, 0.f);
-                const Piece& p = list.piece[x.piece];
-                const size_t r = p.base_row + min(x.tile * kTile + bt, p.len + p.n - 1);
-                return make_float2(__ldg(a.c.ks + r), __ldg(a.c.vs + r));
-            };
-            float2 sc = scales(soon);
-            soon.next(list);
-            for (; ok && here.more(list); here.next(list)) {
+            for (At here(list); ok && here.more(list); here.next(list), ++t) {
                 const unsigned ks = t % kKs, vs = t % kVs, slot = t % S::kAhead;
                 const uint8_t* raw = raw_s + slot * 2 * S::kRawBytes;
                 ok = bar_wait(&bars.raw[slot], (t / S::kAhead) & 1, &gave_up);
                 if (ok && t >= kKs) ok = bar_wait(&bars.k_free[ks], (t / kKs - 1) & 1, &gave_up);
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
-                widen_tile<HD>(raw, bt, 0, k_s + ks * S::kTileBytes);
+                widen_tile<HD>(raw, bt, k_s + ks * S::kTileBytes);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 bar_arrive(&bars.k_full[ks]);
-                const float2 now = sc;
-                sc = scales(soon);
-                soon.next(list);
                 if (t >= kVs) ok = bar_wait(&bars.v_free[vs], (t / kVs - 1) & 1, &gave_up);
                 ok = __all_sync(~0u, ok);
                 if (!ok) break;
-                if (bt < kTile) {
-                    cols[vs].ks[bt] = now.x;
-                    cols[vs].lv[bt] = log_vs(now.y);
-                    cols[vs].iv[bt] = inv_vs(now.y);
-                }
-                widen_tile<HD>(raw + S::kRawBytes, bt, 2, v_s + vs * S::kTileBytes);
+                widen_tile<HD>(raw + S::kRawBytes, bt, v_s + vs * S::kTileBytes);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 bar_arrive(&bars.v_full[vs]);
                 bar_arrive(&bars.raw_free[slot]);
-                if (bt == 0) {                                   // once all three warps have read the codes
-                    ok = bar_wait(&bars.raw_free[slot], (t / S::kAhead) & 1, &gave_up);
-                    if (ok) send();
+            }
+        } else if (warp == 11) {
+            // ---- ask for the codes, make the columns' constants ----
+            const uint32_t raw_a = smem_addr(raw_s);
+            bool ok = !gave_up;
+            unsigned sent = t;                                   // tiles asked for
+            At to_send(list), soon(list);
+            auto send = [&]() {
+                if (!to_send.more(list)) return;
+                if (lane == 0) {
+                    const Piece& p = list.piece[to_send.piece];
+                    const unsigned slot = sent % S::kAhead;
+                    const uint32_t bar = smem_addr(&bars.raw[slot]), to = raw_a + slot * 2 * S::kRawBytes;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * S::kRawBytes) : "memory");
+                    const int y = (int)p.base_row + to_send.tile * kTile;
+                    tma_tile(to, &maps.k, p.g * HD, y, bar);
+                    tma_tile(to + S::kRawBytes, &maps.v, p.g * HD, y, bar);
                 }
-                ++t;
+                ++sent;
+                to_send.next(list);
+            };
+#pragma unroll 1
+            for (int d = 0; d < S::kAhead; ++d) send();
+            // the scales of rows 2 lane and 2 lane + 1, a tile ahead
+            auto scales = [&]() {
+                if (!soon.more(list)) return make_float4(0.f, 0.f, 0.f, 0.f);
+                const Piece& p = list.piece[soon.piece];
+                const int last = p.len + p.n - 1, r = soon.tile * kTile + 2 * lane;
+                const size_t r0 = p.base_row + min(r, last), r1 = p.base_row + min(r + 1, last);
+                soon.next(list);
+                return make_float4(__ldg(a.c.ks + r0), __ldg(a.c.ks + r1), __ldg(a.c.vs + r0), __ldg(a.c.vs + r1));
+            };
+            float4 sc = scales();
+            for (At here(list); here.more(list); here.next(list), ++t) {
+                const unsigned vs = t % kVs;
+                const float4 now = sc;
+                sc = scales();
+                if (t >= kVs) ok = bar_wait(&bars.v_free[vs], (t / kVs - 1) & 1, &gave_up);
+                ok = __all_sync(~0u, ok);
+                if (!ok) break;
+                *reinterpret_cast<float2*>(&cols[vs].ks[2 * lane]) = make_float2(now.x, now.y);
+                *reinterpret_cast<float2*>(&cols[vs].lv[2 * lane]) = make_float2(log_vs(now.z), log_vs(now.w));
+                *reinterpret_cast<float2*>(&cols[vs].iv[2 * lane]) = make_float2(inv_vs(now.z), inv_vs(now.w));
+                bar_arrive(&bars.c_full[vs]);
+                if (to_send.more(list)) {                        // once its team has read the tile's codes
+                    ok = bar_wait(&bars.raw_free[t % S::kAhead], (t / S::kAhead) & 1, &gave_up);
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                    send();
+                }
             }
             // copies of this CTA still on their way, if a wait gave up
-            if (bt == 0)
-                for (; t < sent; ++t) bar_wait(&bars.raw[t % S::kAhead], (t / S::kAhead) & 1, &gave_up, true);
+            if (!ok)
+                for (unsigned i = sent > S::kAhead ? sent - S::kAhead : 0; i < sent; ++i)
+                    bar_wait(&bars.raw[i % S::kAhead], (i / S::kAhead) & 1, &gave_up, true);
         } else if (lane == 0) {
             // ---- issue the products ----
-            const uint32_t qa = smem_addr(q_s), ka = smem_addr(k_s), va = smem_addr(v_s);
             constexpr uint32_t kGroupStride = HD / 8 * 128;       // eight rows
             constexpr uint32_t id_s = idesc_f16(kRows, kTile, false), id_o = idesc_f16(kRows, HD, true);
+            // descriptors of the operands' first blocks; others are so many 16-byte units further
+            const uint64_t qd = umma_desc(smem_addr(q_s), 128, kGroupStride), kd = umma_desc(smem_addr(k_s), 128, kGroupStride),
+                           vd = umma_desc(smem_addr(v_s), kGroupStride, 128);
             bool ok = !gave_up;
-            At qk(list), pv(list);
+            At qk(list), pv(list);                               // the pieces of the first and the second product
+            int qk_left = qk.more(list) ? qk.end - qk.tile : 0, pv_left = pv.end - pv.tile;
+            int pv_done = 0;                                     // tiles of the second's piece that are done
             const unsigned t0 = t;
             unsigned to = t, pq = pc;                            // tile of the second product; piece of the first
+            bool q_new = true;                                   // the first's queries are still to be waited for
             unsigned idle = 0;
             unsigned long long since = 0;
             while (pv.more(list)) {
-                if (to < t) {
-                    const Piece& p = list.piece[pv.piece];
-                    const unsigned vs = to % kVs, sb = to % kScores;
-                    if (bar_test(&bars.p_ready[sb], (to / kScores) & 1) &&
-                        (pv.tile != p.tile0 || !pc || bar_test(&bars.o_free, (pc - 1) & 1)) &&
-                        bar_test(&bars.v_full[vs], (to / kVs) & 1)) {                 // O of tile `to`
-                        fence_after();
-                        const uint32_t vt = va + vs * S::kTileBytes, d = tmem + S::kO + HD * (to & 1), ap = tmem + kTile * sb;
-                        const uint32_t add = pv.tile - p.tile0 >= 2;
+                if (to < t && bar_test(&bars.p_ready[to % kScores], (to / kScores) & 1) &&
+                    (pv_done || !pc || bar_test(&bars.o_free, (pc - 1) & 1)) &&
+                    bar_test(&bars.v_full[to % kVs], (to / kVs) & 1)) {               // O of tile `to`
+                    fence_after();
+                    const uint32_t d = tmem + S::kO + HD * (to & 1), ap = tmem + kTile * (to % kScores);
+                    const uint64_t v = vd + (to % kVs) * (S::kTileBytes / 16);
+                    const uint32_t add = pv_done >= 2;
 #pragma unroll
-                        for (int q = 0; q < NT; ++q)
+                    for (int q = 0; q < NT; ++q)
 #pragma unroll
-                            for (int k = 0; k < kTile / 16; ++k)
-                                mma_ts(d, ap + 32 * q + 8 * k, umma_desc(vt + k * 2 * kGroupStride, kGroupStride, 128), id_o,
-                                       add | (q + k > 0));
-                        mma_commit(&bars.v_free[vs]);
-                        mma_commit(&bars.o_done[to & 1]);
-                        if (pv.tile == p.tile1 - 1) ++pc;
-                        ++to;
+                        for (int k = 0; k < kTile / 16; ++k)
+                            mma_ts(d, ap + 32 * q + 8 * k, v + k * (2 * kGroupStride / 16), id_o, q + k > 0 ? 1u : add);
+                    mma_commit(&bars.v_free[to % kVs]);
+                    mma_commit(&bars.o_done[to & 1]);
+                    ++to;
+                    ++pv_done;
+                    if (--pv_left == 0) {
+                        ++pc;
+                        pv.tile = pv.end - 1;
                         pv.next(list);
-                        idle = 0;
-                        continue;
+                        pv_left = pv.end - pv.tile;
+                        pv_done = 0;
                     }
-                }
-                if (qk.more(list) && t - to < kScores) {
-                    const Piece& p = list.piece[qk.piece];
-                    const unsigned ks = t % kKs, b = pq % S::kQs;
-                    if (bar_test(&bars.k_full[ks], (t / kKs) & 1) &&
-                        (qk.tile != p.tile0 || bar_test(&bars.q_full[b], (pq / S::kQs) & 1))) {   // S of tile t
-                        fence_after();
-                        const uint32_t kt = ka + ks * S::kTileBytes, qb = qa + b * NT * S::kQBytes, d = tmem + kTile * (t % kScores);
+                    idle = 0;
+                } else if (qk_left && t - to < kScores && bar_test(&bars.k_full[t % kKs], (t / kKs) & 1) &&
+                           (!q_new || bar_test(&bars.q_full[pq % S::kQs], (pq / S::kQs) & 1))) {   // S of tile t
+                    fence_after();
+                    q_new = false;
+                    const uint32_t d = tmem + kTile * (t % kScores);
+                    const uint64_t k0 = kd + (t % kKs) * (S::kTileBytes / 16), q0 = qd + (pq % S::kQs) * (NT * S::kQBytes / 16);
 #pragma unroll
-                        for (int q = 0; q < NT; ++q)
+                    for (int q = 0; q < NT; ++q)
 #pragma unroll
-                            for (int k = 0; k < HD / 16; ++k)
-                                mma_ss(d, umma_desc(qb + q * S::kQBytes + k * 256, 128, kGroupStride),
-                                       umma_desc(kt + k * 256, 128, kGroupStride), id_s, q + k > 0);
-                        mma_commit(&bars.s_ready[t % kScores]);
-                        mma_commit(&bars.k_free[ks]);
-                        if (qk.tile == p.tile1 - 1) mma_commit(&bars.q_free[b]), ++pq;
-                        ++t;
+                        for (int k = 0; k < HD / 16; ++k)
+                            mma_ss(d, q0 + q * (S::kQBytes / 16) + k * 16, k0 + k * 16, id_s, q + k > 0);
+                    mma_commit(&bars.s_ready[t % kScores]);
+                    mma_commit(&bars.k_free[t % kKs]);
+                    ++t;
+                    if (--qk_left == 0) {
+                        mma_commit(&bars.q_free[pq % S::kQs]);
+                        ++pq;
+                        qk.tile = qk.end - 1;
                         qk.next(list);
-                        idle = 0;
-                        continue;
+                        qk_left = qk.more(list) ? qk.end - qk.tile : 0;
+                        q_new = true;
                     }
-                }
-                if ((++idle & 1023u) == 0) {                     // as bounded as the other roles' waits
+                    idle = 0;
+                } else if ((++idle & 1023u) == 0) {              // as bounded as the other roles' waits
                     unsigned long long now;
                     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
                     if (idle == 1024u) since = now;
