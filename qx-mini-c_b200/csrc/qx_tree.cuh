@@ -274,7 +274,11 @@ struct RowScale {
 __device__ __forceinline__ float log_vs(float vs) {
     return vs >= 0.f ? fmaxf(__log2f(vs), kMinLogVs) : __int_as_float(0x7fc00000);
 }
-__device__ __forceinline__ float inv_vs(float vs) { return vs > 0x1p-90f ? __frcp_rn(vs) : 0x1p90f; }
+__device__ __forceinline__ float inv_vs(float vs) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(vs));   // one ulp
+    return vs > 0x1p-90f ? r : 0x1p90f;
+}
 
 // ---- visibility ----------------------------------------------------------------
 

@@ -5,13 +5,14 @@
 // Roles, by warp:
 //   0-3, 4-7   two softmax groups, which take the tiles in turn; a thread has
 //              one query row (TMEM lane), and each group its own reference,
-//              sum and output accumulator.  Both bring the query blocks, too
-//   8          issues the MMAs: S = Q K^T (128 x 64), then O += P V with P read
-//              from TMEM, where it overwrites the S it came from; whichever
-//              has its operands, S up to four tiles ahead of O
-//   9, 10      turn the INT8 codes into F16 operands
-//   11         asks for the codes, by TMA some tiles ahead, and makes the per-row
-//              constants of the scores
+//              sum and output accumulator
+//   8          issues S = Q K^T (128 x 64), up to four tiles ahead
+//   9          makes the per-row constants of the scores
+//   10         asks for the codes, by TMA some tiles ahead
+//   11         issues O += P V, P read from TMEM, where it overwrites the S it
+//              came from
+//   12-15      turn the INT8 codes into F16 operands, and bring the next piece's
+//              query block (the first one everybody)
 //
 // F16 operands are in the no-swizzle core-matrix layout: 8 rows x 16 bytes
 // each, [row / 8][dim / 8][row % 8].  That one layout is K-major for K (rows =
@@ -29,10 +30,14 @@ namespace qx {
 namespace ops {
 namespace {
 
-constexpr int kRows = 128, kGroup = 128, kTeam = 64, kTcThreads = 2 * kGroup + 128;
+constexpr int kRows = 128, kGroup = 128, kTeam = 128, kTcThreads = 512;
 constexpr int kKs = 2, kVs = 4;            // operand tiles: K goes once S is computed, V stays through the softmax
 constexpr int kScores = 4;                 // S buffers
-constexpr int kFacs = 8;                   // pieces whose row factors may be in use (queries run at most 6 ahead)
+// Row factors and "queries are there" of so many pieces: the queries of piece
+// P + 8 are brought once S of all of P + 6 is computed, a tile that is at least 6
+// past P's first; S runs less than 4 tiles ahead of O, so by then both groups
+// have had their first tiles of P.
+constexpr int kFacs = 8;
 
 template <int HD, int NT>
 struct Shape {
@@ -48,7 +53,7 @@ struct Shape {
 };
 
 struct Bars {
-    unsigned long long raw[4], raw_free[4], k_full[kKs], k_free[kKs], v_full[kVs], v_free[kVs], c_full[kVs], s_ready[kScores], p_ready[kScores], o_done[2], q_full[2], q_free[2],
+    unsigned long long raw[4], raw_free[4], k_full[kKs], k_free[kKs], v_full[kVs], v_free[kVs], c_full[kVs], s_ready[kScores], p_ready[kScores], o_done[2], q_full[kFacs], q_free[2],
         both, o_free;
 };
 struct alignas(16) Columns {
@@ -62,6 +67,12 @@ __device__ __forceinline__ void bar_init(unsigned long long* b, unsigned count) 
 __device__ __forceinline__ void bar_arrive(unsigned long long* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
 }
+// One arrival for the warp, after what its lanes did (32 arrivals on one word
+// take their turns in shared memory).
+__device__ __forceinline__ void warp_arrive(unsigned long long* b) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(b);
+}
 __device__ __forceinline__ bool bar_try(unsigned long long* b, unsigned parity) {
     uint32_t done;
     asm volatile(
@@ -71,14 +82,10 @@ __device__ __forceinline__ bool bar_try(unsigned long long* b, unsigned parity) 
         : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool bar_test(unsigned long long* b, unsigned parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(smem_addr(b)), "r"(parity)
-        : "memory");
-    return done != 0;
+__device__ __forceinline__ bool elected() {
+    uint32_t is;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+    return is != 0;
 }
 // Bounded wait for a phase (2 s; a healthy one takes microseconds).  Gives up
 // soon after another role has, unless it is for work of its own in flight.
@@ -195,25 +202,22 @@ __device__ __forceinline__ void widen(const uint4& w, uint8_t* to) {
     *reinterpret_cast<uint4*>(to) = make_uint4(low_pair(c[0]), high_pair(c[0]), low_pair(c[1]), high_pair(c[1]));
     *reinterpret_cast<uint4*>(to + 128) = make_uint4(low_pair(c[2]), high_pair(c[2]), low_pair(c[3]), high_pair(c[3]));
 }
-// A tile's codes of K or V to F16, by two warps: a warp takes eight rows of four
-// 16-byte chunks at a time, four such units' reads before their writes.
+// A tile's codes of K or V to F16, by four warps: a warp takes eight rows of
+// four 16-byte chunks at a time, all its reads before its writes.
 template <int HD>
 __device__ __forceinline__ void widen_tile(const uint8_t* raw, int bt, uint8_t* to) {
-    constexpr int kUnits = kTile / 8 * (HD / 64), kBatch = 4;
+    constexpr int kMine = kTile / 8 * (HD / 64) / 4;
     const int lane = bt & 31, r8 = lane & 7, c4 = lane >> 3, w = bt >> 5;
-    // unit 2 i + w: with 128 dims chunks 4 w .. 4 w + 3 of rows 8 i .., with 64 rows 8 (2 i + w) ..
-    const int chunk = (HD == 128 ? 4 * w : 0) + c4, row0 = HD == 128 ? 0 : 8 * w;
-    constexpr int kStep = HD == 128 ? 8 : 16;                  // rows from one of a warp's units to the next
+    // with 128 dims chunks 4 (w % 2) .. and every second eight rows from 8 (w / 2), with 64 every fourth from 8 w
+    const int chunk = (HD == 128 ? 4 * (w & 1) : 0) + c4, row0 = HD == 128 ? 8 * (w >> 1) : 8 * w;
+    constexpr int kStep = HD == 128 ? 16 : 32;
     raw += (row0 + r8) * HD + (HD == 128 ? chunk ^ r8 : chunk ^ (r8 >> 1)) * 16;
     to += row0 / 8 * (HD / 8 * 128) + chunk * 256 + r8 * 16;
+    uint4 x[kMine];
 #pragma unroll
-    for (int i = 0; i < kUnits / 2; i += kBatch) {
-        uint4 x[kBatch];
+    for (int i = 0; i < kMine; ++i) x[i] = *reinterpret_cast<const uint4*>(raw + i * kStep * HD);
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) x[k] = *reinterpret_cast<const uint4*>(raw + (i + k) * kStep * HD);
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) widen(x[k], to + (i + k) * (kStep / 8) * (HD / 8 * 128));
-    }
+    for (int i = 0; i < kMine; ++i) widen(x[i], to + i * (kStep / 8) * (HD / 8 * 128));
 }
 __device__ __forceinline__ void tma_tile(uint32_t to, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
@@ -222,15 +226,15 @@ __device__ __forceinline__ void tma_tile(uint32_t to, const CUtensorMap* map, in
 }
 
 // The query block of a piece as F16 terms, and the factors that undo the rows'
-// powers of two; both softmax groups, two neighbouring lanes to a row, which
-// take its units of eight values in turn.
+// powers of two: eight rows by a warp, four lanes to a row, which take its units
+// of eight values in turn.
 template <class T, int HD, int NT>
-__device__ __noinline__ void stage_queries(const TreeArgs& a, const Piece& p, int tid, uint8_t* qt, float* fac) {
-    constexpr int V = 16 / sizeof(T), kSteps = HD / 16, kPacks = 8 / V;
-    const int row = tid >> 1, half = tid & 1, r = p.row0 + row;
+__device__ __noinline__ void stage_queries(const TreeArgs& a, const Piece& p, int row0, uint8_t* qt, float* fac) {
+    constexpr int V = 16 / sizeof(T), kSteps = HD / 32, kPacks = 8 / V;
+    const int lane = threadIdx.x & 31, r8 = lane & 7, c4 = lane >> 3, row = row0 + r8, r = p.row0 + row;
     const bool real = row < p.have;
     const T* src = (const T*)a.q.p + p.s * a.q.seq + (real ? r / a.group : 0) * a.q.node +
-                   (size_t)(p.g * a.group + (real ? r % a.group : 0)) * a.q.head + half * 8;
+                   (size_t)(p.g * a.group + (real ? r % a.group : 0)) * a.q.head + c4 * 8;
     Pack<T, V> x[kSteps][kPacks];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
@@ -238,53 +242,40 @@ __device__ __noinline__ void stage_queries(const TreeArgs& a, const Piece& p, in
         for (int k = 0; k < kPacks; ++k) {
 #pragma unroll
             for (int u = 0; u < V; ++u) x[i][k].v[u] = from_f32<T>(0.f);
-            if (real && a.wide) x[i][k] = *reinterpret_cast<const Pack<T, V>*>(src + 16 * i + V * k);
+            if (real && a.wide) x[i][k] = *reinterpret_cast<const Pack<T, V>*>(src + 32 * i + V * k);
         }
     if (real && !a.wide)
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-            for (int k = 0; k < kPacks; ++k)
-#pragma unroll
-                for (int u = 0; u < V; ++u) x[i][k].v[u] = src[16 * i + V * k + u];
+            for (int e = 0; e < 8; ++e) x[i][e / V].v[e % V] = src[32 * i + e];
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float y = to_f32(x[i][e / V].v[e % V]);
-            big = fmaxf(big, isfinite(y) ? fabsf(y) : 0.f);
+            const float y = fabsf(to_f32(x[i][e / V].v[e % V]));
+            big = fmaxf(big, y <= 3.402823466e38f ? y : 0.f);
         }
-    big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(~0u, big, 8));
+    big = fmaxf(big, __shfl_xor_sync(~0u, big, 16));
     const RowScale rs(big);
-    uint8_t* to = qt + (row >> 3) * (HD / 8 * 128) + (row & 7) * 16 + half * 128;
+    uint8_t* to = qt + (row >> 3) * (HD / 8 * 128) + r8 * 16 + c4 * 128;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = to_f32(x[i][e / V].v[e % V]) * rs.f0 * rs.f1;
         const uint4 hi = make_uint4(pack_half(y[0], y[1]), pack_half(y[2], y[3]), pack_half(y[4], y[5]), pack_half(y[6], y[7]));
-        *reinterpret_cast<uint4*>(to + i * 256) = hi;
+        *reinterpret_cast<uint4*>(to + i * 512) = hi;
         if (NT == 2)
-            *reinterpret_cast<uint4*>(to + Shape<HD, NT>::kQBytes + i * 256) =
+            *reinterpret_cast<uint4*>(to + Shape<HD, NT>::kQBytes + i * 512) =
                 make_uint4(rest_half(y[0], y[1], hi.x), rest_half(y[2], y[3], hi.y), rest_half(y[4], y[5], hi.z),
                            rest_half(y[6], y[7], hi.w));
     }
-    if (half == 0) fac[row] = rs.undo(a.scale);
+    if (c4 == 0) fac[row] = rs.undo(a.scale);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-
-// A place in the list: the pieces that have tiles, tile by tile.
-struct At {
-    int piece, tile, end;
-    __device__ __forceinline__ explicit At(const PieceList& l) : piece(-1), tile(0), end(0) { next(l); }
-    __device__ __forceinline__ void next(const PieceList& l) {
-        ++tile;
-        while (tile >= end && piece < l.count) {
-            if (++piece < l.count) tile = l.piece[piece].tile0, end = l.piece[piece].tile1;
-        }
-    }
-    __device__ __forceinline__ bool more(const PieceList& l) const { return piece < l.count; }
-};
 
 // ---- the kernel ----------------------------------------------------------------
 
@@ -319,18 +310,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
     }
     if (tid == 0) {
         gave_up = 0;
-        for (int i = 0; i < 4; ++i) bar_init(&bars.raw[i], 1), bar_init(&bars.raw_free[i], kTeam);
-        for (int i = 0; i < kKs; ++i) bar_init(&bars.k_full[i], kTeam), bar_init(&bars.k_free[i], 1);
-        for (int i = 0; i < kVs; ++i) bar_init(&bars.v_full[i], kTeam), bar_init(&bars.v_free[i], 1), bar_init(&bars.c_full[i], 32);
-        for (int i = 0; i < kScores; ++i) bar_init(&bars.s_ready[i], 1), bar_init(&bars.p_ready[i], kGroup);
-        for (int i = 0; i < 2; ++i) bar_init(&bars.o_done[i], 1), bar_init(&bars.q_full[i], 2 * kGroup), bar_init(&bars.q_free[i], 1);
-        bar_init(&bars.both, 2 * kGroup);
-        bar_init(&bars.o_free, 2 * kGroup);
+        for (int i = 0; i < 4; ++i) bar_init(&bars.raw[i], 1), bar_init(&bars.raw_free[i], kTeam / 32);
+        for (int i = 0; i < kKs; ++i) bar_init(&bars.k_full[i], kTeam / 32), bar_init(&bars.k_free[i], 1);
+        for (int i = 0; i < kVs; ++i) bar_init(&bars.v_full[i], kTeam / 32), bar_init(&bars.v_free[i], 1), bar_init(&bars.c_full[i], 1);
+        for (int i = 0; i < kScores; ++i) bar_init(&bars.s_ready[i], 1), bar_init(&bars.p_ready[i], kGroup / 32);
+        for (int i = 0; i < 2; ++i) bar_init(&bars.o_done[i], 1), bar_init(&bars.q_free[i], 1);
+        for (int i = 0; i < kFacs; ++i) bar_init(&bars.q_full[i], kTeam / 32);
+        bar_init(&bars.both, 2 * kGroup / 32);
+        bar_init(&bars.o_free, 2 * kGroup / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // the first piece's queries, if it has tiles (a part may lie past what its rows see)
+    const bool eager = list.piece[0].tile1 > list.piece[0].tile0;
+    if (eager) stage_queries<T, HD, NT>(a, list.piece[0], warp * 8, q_s, fac_s[0]);
     fence_before();
     __syncthreads();
     fence_after();
+    if (eager && tid < kTeam / 32) bar_arrive(&bars.q_full[0]);
     const uint32_t tmem = tmem_s;
     unsigned t = 0, pc = 0;                                      // tiles and pieces of the lists before
     for (int batch = 0;; ++batch) {
@@ -340,26 +336,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
             const int w = warp >> 2, row = tid & 127;
             const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), to = lanes + S::kO + HD * w;
             bool ok = !gave_up;
-            unsigned qc = pc;                                    // query blocks staged
-            At q_at(list);
-            auto stage = [&]() {
-                if (!q_at.more(list)) return;
-                const unsigned b = qc % S::kQs, use = qc / S::kQs;
-                if (use) ok = bar_wait(&bars.q_free[b], (use - 1) & 1, &gave_up) && ok;
-                ok = __all_sync(~0u, ok);
-                if (!ok) return;
-                stage_queries<T, HD, NT>(a, list.piece[q_at.piece], tid, q_s + b * NT * S::kQBytes, fac_s[qc % kFacs]);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(&bars.q_full[b]);
-                ++qc;
-                q_at.tile = q_at.end - 1;                        // on to the next piece with tiles
-                q_at.next(list);
-            };
-            stage();
             for (int i = 0; ok && i < count; ++i) {
                 const Piece& p = list.piece[i];
-                if (S::kQs == 2 && p.tile1 > p.tile0) stage();   // the next piece's, before this one's tiles
-                if (!ok) break;
                 const int nt = max(0, p.tile1 - p.tile0), j0 = (w ^ t) & 1;
                 const int node = row < p.have ? (p.row0 + row) / a.group : -1;
                 float m = -INFINITY, fac = 0.f;
@@ -367,77 +345,96 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                 for (int j = j0; j < nt; j += 2) {
                     const unsigned tt = t + j, st = tt % kVs;
                     const uint32_t ts = lanes + kTile * (tt % kScores);
-                    ok = (j != j0 || bar_wait(&bars.q_full[pc % S::kQs], (pc / S::kQs) & 1, &gave_up)) &&
+                    ok = (j != j0 || bar_wait(&bars.q_full[pc % kFacs], (pc / kFacs) & 1, &gave_up)) &&
                          bar_wait(&bars.c_full[st], (tt / kVs) & 1, &gave_up) &&
                          bar_wait(&bars.s_ready[tt % kScores], (tt / kScores) & 1, &gave_up);
                     ok = __all_sync(~0u, ok);                    // and the warp is one again for what follows
                     if (!ok) break;
                     fence_after();
                     if (j == j0) fac = fac_s[pc % kFacs][row];
-                    float2 x[32];
-                    tmem_ld32(ts, reinterpret_cast<uint32_t*>(x));
-                    tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(x + 16));
                     const Columns& col = cols[st];
                     const float2 fac2 = make_float2(fac, fac);
-                    wait_ld();
-                    loaded(x);
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float4 k = *reinterpret_cast<const float4*>(&col.ks[2 * c]), v = *reinterpret_cast<const float4*>(&col.lv[2 * c]);
-                        x[c] = fma2(mul2(x[c], fac2), make_float2(k.x, k.y), make_float2(v.x, v.y));
-                        x[c + 1] = fma2(mul2(x[c + 1], fac2), make_float2(k.z, k.w), make_float2(v.z, v.w));
-                    }
                     const int t0 = (p.tile0 + j) * kTile;
-                    if (t0 + kTile > p.len) {
-                        const unsigned long long see =
-                            node < 0 ? 0ull
-                                     : sees64(a.mask ? a.mask + ((size_t)p.s * a.d.max_nodes + node) * a.words : nullptr, a.words, node,
-                                              t0, p.len, p.n);
-                        const uint32_t lo = (uint32_t)see, hi = (uint32_t)(see >> 32);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            const uint32_t bits = c < 16 ? lo : hi;
-                            if (!(bits >> (2 * (c & 15)) & 1u)) x[c].x = -INFINITY;
-                            if (!(bits >> (2 * (c & 15) + 1) & 1u)) x[c].y = -INFINITY;
-                        }
-                    }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], fmaxf(x[c].x, x[c].y));
-                    const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    const bool raise = big > m + kSlack || (m == -INFINITY && big > -INFINITY);
-                    if (__any_sync(~0u, raise)) {
-                        const float f = raise ? exp2_fast(m - big) : 1.f;
-                        if (raise) m = big;
-                        l2 = mul2(l2, make_float2(f, f));
-                        if (j != j0) {                           // an accumulator to rescale, once its last product is in
-                            ok = bar_wait(&bars.o_done[w], ((tt - 2) >> 1) & 1, &gave_up);
-                            ok = __all_sync(~0u, ok);
-                            if (!ok) break;
-                            fence_after();
+                    const bool edge = t0 + kTile > p.len;
+                    unsigned long long see = 0ull;
+                    if (edge && node >= 0)
+                        see = sees64(a.mask ? a.mask + ((size_t)p.s * a.d.max_nodes + node) * a.words : nullptr, a.words, node, t0, p.len, p.n);
+                    // 32 columns at a time, in a loop: half the registers, and half the code to fetch
 #pragma unroll 1
-                            for (int c = 0; c < HD; c += 16) {
-                                float2 o[8];
-                                tmem_ld16(to + c, reinterpret_cast<uint32_t*>(o));
-                                wait_ld();
-                                loaded(o);
+                    for (int h = 0; h < 2; ++h) {
+                        float2 x[16];
+                        tmem_ld32(ts + 32 * h, reinterpret_cast<uint32_t*>(x));
+                        wait_ld();
+                        loaded(x);
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) o[e] = mul2(o[e], make_float2(f, f));
-                                tmem_st16(to + c, reinterpret_cast<const uint32_t*>(o));
+                        for (int c = 0; c < 16; c += 2) {
+                            const float4 k = *reinterpret_cast<const float4*>(&col.ks[32 * h + 2 * c]),
+                                         v = *reinterpret_cast<const float4*>(&col.lv[32 * h + 2 * c]);
+                            x[c] = fma2(mul2(x[c], fac2), make_float2(k.x, k.y), make_float2(v.x, v.y));
+                            x[c + 1] = fma2(mul2(x[c + 1], fac2), make_float2(k.z, k.w), make_float2(v.z, v.w));
+                        }
+                        if (edge) {
+                            const uint32_t bits = (uint32_t)(see >> (32 * h));
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) {
+                                if (!(bits >> (2 * c) & 1u)) x[c].x = -INFINITY;
+                                if (!(bits >> (2 * c + 1) & 1u)) x[c].y = -INFINITY;
                             }
                         }
-                    }
-                    const float up = kPBias - (m == -INFINITY ? 0.f : m);
-                    const float2 up2 = make_float2(up, up);
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                        for (int c = 0; c < 16; ++c) mx[c & 3] = fmaxf(mx[c & 3], fmaxf(x[c].x, x[c].y));
+                        const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        const bool raise = big > m + kSlack || (m == -INFINITY && big > -INFINITY);
+                        if (__any_sync(~0u, raise)) {            // rare once a row has seen some of its scores
+                            // a whole number of powers of two, so that what is rescaled loses no bits
+                            const float m1 = raise ? (m == -INFINITY ? big : m + ceilf(big - m)) : m;
+                            const float f = raise ? exp2_fast(m - m1) : 1.f;
+                            m = m1;
+                            l2 = mul2(l2, make_float2(f, f));
+                            if (j != j0) {                       // the accumulator, once its last product is in
+                                ok = bar_wait(&bars.o_done[w], ((tt - 2) >> 1) & 1, &gave_up);
+                                ok = __all_sync(~0u, ok);
+                                if (!ok) break;
+                                fence_after();
+#pragma unroll 1
+                                for (int c = 0; c < HD; c += 16) {
+                                    float2 o[8];
+                                    tmem_ld16(to + c, reinterpret_cast<uint32_t*>(o));
+                                    wait_ld();
+                                    loaded(o);
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) o[e] = mul2(o[e], make_float2(f, f));
+                                    tmem_st16(to + c, reinterpret_cast<const uint32_t*>(o));
+                                }
+                            }
+                            if (h) {                             // and the weights of the first half
+#pragma unroll 1
+                                for (int q = 0; q < NT; ++q) {
+                                    float2 w2[8];
+                                    uint32_t* u = reinterpret_cast<uint32_t*>(w2);
+                                    wait_st();
+                                    tmem_ld16(ts + 16 * q, u);
+                                    wait_ld();
+                                    loaded(w2);
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e) {
+                                        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(u + e));
+                                        u[e] = pack_half(g.x * f, g.y * f);
+                                    }
+                                    tmem_st16(ts + 16 * q, u);
+                                }
+                            }
+                        }
+                        const float up = kPBias - (m == -INFINITY ? 0.f : m);
+                        const float2 up2 = make_float2(up, up);
                         uint32_t ph[16], pl[16];
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
                             const float4 iv = *reinterpret_cast<const float4*>(&col.iv[32 * h + 2 * c]);
 #pragma unroll
                             for (int u = 0; u < 2; ++u) {
-                                float2 e = add2(x[16 * h + c + u], up2);
+                                float2 e = add2(x[c + u], up2);
                                 e.x = exp2_fast(e.x);
                                 e.y = exp2_fast(e.y);
                                 l2 = fma2(e, u ? make_float2(iv.z, iv.w) : make_float2(iv.x, iv.y), l2);
@@ -445,15 +442,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                                 if (NT == 2) pl[c + u] = rest_half(e.x, e.y, ph[c + u]);
                             }
                         }
-                        tmem_st16(ts + 16 * h, ph);
-                        if (NT == 2) tmem_st16(ts + 32 + 16 * h, pl);
+                        // P of 32 columns over their S: 16 registers of the first term, 16 of the rest
+                        tmem_st16(ts + 32 * h, ph);
+                        if (NT == 2) tmem_st16(ts + 32 * h + 16, pl);
                     }
+                    if (!ok) break;
                     wait_st();
+                    // The group's products before this one, each in its turn: a wait tells a phase from the next only, so
+                    // none may be passed over.  Long done, as a rule.
+                    if (tt >= 2) ok = bar_wait(&bars.o_done[w], ((tt - 2) >> 1) & 1, &gave_up);
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
                     fence_before();
-                    bar_arrive(&bars.p_ready[tt % kScores]);
+                    warp_arrive(&bars.p_ready[tt % kScores]);
                 }
-                if (!ok) break;
-                if (S::kQs == 1 && nt > 0) stage();              // one block: once this piece's scores are all computed
                 if (!ok) break;
                 // both groups' references and sums, then half of the dims each
                 float* part = part_of(a, blockIdx.x, p.begins) + (size_t)row * (kPartHead + HD);
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                         const unsigned last = t + nt - 1 - ((nt - 1 - j0) & 1);
                         ok = bar_wait(&bars.o_done[w], (last >> 1) & 1, &gave_up);
                     }
-                    bar_arrive(&bars.both);
+                    warp_arrive(&bars.both);
                     ok = bar_wait(&bars.both, pc & 1, &gave_up) && ok;
                     ok = __all_sync(~0u, ok);
                     if (!ok) break;
@@ -518,7 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                         else part[0] = top, part[1] = sum;
                     }
                     fence_before();
-                    bar_arrive(&bars.o_free);
+                    warp_arrive(&bars.o_free);
                     ++pc;
                 } else if (node >= 0) {                          // no row of the block sees these tiles
 #pragma unroll 1
@@ -528,162 +530,188 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                 }
                 t += nt;
             }
-        } else if (warp == 9 || warp == 10) {
-            // ---- widen the codes ----
-            const int bt = tid - 2 * kGroup - 32;
+        } else if (warp >= 12) {
+            // ---- widen the codes, bring the queries ----
+            const int bt = tid - 384;
             bool ok = !gave_up;
-            for (At here(list); ok && here.more(list); here.next(list), ++t) {
-                const unsigned ks = t % kKs, vs = t % kVs, slot = t % S::kAhead;
-                const uint8_t* raw = raw_s + slot * 2 * S::kRawBytes;
-                ok = bar_wait(&bars.raw[slot], (t / S::kAhead) & 1, &gave_up);
-                if (ok && t >= kKs) ok = bar_wait(&bars.k_free[ks], (t / kKs - 1) & 1, &gave_up);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                widen_tile<HD>(raw, bt, k_s + ks * S::kTileBytes);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(&bars.k_full[ks]);
-                if (t >= kVs) ok = bar_wait(&bars.v_free[vs], (t / kVs - 1) & 1, &gave_up);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                widen_tile<HD>(raw + S::kRawBytes, bt, v_s + vs * S::kTileBytes);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(&bars.v_full[vs]);
-                bar_arrive(&bars.raw_free[slot]);
-            }
-        } else if (warp == 11) {
-            // ---- ask for the codes, make the columns' constants ----
-            const uint32_t raw_a = smem_addr(raw_s);
-            bool ok = !gave_up;
-            unsigned sent = t;                                   // tiles asked for
-            At to_send(list), soon(list);
-            auto send = [&]() {
-                if (!to_send.more(list)) return;
-                if (lane == 0) {
-                    const Piece& p = list.piece[to_send.piece];
-                    const unsigned slot = sent % S::kAhead;
-                    const uint32_t bar = smem_addr(&bars.raw[slot]), to = raw_a + slot * 2 * S::kRawBytes;
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * S::kRawBytes) : "memory");
-                    const int y = (int)p.base_row + to_send.tile * kTile;
-                    tma_tile(to, &maps.k, p.g * HD, y, bar);
-                    tma_tile(to + S::kRawBytes, &maps.v, p.g * HD, y, bar);
-                }
-                ++sent;
-                to_send.next(list);
-            };
+            unsigned qc = pc;                                    // query blocks staged
+            int q_at = -1;                                       // the piece of the last
+            auto stage = [&]() {                                 // the next piece's, if there is one
+                do ++q_at;
+                while (q_at < count && list.piece[q_at].tile1 <= list.piece[q_at].tile0);
+                if (q_at >= count) return;
+                if (qc || !eager) {
+                    const unsigned b = qc % S::kQs, use = qc / S::kQs;
+                    if (use) ok = bar_wait(&bars.q_free[b], (use - 1) & 1, &gave_up) && ok;
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) return;
 #pragma unroll 1
-            for (int d = 0; d < S::kAhead; ++d) send();
-            // the scales of rows 2 lane and 2 lane + 1, a tile ahead
-            auto scales = [&]() {
-                if (!soon.more(list)) return make_float4(0.f, 0.f, 0.f, 0.f);
-                const Piece& p = list.piece[soon.piece];
-                const int last = p.len + p.n - 1, r = soon.tile * kTile + 2 * lane;
-                const size_t r0 = p.base_row + min(r, last), r1 = p.base_row + min(r + 1, last);
-                soon.next(list);
-                return make_float4(__ldg(a.c.ks + r0), __ldg(a.c.ks + r1), __ldg(a.c.vs + r0), __ldg(a.c.vs + r1));
+                    for (int r = 0; r < kRows; r += 8 * (kTeam / 32))
+                        stage_queries<T, HD, NT>(a, list.piece[q_at], r + 8 * (bt >> 5), q_s + b * NT * S::kQBytes, fac_s[qc % kFacs]);
+                    warp_arrive(&bars.q_full[qc % kFacs]);
+                }
+                ++qc;
             };
-            float4 sc = scales();
-            for (At here(list); here.more(list); here.next(list), ++t) {
-                const unsigned vs = t % kVs;
-                const float4 now = sc;
-                sc = scales();
-                if (t >= kVs) ok = bar_wait(&bars.v_free[vs], (t / kVs - 1) & 1, &gave_up);
-                ok = __all_sync(~0u, ok);
-                if (!ok) break;
-                *reinterpret_cast<float2*>(&cols[vs].ks[2 * lane]) = make_float2(now.x, now.y);
-                *reinterpret_cast<float2*>(&cols[vs].lv[2 * lane]) = make_float2(log_vs(now.z), log_vs(now.w));
-                *reinterpret_cast<float2*>(&cols[vs].iv[2 * lane]) = make_float2(inv_vs(now.z), inv_vs(now.w));
-                bar_arrive(&bars.c_full[vs]);
-                if (to_send.more(list)) {                        // once its team has read the tile's codes
-                    ok = bar_wait(&bars.raw_free[t % S::kAhead], (t / S::kAhead) & 1, &gave_up);
+            stage();
+            for (int i = 0; ok && i < count; ++i) {
+                const int nt = list.piece[i].tile1 - list.piece[i].tile0;
+                for (int j = 0; j < nt; ++j, ++t) {
+                    const unsigned ks = t % kKs, vs = t % kVs, slot = t % S::kAhead;
+                    const uint8_t* raw = raw_s + slot * 2 * S::kRawBytes;
+                    ok = bar_wait(&bars.raw[slot], (t / S::kAhead) & 1, &gave_up);
+                    if (ok && t >= kKs) ok = bar_wait(&bars.k_free[ks], (t / kKs - 1) & 1, &gave_up);
                     ok = __all_sync(~0u, ok);
                     if (!ok) break;
-                    send();
-                }
-            }
-            // copies of this CTA still on their way, if a wait gave up
-            if (!ok)
-                for (unsigned i = sent > S::kAhead ? sent - S::kAhead : 0; i < sent; ++i)
-                    bar_wait(&bars.raw[i % S::kAhead], (i / S::kAhead) & 1, &gave_up, true);
-        } else if (lane == 0) {
-            // ---- issue the products ----
-            constexpr uint32_t kGroupStride = HD / 8 * 128;       // eight rows
-            constexpr uint32_t id_s = idesc_f16(kRows, kTile, false), id_o = idesc_f16(kRows, HD, true);
-            // descriptors of the operands' first blocks; others are so many 16-byte units further
-            const uint64_t qd = umma_desc(smem_addr(q_s), 128, kGroupStride), kd = umma_desc(smem_addr(k_s), 128, kGroupStride),
-                           vd = umma_desc(smem_addr(v_s), kGroupStride, 128);
-            bool ok = !gave_up;
-            At qk(list), pv(list);                               // the pieces of the first and the second product
-            int qk_left = qk.more(list) ? qk.end - qk.tile : 0, pv_left = pv.end - pv.tile;
-            int pv_done = 0;                                     // tiles of the second's piece that are done
-            const unsigned t0 = t;
-            unsigned to = t, pq = pc;                            // tile of the second product; piece of the first
-            bool q_new = true;                                   // the first's queries are still to be waited for
-            unsigned idle = 0;
-            unsigned long long since = 0;
-            while (pv.more(list)) {
-                if (to < t && bar_test(&bars.p_ready[to % kScores], (to / kScores) & 1) &&
-                    (pv_done || !pc || bar_test(&bars.o_free, (pc - 1) & 1)) &&
-                    bar_test(&bars.v_full[to % kVs], (to / kVs) & 1)) {               // O of tile `to`
-                    fence_after();
-                    const uint32_t d = tmem + S::kO + HD * (to & 1), ap = tmem + kTile * (to % kScores);
-                    const uint64_t v = vd + (to % kVs) * (S::kTileBytes / 16);
-                    const uint32_t add = pv_done >= 2;
-#pragma unroll
-                    for (int q = 0; q < NT; ++q)
-#pragma unroll
-                        for (int k = 0; k < kTile / 16; ++k)
-                            mma_ts(d, ap + 32 * q + 8 * k, v + k * (2 * kGroupStride / 16), id_o, q + k > 0 ? 1u : add);
-                    mma_commit(&bars.v_free[to % kVs]);
-                    mma_commit(&bars.o_done[to & 1]);
-                    ++to;
-                    ++pv_done;
-                    if (--pv_left == 0) {
-                        ++pc;
-                        pv.tile = pv.end - 1;
-                        pv.next(list);
-                        pv_left = pv.end - pv.tile;
-                        pv_done = 0;
-                    }
-                    idle = 0;
-                } else if (qk_left && t - to < kScores && bar_test(&bars.k_full[t % kKs], (t / kKs) & 1) &&
-                           (!q_new || bar_test(&bars.q_full[pq % S::kQs], (pq / S::kQs) & 1))) {   // S of tile t
-                    fence_after();
-                    q_new = false;
-                    const uint32_t d = tmem + kTile * (t % kScores);
-                    const uint64_t k0 = kd + (t % kKs) * (S::kTileBytes / 16), q0 = qd + (pq % S::kQs) * (NT * S::kQBytes / 16);
-#pragma unroll
-                    for (int q = 0; q < NT; ++q)
-#pragma unroll
-                        for (int k = 0; k < HD / 16; ++k)
-                            mma_ss(d, q0 + q * (S::kQBytes / 16) + k * 16, k0 + k * 16, id_s, q + k > 0);
-                    mma_commit(&bars.s_ready[t % kScores]);
-                    mma_commit(&bars.k_free[t % kKs]);
-                    ++t;
-                    if (--qk_left == 0) {
-                        mma_commit(&bars.q_free[pq % S::kQs]);
-                        ++pq;
-                        qk.tile = qk.end - 1;
-                        qk.next(list);
-                        qk_left = qk.more(list) ? qk.end - qk.tile : 0;
-                        q_new = true;
-                    }
-                    idle = 0;
-                } else if ((++idle & 1023u) == 0) {              // as bounded as the other roles' waits
-                    unsigned long long now;
-                    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-                    if (idle == 1024u) since = now;
-                    if (*(volatile int*)&gave_up || now - since > 2000000000ull) {
-                        *(volatile int*)&gave_up = 1;
-                        ok = false;
+                    widen_tile<HD>(raw, bt, k_s + ks * S::kTileBytes);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    warp_arrive(&bars.k_full[ks]);
+                    if (t >= kVs) ok = bar_wait(&bars.v_free[vs], (t / kVs - 1) & 1, &gave_up);
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                    widen_tile<HD>(raw + S::kRawBytes, bt, v_s + vs * S::kTileBytes);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    warp_arrive(&bars.v_full[vs]);
+                    warp_arrive(&bars.raw_free[slot]);
+                    // with two blocks, while the softmax still has tiles of this piece before it; with one, behind its last S
+                    if (j == (S::kQs == 2 ? min(nt, kVs) : nt) - 1) stage();
+                    if (!ok) {
+                        ++t;
                         break;
                     }
                 }
             }
-            // the last products are in before TMEM goes (the softmax groups have waited for them, unless a wait gave up)
-            if (!ok) {
-                for (unsigned i = t > t0 + kScores ? t - kScores : t0; i < t; ++i)
-                    bar_wait(&bars.s_ready[i % kScores], (i / kScores) & 1, &gave_up, true);
-                for (unsigned i = to > t0 + 2 ? to - 2 : t0; i < to; ++i) bar_wait(&bars.o_done[i & 1], (i >> 1) & 1, &gave_up, true);
+        } else if (warp == 10) {
+            // ---- ask for the codes ----
+            const uint32_t raw_a = smem_addr(raw_s);
+            const unsigned t0 = t;
+            bool ok = !gave_up;
+            for (int i = 0; ok && i < count; ++i) {
+                const Piece& p = list.piece[i];
+                const int x = p.g * HD;
+                int y = (int)p.base_row + p.tile0 * kTile;
+                for (int left = p.tile1 - p.tile0; left > 0; --left, ++t, y += kTile) {
+                    const unsigned slot = t % S::kAhead, use = t / S::kAhead;
+                    if (use) ok = bar_wait(&bars.raw_free[slot], (use - 1) & 1, &gave_up);   // the codes before have been read
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        const uint32_t bar = smem_addr(&bars.raw[slot]), to = raw_a + slot * 2 * S::kRawBytes;
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * S::kRawBytes) : "memory");
+                        tma_tile(to, &maps.k, x, y, bar);
+                        tma_tile(to + S::kRawBytes, &maps.v, x, y, bar);
+                    }
+                    __syncwarp();
+                }
+            }
+            // copies still on their way, if a wait gave up
+            if (!ok)
+                for (unsigned i = t > t0 + S::kAhead ? t - S::kAhead : t0; i < t; ++i)
+                    bar_wait(&bars.raw[i % S::kAhead], (i / S::kAhead) & 1, &gave_up, true);
+        } else if (warp == 9) {
+            // ---- make the columns' constants ----
+            bool ok = !gave_up;
+            for (int i = 0; ok && i < count; ++i) {
+                const Piece& p = list.piece[i];
+                const int last = p.len + p.n - 1, end = p.tile1;
+                int tile = p.tile0;
+                if (tile >= end) continue;
+                // the scales of rows 2 lane and 2 lane + 1, a tile ahead
+                const float *ks = a.c.ks + p.base_row, *vs = a.c.vs + p.base_row;
+                auto scales = [&](int at) {
+                    const int r0 = min(at * kTile + 2 * lane, last), r1 = min(at * kTile + 2 * lane + 1, last);
+                    return make_float4(__ldg(ks + r0), __ldg(ks + r1), __ldg(vs + r0), __ldg(vs + r1));
+                };
+                float4 sc = scales(tile);
+                for (; tile < end; ++tile, ++t) {
+                    const unsigned st = t % kVs;
+                    const float4 now = sc;
+                    if (tile + 1 < end) sc = scales(tile + 1);
+                    if (t >= kVs) ok = bar_wait(&bars.v_free[st], (t / kVs - 1) & 1, &gave_up);
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                    *reinterpret_cast<float2*>(&cols[st].ks[2 * lane]) = make_float2(now.x, now.y);
+                    *reinterpret_cast<float2*>(&cols[st].lv[2 * lane]) = make_float2(log_vs(now.z), log_vs(now.w));
+                    *reinterpret_cast<float2*>(&cols[st].iv[2 * lane]) = make_float2(inv_vs(now.z), inv_vs(now.w));
+                    warp_arrive(&bars.c_full[st]);
+                }
+            }
+        } else {
+            // ---- issue the products ----
+            // The whole warp goes along, so that what the instructions take is uniform; one lane issues.
+            constexpr uint32_t kGroupStride = HD / 8 * 128;       // eight rows
+            const bool issues = elected();
+            const unsigned t0 = t;
+            bool ok = !gave_up;
+            if (warp == 8) {
+                constexpr uint32_t id = idesc_f16(kRows, kTile, false);
+                // descriptors of the operands' first blocks; others are so many 16-byte units further
+                const uint64_t qd = umma_desc(smem_addr(q_s), 128, kGroupStride), kd = umma_desc(smem_addr(k_s), 128, kGroupStride);
+                for (int i = 0; ok && i < count; ++i) {
+                    int left = list.piece[i].tile1 - list.piece[i].tile0;
+                    if (left <= 0) continue;
+                    const uint64_t q0 = qd + (pc % S::kQs) * (NT * S::kQBytes / 16);
+                    ok = __all_sync(~0u, bar_wait(&bars.q_full[pc % kFacs], (pc / kFacs) & 1, &gave_up));
+                    for (; ok && left > 0; --left, ++t) {
+                        const unsigned ks = t % kKs, sb = t % kScores;
+                        // the keys; and the buffer: P of four tiles before has been used
+                        ok = bar_wait(&bars.k_full[ks], (t / kKs) & 1, &gave_up) &&
+                             (t < kScores || bar_wait(&bars.v_free[t % kVs], (t / kVs - 1) & 1, &gave_up));
+                        ok = __all_sync(~0u, ok);
+                        if (!ok) break;
+                        fence_after();
+                        if (issues) {
+                            const uint64_t k0 = kd + ks * (S::kTileBytes / 16);
+                            const uint32_t d = tmem + kTile * sb;
+#pragma unroll
+                            for (int q = 0; q < NT; ++q)
+#pragma unroll
+                                for (int k = 0; k < HD / 16; ++k)
+                                    mma_ss(d, q0 + q * (S::kQBytes / 16) + k * 16, k0 + k * 16, id, q + k > 0);
+                            mma_commit(&bars.s_ready[sb]);
+                            mma_commit(&bars.k_free[ks]);
+                            if (left == 1) mma_commit(&bars.q_free[pc % S::kQs]);
+                        }
+                        __syncwarp();
+                    }
+                    ++pc;
+                }
+                // what this warp has in flight, if a wait gave up
+                if (!ok)
+                    for (unsigned i = t > t0 + kScores ? t - kScores : t0; i < t; ++i)
+                        bar_wait(&bars.s_ready[i % kScores], (i / kScores) & 1, &gave_up, true);
+            } else {
+                constexpr uint32_t id = idesc_f16(kRows, HD, true);
+                const uint64_t vd = umma_desc(smem_addr(v_s), kGroupStride, 128);
+                for (int i = 0; ok && i < count; ++i) {
+                    const int nt = list.piece[i].tile1 - list.piece[i].tile0;
+                    if (nt <= 0) continue;
+                    if (pc) ok = __all_sync(~0u, bar_wait(&bars.o_free, (pc - 1) & 1, &gave_up));
+                    for (int j = 0; ok && j < nt; ++j, ++t) {
+                        const unsigned vs = t % kVs, sb = t % kScores;
+                        ok = bar_wait(&bars.p_ready[sb], (t / kScores) & 1, &gave_up) &&
+                             bar_wait(&bars.v_full[vs], (t / kVs) & 1, &gave_up);
+                        ok = __all_sync(~0u, ok);
+                        if (!ok) break;
+                        fence_after();
+                        if (issues) {
+                            const uint64_t v0 = vd + vs * (S::kTileBytes / 16);
+                            const uint32_t d = tmem + S::kO + HD * (t & 1), ap = tmem + kTile * sb, add = j >= 2;
+#pragma unroll
+                            for (int q = 0; q < NT; ++q)
+#pragma unroll
+                                for (int k = 0; k < kTile / 16; ++k)
+                                    mma_ts(d, ap + 32 * (k >> 1) + 16 * q + 8 * (k & 1), v0 + k * (2 * kGroupStride / 16), id,
+                                           q + k > 0 ? 1u : add);
+                            mma_commit(&bars.v_free[vs]);
+                            mma_commit(&bars.o_done[t & 1]);
+                        }
+                        __syncwarp();
+                    }
+                    ++pc;
+                }
+                if (!ok)
+                    for (unsigned i = t > t0 + 2 ? t - 2 : t0; i < t; ++i)
+                        bar_wait(&bars.o_done[i & 1], (i >> 1) & 1, &gave_up, true);
             }
         }
         __syncwarp();
