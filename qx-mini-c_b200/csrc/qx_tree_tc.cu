@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                 const Piece& p = list.piece[i];
                 const int nt = max(0, p.tile1 - p.tile0), j0 = (w ^ t) & 1;
                 const int node = row < p.have ? (p.row0 + row) / a.group : -1;
-                float m = -INFINITY, fac = 0.f;
+                float m = -INFINITY, top = -INFINITY, fac = 0.f;
                 float2 l2 = make_float2(0.f, 0.f);
                 for (int j = j0; j < nt; j += 2) {
                     const unsigned tt = t + j, st = tt % kVs;
@@ -385,11 +385,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
 #pragma unroll
                         for (int c = 0; c < 16; ++c) mx[c & 3] = fmaxf(mx[c & 3], fmaxf(x[c].x, x[c].y));
                         const float big = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        top = fmaxf(top, big);
                         const bool raise = big > m + kSlack || (m == -INFINITY && big > -INFINITY);
-                        if (__any_sync(~0u, raise)) {            // rare once a row has seen some of its scores
-                            // a whole number of powers of two, so that what is rescaled loses no bits
-                            const float m1 = raise ? (m == -INFINITY ? big : m + ceilf(big - m)) : m;
-                            const float f = raise ? exp2_fast(m - m1) : 1.f;
+                        if (__any_sync(~0u, raise)) {
+                            // Every row of the warp goes up to the largest score it has seen, so that this is rare from then on;
+                            // by a whole number of powers of two, so that what is rescaled loses no bits.
+                            const float m1 = m == -INFINITY ? top : m + fmaxf(ceilf(top - m), 0.f);
+                            const float f = m == -INFINITY ? 0.f : exp2_fast(m - m1);
                             m = m1;
                             l2 = mul2(l2, make_float2(f, f));
                             if (j != j0) {                       // the accumulator, once its last product is in
@@ -398,14 +400,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                                 if (!ok) break;
                                 fence_after();
 #pragma unroll 1
-                                for (int c = 0; c < HD; c += 16) {
-                                    float2 o[8];
+                                for (int c = 0; c < HD; c += 32) {
+                                    float2 o[8], u[8];
                                     tmem_ld16(to + c, reinterpret_cast<uint32_t*>(o));
+                                    tmem_ld16(to + c + 16, reinterpret_cast<uint32_t*>(u));
                                     wait_ld();
                                     loaded(o);
+                                    loaded(u);
 #pragma unroll
-                                    for (int e = 0; e < 8; ++e) o[e] = mul2(o[e], make_float2(f, f));
+                                    for (int e = 0; e < 8; ++e) o[e] = mul2(o[e], make_float2(f, f)), u[e] = mul2(u[e], make_float2(f, f));
                                     tmem_st16(to + c, reinterpret_cast<const uint32_t*>(o));
+                                    tmem_st16(to + c + 16, reinterpret_cast<const uint32_t*>(u));
                                 }
                             }
                             if (h) {                             // and the weights of the first half
