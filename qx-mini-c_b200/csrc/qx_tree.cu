@@ -24,47 +24,55 @@ __device__ __forceinline__ float load_q(const Tensor& q, size_t at) { return to_
 
 // ---- one warp's 16 cache rows --------------------------------------------------
 
-// Rows 4 j .. 4 j + 3 of the 16 belong to the lanes with lane % 4 = j, in both
+// A warp's steps of 16 cache rows come through a ring of its own in shared
+// memory, filled by asynchronous copies.  A step: the K codes [16][HD], the V
+// codes, then ks[16], vs[16] and log2(vs), 1 / vs, which the warp adds when the
+// step has arrived.  16-byte chunks are swizzled so that what eight lanes read at a time
+// lies in different banks: K by the row's lowest bit, V by row / 4.
+//
+// Rows 4 j .. 4 j + 3 of a step belong to the lanes with lane % 4 = j, in both
 // products: accumulator column 2 j + c of key tile h is row 4 j + 2 h + c.
 template <int HD>
-struct KvRegs {
-    uint4 k[2][HD / 64];       // key tile h, row lane / 4 of it: bytes 64 c + 16 j ..
-    uint32_t v[4][HD / 32];    // rows 4 j + i, dims (lane / 4) * HD / 8 ..
-    float ks[4], vs[4];
+struct Step {
+    static constexpr int kCodes = 16 * HD, kBytes = 2 * kCodes + 4 * 64, kChunks = HD / 16;
+    __device__ static __forceinline__ int k_chunk(int row, int c) { return HD == 128 ? c ^ ((row & 1) << 2) : c; }
+    __device__ static __forceinline__ int v_chunk(int row, int c) { return c ^ ((row >> 2) * 2 % kChunks); }
 };
-
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+// Rows row0 .. of KV head g (k, v, ks, vs: the sequence's row 0); rows past the last repeat it.
 template <int HD>
-__device__ __forceinline__ void load_kv(const TreeArgs& a, size_t base_row, int row0, int last, int g, KvRegs<HD>& r) {
-    const int lane = threadIdx.x & 31, j = lane & 3, n = lane >> 2;
-    const size_t KV = (size_t)a.c.kv_heads * HD;
+__device__ __forceinline__ void copy_step(const int8_t* k, const int8_t* v, const float* ks, const float* vs, int row_bytes,
+                                          int row0, int last, uint32_t to) {
+    constexpr int C = Step<HD>::kChunks;
+    const int lane = threadIdx.x & 31, c = lane % C;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int row = min(row0 + 4 * (n >> 1) + 2 * h + (n & 1), last);
-        const int8_t* p = a.c.k + (base_row + row) * KV + (size_t)g * HD + 16 * j;
-#pragma unroll
-        for (int c = 0; c < HD / 64; ++c) r.k[h][c] = __ldg(reinterpret_cast<const uint4*>(p + 64 * c));
+    for (int i = 0; i < 16 * C / 32; ++i) {
+        const int r = i * (32 / C) + lane / C;
+        const size_t at = (size_t)min(row0 + r, last) * row_bytes + 16 * c;
+        copy16(to + r * HD + 16 * Step<HD>::k_chunk(r, c), k + at);
+        copy16(to + Step<HD>::kCodes + r * HD + 16 * Step<HD>::v_chunk(r, c), v + at);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = min(row0 + 4 * j + i, last);
-        const int8_t* p = a.c.v + (base_row + row) * KV + (size_t)g * HD + (HD / 8) * n;
-        if (HD == 128) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-            r.v[i][0] = w.x, r.v[i][1] = w.y;
-            r.v[i][HD / 32 - 2] = w.z, r.v[i][HD / 32 - 1] = w.w;
-        } else {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
-            r.v[i][0] = w.x, r.v[i][1] = w.y;
-        }
-        r.ks[i] = __ldg(a.c.ks + base_row + row);
-        r.vs[i] = __ldg(a.c.vs + base_row + row);
-    }
+    copy4(to + 2 * Step<HD>::kCodes + 4 * lane, (lane < 16 ? ks : vs) + min(row0 + (lane & 15), last));
+}
+// log2(vs) and 1 / vs beside the step's scales; whole warp.
+template <int HD>
+__device__ __forceinline__ void finish_step(uint8_t* step) {
+    float* f = reinterpret_cast<float*>(step + 2 * Step<HD>::kCodes);
+    const int lane = threadIdx.x & 31;
+    const float v = f[16 + (lane & 15)];
+    f[32 + lane] = lane < 16 ? log_vs(v) : inv_vs(v);
+    __syncwarp();
 }
 
-// q . k for 16 query rows (staged at qs) and the 16 cache rows: acc[h] is the
+// q . k for 16 query rows (staged at qs) and a step's rows: acc[h] is the
 // accumulator of key tile h.
 template <int HD, int NT>
-__device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qterm, const KvRegs<HD>& r, float (&acc)[2][4]) {
+__device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qterm, const uint8_t* step, float (&acc)[2][4]) {
     const int lane = threadIdx.x & 31, j = lane & 3, n = lane >> 2;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -75,7 +83,9 @@ __device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qter
         uint32_t b[2][8];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t w[4] = {r.k[h][c].x, r.k[h][c].y, r.k[h][c].z, r.k[h][c].w};
+            const int row = 4 * (n >> 1) + 2 * h + (n & 1);
+            const uint4 k = *reinterpret_cast<const uint4*>(step + row * HD + 16 * Step<HD>::k_chunk(row, 4 * c + j));
+            const uint32_t w[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t u = w[i] ^ 0x80808080u;
@@ -138,26 +148,42 @@ __device__ __forceinline__ void stage_queries(const TreeArgs& a, int s, int g, i
 // ---- the kernel for small trees ------------------------------------------------
 
 // Blocks of 16 query rows; each of the 4 warps takes 16 of a tile's 64 cache
-// rows, straight from global memory into the registers of the products (the
-// next tile's while this one is computed), keeps its own m, sum and o, and the
-// four are joined when the unit's part ends.
+// rows, kRing - 1 tiles ahead, keeps its own m, sum and o, and the four are
+// joined when the unit's part ends.
+constexpr int kRing = 3;
+template <int HD, int NT>
+struct Small {
+    static constexpr int kQ = NT * 16 * (HD + 8) * 2, kRingBytes = kTreeWarps * kRing * Step<HD>::kBytes;
+    static constexpr int kO = kTreeWarps * 16 * (HD + 4) * 4;             // the warps' o, over the ring
+    static constexpr int kBytes = kQ + (kRingBytes > kO ? kRingBytes : kO);
+};
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(kTreeThreads) k_tree_small(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(kTreeThreads, 3) k_tree_small(const __grid_constant__ TreeArgs a) {
     constexpr int BM = 16, QS = HD + 8, NV = HD / 8;
-    __shared__ __align__(16) __half qs[NT * BM * QS];
+    extern __shared__ __align__(128) uint8_t dyn[];
+    __half* qs = reinterpret_cast<__half*>(dyn);
+    float (*wo)[BM][HD + 4] = reinterpret_cast<float (*)[BM][HD + 4]>(dyn + Small<HD, NT>::kQ);
     __shared__ float qfac[BM];
     __shared__ float wm[kTreeWarps][BM], wl[kTreeWarps][BM];
-    __shared__ __align__(16) float wo[kTreeWarps][BM][HD + 4];
     __shared__ PieceList list;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
+    uint8_t* ring = dyn + Small<HD, NT>::kQ + warp * kRing * Step<HD>::kBytes;
+    const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(ring);
+    const int row_bytes = a.c.kv_heads * HD;
     int batch = 0, at = 0;
     list_pieces(a, list, 0);
     while (at < list.count) {
         const Piece p = list.piece[at];
         const int last = p.len + p.n - 1, stop = p.tile1 * kTile;
-        KvRegs<HD> kv;
-        int r0 = p.tile0 * kTile + 16 * warp;
-        if (r0 < stop) load_kv<HD>(a, p.base_row, r0, last, p.g, kv);
+        const int8_t *k0 = a.c.k + p.base_row * row_bytes + p.g * HD, *v0 = a.c.v + p.base_row * row_bytes + p.g * HD;
+        const float *ks0 = a.c.ks + p.base_row, *vs0 = a.c.vs + p.base_row;
+        int r0 = p.tile0 * kTile + 16 * warp, slot = 0;
+        auto copy = [&](int row, int s) {
+            if (row < stop) copy_step<HD>(k0, v0, ks0, vs0, row_bytes, row, last, ring_a + s * Step<HD>::kBytes);
+            asm volatile("cp.async.commit_group;" ::: "memory");      // empty past the end: the groups stay countable
+        };
+#pragma unroll
+        for (int i = 0; i < kRing - 1; ++i) copy(r0 + i * kTile, i);
         stage_queries<T, HD, NT>(a, p.s, p.g, p.row0, BM, p.have, qs, QS, BM * QS, qfac);
         __syncthreads();
         float m[2], l[2], o[NV][4], fac[2];
@@ -174,12 +200,21 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_small(const __grid_consta
 #pragma unroll
         for (int d = 0; d < NV; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
         for (; r0 < stop; r0 += kTile) {
+            __syncwarp();                                              // the slot to fill has been read
+            copy(r0 + (kRing - 1) * kTile, slot == 0 ? kRing - 1 : slot - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+            __syncwarp();
+            uint8_t* step = ring + slot * Step<HD>::kBytes;
+            slot = slot == kRing - 1 ? 0 : slot + 1;
+            finish_step<HD>(step);
+            const float* f = reinterpret_cast<const float*>(step + 2 * Step<HD>::kCodes);
             float ks[4], lv[4], iv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ks[i] = kv.ks[i], lv[i] = log_vs(kv.vs[i]), iv[i] = inv_vs(kv.vs[i]);
+            *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(f + 4 * j);
+            *reinterpret_cast<float4*>(lv) = *reinterpret_cast<const float4*>(f + 32 + 4 * j);
+            *reinterpret_cast<float4*>(iv) = *reinterpret_cast<const float4*>(f + 48 + 4 * j);
             const bool edge = r0 + 16 > p.len;
             float acc[2][4];
-            dot_keys<HD, NT>(qs, QS, BM * QS, kv, acc);
+            dot_keys<HD, NT>(qs, QS, BM * QS, step, acc);
             // acc[h][2 u + c]: query row n8 + 8 u, cache row r0 + 4 j + 2 h + c
             float x[2][4], up[2];
             bool grew = false;
@@ -224,21 +259,34 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_small(const __grid_consta
                 }
             }
             // values: dims (lane / 4) * NV + d of rows 4 j .. 4 j + 3 are column lane / 4 of value tile d
+            uint32_t v[4][HD / 32];
 #pragma unroll
-            for (int v = 0; v < HD / 32; ++v) {
-                const uint32_t v0 = kv.v[0][v] ^ 0x80808080u, v1 = kv.v[1][v] ^ 0x80808080u,
-                               v2 = kv.v[2][v] ^ 0x80808080u, v3 = kv.v[3][v] ^ 0x80808080u;
-                const uint32_t a0 = __byte_perm(v0, v1, 0x5140), a1 = __byte_perm(v0, v1, 0x7362);
-                const uint32_t c0 = __byte_perm(v2, v3, 0x5140), c1 = __byte_perm(v2, v3, 0x7362);
+            for (int i = 0; i < 4; ++i) {
+                const int row = 4 * j + i;
+                const uint8_t* at_v = step + Step<HD>::kCodes + row * HD;
+                if (HD == 128) {
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(at_v + 16 * Step<HD>::v_chunk(row, n8));
+                    v[i][0] = w4.x ^ 0x80808080u, v[i][1] = w4.y ^ 0x80808080u;
+                    v[i][HD / 32 - 2] = w4.z ^ 0x80808080u, v[i][HD / 32 - 1] = w4.w ^ 0x80808080u;
+                } else {
+                    const uint2 w2 = *reinterpret_cast<const uint2*>(at_v + 16 * Step<HD>::v_chunk(row, n8 >> 1) + 8 * (n8 & 1));
+                    v[i][0] = w2.x ^ 0x80808080u, v[i][1] = w2.y ^ 0x80808080u;
+                }
+            }
+#pragma unroll
+            for (int d4 = 0; d4 < HD / 32; ++d4) {
+                const uint32_t a0 = __byte_perm(v[0][d4], v[1][d4], 0x5140), a1 = __byte_perm(v[0][d4], v[1][d4], 0x7362);
+                const uint32_t c0 = __byte_perm(v[2][d4], v[3][d4], 0x5140), c1 = __byte_perm(v[2][d4], v[3][d4], 0x7362);
                 const uint32_t b0[4] = {low_pair(a0), high_pair(a0), low_pair(a1), high_pair(a1)};
                 const uint32_t b1[4] = {low_pair(c0), high_pair(c0), low_pair(c1), high_pair(c1)};
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
-                    for (int q = 0; q < NT; ++q) mma16816(o[4 * v + d], w[q], b0[d], b1[d]);
+                    for (int q = 0; q < NT; ++q) mma16816(o[4 * d4 + d], w[q], b0[d], b1[d]);
             }
-            if (r0 + kTile < stop) load_kv<HD>(a, p.base_row, r0 + kTile, last, p.g, kv);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();                                               // every warp's steps are read: its o may go over them
         // join the four warps
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -289,36 +337,60 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_small(const __grid_consta
 }
 
 // Adds the parts of the units that several CTAs worked on, by the records
-// they left.  grid: (CTA of the kernel before, group of rows).
-constexpr int kJoinThreads = 128;
+// they left, in two halves of their order.  grid: (CTA of the kernel before,
+// two of the unit's rows).
+constexpr int kJoinRows = 2, kJoinHalves = 2;
 template <class T, int HD>
-__global__ void __launch_bounds__(kJoinThreads) k_tree_join(const __grid_constant__ TreeArgs a) {
-    constexpr int kRows = kJoinThreads / (HD / 4);
+__global__ void __launch_bounds__(kJoinRows * kJoinHalves * HD / 4) k_tree_join(const __grid_constant__ TreeArgs a) {
+    constexpr int kLanes = HD / 4, kThreads = kJoinRows * kJoinHalves * kLanes;
+    __shared__ float weight[kJoinRows][kMaxCtas], sums[kJoinRows], tops[kJoinRows];
+    __shared__ float4 halves[kJoinRows][kLanes];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before still runs
     const Join j = a.joins[blockIdx.x];
-    const int row = blockIdx.y * kRows + threadIdx.x / (HD / 4), d0 = threadIdx.x % (HD / 4) * 4;
-    if (row >= (j.parts ? j.have : 0)) return;
+    const int row0 = blockIdx.y * kJoinRows, tid = threadIdx.x;
+    if (row0 >= (j.parts ? j.have : 0)) return;
     // the first part begins the unit, the others are what their CTAs began with
-    auto part = [&](int i) { return part_of(a, blockIdx.x - 1 + i, i == 0) + (size_t)row * (kPartHead + HD); };
-    float mx = -INFINITY, sum = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < j.parts; ++i) mx = fmaxf(mx, part(i)[0]);
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < j.parts; ++i) {
-        const float* p = part(i);
-        const float2 ml = *reinterpret_cast<const float2*>(p);
-        const float4 v = *reinterpret_cast<const float4*>(p + kPartHead + d0);
-        const float f = part_weight(ml.x, ml.y, mx);
-        sum = fmaf(f, ml.y, sum);
-        y = make_float4(fmaf(f, v.x, y.x), fmaf(f, v.y, y.y), fmaf(f, v.z, y.z), fmaf(f, v.w, y.w));
+    auto part = [&](int i, int row) {
+        return part_of(a, blockIdx.x - 1 + i, i == 0) + (size_t)row * (kPartHead + HD);
+    };
+    // the parts' factors: a warp to a row
+    for (int r = tid >> 5; r < kJoinRows; r += kThreads / 32) {
+        const int lane = tid & 31, row = min(row0 + r, j.have - 1);
+        float mx = -INFINITY, sum = 0.f;
+        for (int i = lane; i < j.parts; i += 32) mx = fmaxf(mx, part(i, row)[0]);
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+        for (int i = lane; i < j.parts; i += 32) {
+            const float2 ml = *reinterpret_cast<const float2*>(part(i, row));
+            const float f = part_weight(ml.x, ml.y, mx);
+            weight[r][i] = f;
+            sum = fmaf(f, ml.y, sum);
+        }
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (lane == 0) sums[r] = sum, tops[r] = mx;
     }
+    __syncthreads();
+    const int d = tid % kLanes, r = tid / kLanes % kJoinRows, half = tid / (kLanes * kJoinRows), row = row0 + r;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < j.have) {
+        const int first = half * ((j.parts + 1) / 2), end = half ? j.parts : (j.parts + 1) / 2;
+#pragma unroll 8
+        for (int i = first; i < end; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(part(i, row) + kPartHead + 4 * d);
+            const float f = weight[r][i];
+            y = make_float4(fmaf(f, v.x, y.x), fmaf(f, v.y, y.y), fmaf(f, v.z, y.z), fmaf(f, v.w, y.w));
+        }
+    }
+    if (half) halves[r][d] = y;
+    __syncthreads();
+    if (half || row >= j.have) return;
+    const float4 z = halves[r][d];
+    const float sum = sums[r], by = sum == 0.f ? 0.f : 1.f / sum;
     const int nd = (j.row0 + row) / a.group, h = j.g * a.group + (j.row0 + row) % a.group;
-    T* dst = (T*)a.out.p + j.s * a.out.seq + nd * a.out.node + h * a.out.head + d0;
-    const float z[4] = {y.x, y.y, y.z, y.w};
+    T* dst = (T*)a.out.p + j.s * a.out.seq + nd * a.out.node + h * a.out.head + 4 * d;
+    const float out[4] = {(y.x + z.x) * by, (y.y + z.y) * by, (y.z + z.z) * by, (y.w + z.w) * by};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : z[e] / sum);
-    if (d0 == 0) write_lse(a, j.s, nd, h, mx, sum);
+    for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : out[e]);
+    if (d == 0) write_lse(a, j.s, nd, h, tops[r], sum);
 }
 
 // ---- what each cache row got ---------------------------------------------------
@@ -331,6 +403,7 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
     constexpr int QS = HD + 8;
     __shared__ __align__(16) __half qs[NT * 16 * QS];
     __shared__ float qfac[16];
+    __shared__ __align__(16) uint8_t steps[kTreeWarps][Step<HD>::kBytes];
     __shared__ int warp_sum[kScanThreads / 32], at_seq, at_first, clash;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
     // shares here are of tiles alone, one "unit" a sequence
@@ -368,15 +441,21 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
         const size_t base_row = (size_t)slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
         float got[4] = {};
         for (int g = 0; g < a.c.kv_heads; ++g) {
-            KvRegs<HD> kv;
-            load_kv<HD>(a, base_row, min(r0, last), last, g, kv);
+            uint8_t* step = steps[warp];
+            __syncwarp();
+            copy_step<HD>(a.c.k + base_row * a.c.kv_heads * HD + g * HD, a.c.v + base_row * a.c.kv_heads * HD + g * HD, a.c.ks + base_row,
+                          a.c.vs + base_row, a.c.kv_heads * HD, min(r0, last), last, (uint32_t)__cvta_generic_to_shared(step));
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+            const float4 ks4 = *reinterpret_cast<const float4*>(step + 2 * Step<HD>::kCodes + 16 * j);
+            const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
             for (int row0 = 0; row0 < n * a.group; row0 += 16) {
                 const int have = min(16, n * a.group - row0);
                 __syncthreads();
                 stage_queries<T, HD, NT>(a, s, g, row0, 16, have, qs, QS, 16 * QS, qfac);
                 __syncthreads();
                 float acc[2][4];
-                dot_keys<HD, NT>(qs, QS, 16 * QS, kv, acc);
+                dot_keys<HD, NT>(qs, QS, 16 * QS, step, acc);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int r = n8 + 8 * u;
@@ -389,7 +468,7 @@ __global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
                     for (int i = 0; i < 4; ++i) {
                         const int t = r0 + 4 * j + i;
                         if (t <= last && sees(mrow, node, t, len, n))
-                            got[i] += exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * qfac[r], kv.ks[i], -lg));
+                            got[i] += exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * qfac[r], ks[i], -lg));
                     }
                 }
             }
@@ -445,18 +524,19 @@ cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t
         e = launch_tree_tc(a, type, sms, st);
     } else {
         int per = 0;
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_tree_small<T, HD, NT>, kTreeThreads, 0);
+        constexpr int kBytes = Small<HD, NT>::kBytes;
+        e = cudaFuncSetAttribute((const void*)k_tree_small<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_tree_small<T, HD, NT>, kTreeThreads, kBytes);
         if (e != cudaSuccess) return e;
         a.ctas = sms * (per < 1 ? 1 : per);
         if (a.ctas > kMaxCtas) a.ctas = kMaxCtas;
-        k_tree_small<T, HD, NT><<<a.ctas, kTreeThreads, 0, st>>>(a);
+        k_tree_small<T, HD, NT><<<a.ctas, kTreeThreads, kBytes, st>>>(a);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    constexpr int kRows = kJoinThreads / (HD / 4);
-    cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)(a.block_rows / kRows));
-    cfg.blockDim = dim3(kJoinThreads);
+    cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)(a.block_rows / kJoinRows));
+    cfg.blockDim = dim3(kJoinRows * kJoinHalves * HD / 4);
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
