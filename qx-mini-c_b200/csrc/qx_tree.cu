@@ -337,42 +337,47 @@ __global__ void __launch_bounds__(kTreeThreads, 3) k_tree_small(const __grid_con
 }
 
 // Adds the parts of the units that several CTAs worked on, by the records
-// they left, in two halves of their order.  grid: (CTA of the kernel before,
-// two of the unit's rows).
-constexpr int kJoinRows = 2, kJoinHalves = 2;
-template <class T, int HD>
-__global__ void __launch_bounds__(kJoinRows * kJoinHalves * HD / 4) k_tree_join(const __grid_constant__ TreeArgs a) {
-    constexpr int kLanes = HD / 4, kThreads = kJoinRows * kJoinHalves * kLanes;
-    __shared__ float weight[kJoinRows][kMaxCtas], sums[kJoinRows], tops[kJoinRows];
-    __shared__ float4 halves[kJoinRows][kLanes];
+// they left.  grid: (CTA of the kernel before, R of the unit's rows); G groups
+// of threads take a share of the parts each (many for the small kernel's units,
+// which can be spread over hundreds of CTAs; one for those of 128 rows), and are added in order.
+constexpr int kJoinThreads = 256;
+template <class T, int HD, int R>
+__global__ void __launch_bounds__(kJoinThreads) k_tree_join(const __grid_constant__ TreeArgs a) {
+    constexpr int kLanes = HD / 4, G = kJoinThreads / (R * kLanes), kPer = kJoinThreads / R, kMost = R == 8 ? kMaxCtas / 8 : kMaxCtas;
+    __shared__ float weight[R][kMost], red[2][kJoinThreads / 32], tops[R];
+    __shared__ float4 shares[G][R][kLanes];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before still runs
     const Join j = a.joins[blockIdx.x];
-    const int row0 = blockIdx.y * kJoinRows, tid = threadIdx.x;
+    const int row0 = blockIdx.y * R, tid = threadIdx.x;
     if (row0 >= (j.parts ? j.have : 0)) return;
     // the first part begins the unit, the others are what their CTAs began with
-    auto part = [&](int i, int row) {
-        return part_of(a, blockIdx.x - 1 + i, i == 0) + (size_t)row * (kPartHead + HD);
-    };
-    // the parts' factors: a warp to a row
-    for (int r = tid >> 5; r < kJoinRows; r += kThreads / 32) {
-        const int lane = tid & 31, row = min(row0 + r, j.have - 1);
-        float mx = -INFINITY, sum = 0.f;
-        for (int i = lane; i < j.parts; i += 32) mx = fmaxf(mx, part(i, row)[0]);
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
-        for (int i = lane; i < j.parts; i += 32) {
-            const float2 ml = *reinterpret_cast<const float2*>(part(i, row));
-            const float f = part_weight(ml.x, ml.y, mx);
-            weight[r][i] = f;
-            sum = fmaf(f, ml.y, sum);
-        }
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (lane == 0) sums[r] = sum, tops[r] = mx;
+    const size_t row_floats = kPartHead + HD, step = 2 * (size_t)a.block_rows * row_floats;
+    const float* parts = part_of(a, blockIdx.x - 1, false);
+    auto part = [&](int i, int row) { return parts + i * step + (i == 0 ? step / 2 : 0) + row * row_floats; };
+    // the parts' factors: kPer threads (whole warps) to a row
+    const int wr = tid / kPer, wi = tid % kPer, wrow = min(row0 + wr, j.have - 1);
+    float mx = -INFINITY, sum = 0.f;
+    for (int i = wi; i < j.parts; i += kPer) mx = fmaxf(mx, part(i, wrow)[0]);
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+    if (kPer > 32) {
+        if ((tid & 31) == 0) red[0][tid >> 5] = mx;
+        __syncthreads();
+        for (int i = 0; i < kPer / 32; ++i) mx = fmaxf(mx, red[0][wr * (kPer / 32) + i]);
     }
+    for (int i = wi; i < j.parts; i += kPer) {
+        const float2 ml = *reinterpret_cast<const float2*>(part(i, wrow));
+        const float f = part_weight(ml.x, ml.y, mx);
+        weight[wr][i] = f;
+        sum = fmaf(f, ml.y, sum);
+    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if ((tid & 31) == 0) red[1][tid >> 5] = sum;
+    if (wi == 0) tops[wr] = mx;
     __syncthreads();
-    const int d = tid % kLanes, r = tid / kLanes % kJoinRows, half = tid / (kLanes * kJoinRows), row = row0 + r;
+    const int d = tid % kLanes, r = tid / kLanes % R, g = tid / (kLanes * R), row = row0 + r;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row < j.have) {
-        const int first = half * ((j.parts + 1) / 2), end = half ? j.parts : (j.parts + 1) / 2;
+        const int each = (j.parts + G - 1) / G, first = g * each, end = min(j.parts, first + each);
 #pragma unroll 8
         for (int i = first; i < end; ++i) {
             const float4 v = *reinterpret_cast<const float4*>(part(i, row) + kPartHead + 4 * d);
@@ -380,14 +385,21 @@ __global__ void __launch_bounds__(kJoinRows * kJoinHalves * HD / 4) k_tree_join(
             y = make_float4(fmaf(f, v.x, y.x), fmaf(f, v.y, y.y), fmaf(f, v.z, y.z), fmaf(f, v.w, y.w));
         }
     }
-    if (half) halves[r][d] = y;
-    __syncthreads();
-    if (half || row >= j.have) return;
-    const float4 z = halves[r][d];
-    const float sum = sums[r], by = sum == 0.f ? 0.f : 1.f / sum;
+    if (G > 1) {
+        shares[g][r][d] = y;
+        __syncthreads();
+    }
+    if (g || row >= j.have) return;
+    for (int i = 1; i < G; ++i) {
+        const float4 z = shares[i][r][d];
+        y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+    }
+    sum = 0.f;
+    for (int i = 0; i < kPer / 32; ++i) sum += red[1][r * (kPer / 32) + i];
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
     const int nd = (j.row0 + row) / a.group, h = j.g * a.group + (j.row0 + row) % a.group;
     T* dst = (T*)a.out.p + j.s * a.out.seq + nd * a.out.node + h * a.out.head + 4 * d;
-    const float out[4] = {(y.x + z.x) * by, (y.y + z.y) * by, (y.z + z.z) * by, (y.w + z.w) * by};
+    const float out[4] = {y.x * by, y.y * by, y.z * by, y.w * by};
 #pragma unroll
     for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : out[e]);
     if (d == 0) write_lse(a, j.s, nd, h, tops[r], sum);
@@ -535,15 +547,15 @@ cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t
     }
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)(a.block_rows / kJoinRows));
-    cfg.blockDim = dim3(kJoinRows * kJoinHalves * HD / 4);
+    cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)(a.block_rows / (tc ? 8 : 2)));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, k_tree_join<T, HD>, a);
+    e = tc ? cudaLaunchKernelEx(&cfg, k_tree_join<T, HD, 8>, a) : cudaLaunchKernelEx(&cfg, k_tree_join<T, HD, 2>, a);
     if (e != cudaSuccess || !a.mass) return e;
     k_tree_mass<T, HD, NT><<<sms * 4, kTreeThreads, 0, st>>>(a);
     return cudaGetLastError();
