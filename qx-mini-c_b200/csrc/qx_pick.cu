@@ -1,18 +1,21 @@
 // Penalties, biases and a grammar mask on logits, and the greedy token of each
 // row (qx_cuda_pick_tokens).
 //
-// A cluster of CTAs takes one row; each CTA owns a slice of the vocabulary and
-// keeps one 32-bit word per token of it in shared memory: the token's count in
-// the history (low 20 bits) and the last bias entry that names it, plus one
-// (high 12 bits).  Every CTA reads the whole history and counts what falls in
-// its slice, in its own shared memory: counting each part of the history once
-// and into other CTAs' memory instead reads an eighth, but histories repeat
-// few tokens, whose CTA then takes thousands of single remote additions (256
-// rows of 151936, histories of 4096: 155 us against XX).  Integer atomics, so
-// the order they land in changes nothing.  Then each CTA streams its slice of
-// the logits once, the first of it in registers since before the counting
-// began, and the row's best is joined through the cluster, with no workspace
-// and one launch.
+// A cluster of CTAs takes row after row; each CTA owns a slice of the
+// vocabulary (every eighth 64 tokens: frequent tokens lie together, and one CTA
+// with all of them held the others up, 131 us against XX for 256 rows of
+// 151936) and keeps one 32-bit word per token of it in shared memory: the
+// token's count in the history (low 20 bits) and the last bias entry that names
+// it, plus one (high 12 bits).  Every CTA reads the whole history and counts
+// what falls in its slice: counting an eighth each into the others' memory reads
+// less, but histories repeat few tokens, whose CTA then takes thousands of
+// single remote additions (256 rows of 151936 with histories of 4096: 155 us,
+// where this way took 135).  Integer atomics, so the order they land in changes
+// nothing.  Then each CTA streams its slice of the logits once, putting the
+// words it finds back to 0 for the next row, and leaves its best with the
+// cluster's first CTA, which joins a row's eight while the next is counted: no
+// workspace, one launch, and no wait between rows that the next row's first
+// loads do not overlap.
 //
 // Rows need not start on 16-byte boundaries: a row's tokens are numbered from
 // the boundary before it ("places"), and slices and packs are of places.
@@ -34,7 +37,7 @@ struct PickArgs {
     const void* logits;
     void* out;
     size_t logits_stride, out_stride;
-    int vocab, slice, max_history, max_bias;
+    int rows, vocab, slice, max_history, max_bias;
     const int *history, *history_lens;
     const float *repetition, *frequency, *presence;
     const int *bias_ids, *bias_lens;
@@ -54,182 +57,231 @@ __device__ __forceinline__ void better(Best& a, float v, int i) {
     if (v > a.v || (v == a.v && i < a.i)) a.v = v, a.i = i;
 }
 
+// The cluster's barrier, its two halves apart.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 __device__ __forceinline__ int clamped(const int* lens, int r, int most) {
     return lens ? max(0, min(lens[r], most)) : most;
 }
 
+// Place p is word p / 512 * 64 + p % 64 of the CTA p / 64 % 8 of the cluster.
+constexpr int kChunk = 64, kRound = kChunk * kPickCluster;
+__device__ __forceinline__ int place_of(int word, int rank) {
+    return word / kChunk * kRound + rank * kChunk + word % kChunk;
+}
+
+// A row's addresses, and where its tokens are.
+template <class T>
+struct Row {
+    static constexpr int V = 16 / sizeof(T);
+    const T* x;
+    T* o;
+    const uint32_t* allowed;
+    int shift, end;                  // token t is at place t + shift; the row ends before place `end`
+    bool wide_out;
+    __device__ __forceinline__ Row(const PickArgs& a, int row) {
+        x = (const T*)a.logits + row * a.logits_stride;
+        o = a.out ? (T*)a.out + row * a.out_stride : nullptr;
+        allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+        shift = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % V);
+        wide_out = o && (int)(reinterpret_cast<uintptr_t>(o) / sizeof(T) % V) == shift;
+        end = a.vocab + shift;
+    }
+    __device__ __forceinline__ bool whole(int p) const { return p >= shift && p + V <= end; }
+    // a pack's logits, and the mask word of its first token
+    __device__ __forceinline__ void load(int p, Pack<T, V>& v, uint32_t& bits) const {
+        if (whole(p)) {
+            v = *reinterpret_cast<const Pack<T, V>*>(x + (p - shift));
+            bits = allowed ? allowed[(p - shift) >> 5] : ~0u;
+        }
+    }
+};
+
 template <class T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_constant__ PickArgs a) {
     constexpr int V = 16 / sizeof(T), kAhead = V == 4 ? 4 : 2;         // packs a thread has in flight
     extern __shared__ __align__(16) uint32_t words[];
-    __shared__ Best wbest[THREADS / 32], cbest;
+    __shared__ Best wbest[THREADS / 32], row_best[2][kPickCluster];     // row_best: in the cluster's first CTA
     cg::cluster_group cl = cg::this_cluster();
-    const int rank = (int)cl.block_rank(), r = blockIdx.x / kPickCluster, tid = threadIdx.x;
+    const int rank = (int)cl.block_rank(), step = gridDim.x / kPickCluster, tid = threadIdx.x;
     const bool touched = a.history || a.bias_ids;
-    // token t is at place t + shift
-    const T* x = (const T*)a.logits + r * a.logits_stride;
-    T* o = a.out ? (T*)a.out + r * a.out_stride : nullptr;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % V);
-    const bool wide_out = o && (int)(reinterpret_cast<uintptr_t>(o) / sizeof(T) % V) == shift;
-    const int lo = rank * a.slice, hi = min(lo + a.slice, a.vocab + shift);      // places of this CTA, from shift on in the first
-    const uint32_t* allowed = a.allowed ? a.allowed + r * a.allowed_stride : nullptr;
-    auto whole = [&](int p) { return p >= shift && p + V <= min(hi, a.vocab + shift); };
-    // a pack's logits, and its tokens' bits of the mask
-    auto load = [&](int p, Pack<T, V>& v, uint32_t& bits) {
-        bits = ~0u;
-        if (whole(p)) {
-            const int t = p - shift;
-            v = *reinterpret_cast<const Pack<T, V>*>(x + t);
-            if (allowed) bits = __funnelshift_r(allowed[t >> 5], allowed[(t + V - 1) >> 5], t & 31);
-        }
-    };
-    Pack<T, V> pack[kAhead];
-    uint32_t bits[kAhead];
-    int p0 = lo + tid * V;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(p0 + i * THREADS * V, pack[i], bits[i]);
-    const float rep = a.repetition ? a.repetition[r] : 1.f, freq = a.frequency ? a.frequency[r] : 0.f,
-                pres = a.presence ? a.presence[r] : 0.f;
     if (touched) {
         for (int i = tid * 4; i < a.slice; i += THREADS * 4) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        const int l0 = max(lo - shift, 0), n = hi - shift - l0;          // the slice's tokens l0 .. l0 + n
-        uint32_t* word = words + (l0 + shift - lo);
-        if (a.bias_ids) {
-            const int nb = clamped(a.bias_lens, r, a.max_bias);
-            for (int j = tid; j < nb; j += THREADS) {
-                const int k = a.bias_ids[r * a.bias_stride + j] - l0;
-                if ((unsigned)k < (unsigned)max(n, 0) && k + l0 >= 0) atomicMax(&word[k], (uint32_t)(j + 1) << kCountBits);
-            }
-            __syncthreads();
-        }
-        if (a.history) {
-            const int nh = clamped(a.history_lens, r, a.max_history);
-            const int* h = a.history + r * a.history_stride;
-            auto count = [&](int id) {
-                const unsigned k = (unsigned)id - (unsigned)l0;
-                if (k < (unsigned)max(n, 0)) atomicAdd(&word[k], 1u);
-            };
-            int j = tid * 4;
-            if (aligned16(h))
-                for (; j + 4 <= nh; j += THREADS * 4) {
-                    const int4 q = *reinterpret_cast<const int4*>(h + j);
-                    count(q.x), count(q.y), count(q.z), count(q.w);
-                }
-            else
-                for (; j + 4 <= nh; j += THREADS * 4) {
-                    const int q0 = h[j], q1 = h[j + 1], q2 = h[j + 2], q3 = h[j + 3];
-                    count(q0), count(q1), count(q2), count(q3);
-                }
-            for (int e = j; e < min(j + 4, nh); ++e) count(h[e]);
-        }
-        __syncthreads();
     }
-    Best best{-INFINITY, 0x7fffffff, 0};
-    auto touch = [&](float v, uint32_t w) {
-        const uint32_t c = w & kCountMask, b = w >> kCountBits;
-        if (c) {
-            v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-            v = __fsub_rn(v, __fmul_rn(freq, (float)c));
-            v = __fsub_rn(v, pres);
-        }
-        if (b) v = __fadd_rn(v, a.bias_values[r * a.bias_stride + b - 1]);
-        return v;
-    };
-    for (; p0 < hi; p0 += kAhead * THREADS * V) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int p = p0 + i * THREADS * V, t = p - shift;
-            if (whole(p)) {
-                float v[V];
-#pragma unroll
-                for (int u = 0; u < V; ++u) v[u] = to_f32(pack[i].v[u]);
-                const uint32_t ok = bits[i];
-                load(p + kAhead * THREADS * V, pack[i], bits[i]);        // on its way while this one is worked on
-                if (touched)
-#pragma unroll
-                    for (int u = 0; u < V; u += 4) {
-                        const uint4 q = *reinterpret_cast<const uint4*>(words + (p - lo) + u);
-                        if (q.x | q.y | q.z | q.w) {
-                            if (q.x) v[u] = touch(v[u], q.x);
-                            if (q.y) v[u + 1] = touch(v[u + 1], q.y);
-                            if (q.z) v[u + 2] = touch(v[u + 2], q.z);
-                            if (q.w) v[u + 3] = touch(v[u + 3], q.w);
-                        }
-                    }
-                float big = -INFINITY;
-                Pack<T, V> y;
-#pragma unroll
-                for (int u = 0; u < V; ++u) {
-                    if (!(ok >> u & 1u)) v[u] = -INFINITY;
-                    best.bad |= !(v[u] < INFINITY);
-                    big = fmaxf(big, v[u]);
-                    y.v[u] = from_f32<T>(v[u]);
-                }
-                if (big > best.v) {
-                    best.v = big;
-#pragma unroll
-                    for (int u = V - 1; u >= 0; --u)
-                        if (v[u] == big) best.i = t + u;
-                }
-                if (wide_out) {
-                    *reinterpret_cast<Pack<T, V>*>(o + t) = y;
-                } else if (o) {
-#pragma unroll
-                    for (int u = 0; u < V; ++u) o[t + u] = y.v[u];
-                }
-            } else {
-                if (p < hi)
-#pragma unroll 1
-                    for (int u = 0; u < V; ++u) {                        // the row's ends
-                        const int e = t + u;
-                        if (e < 0 || p + u >= hi || e >= a.vocab) continue;
-                        float v = to_f32(x[e]);
-                        if (touched && words[p + u - lo]) v = touch(v, words[p + u - lo]);
-                        if (allowed && !(allowed[e >> 5] >> (e & 31) & 1u)) v = -INFINITY;
-                        best.bad |= !(v < INFINITY);
-                        if (v > best.v) best.v = v, best.i = e;
-                        if (o) o[e] = from_f32<T>(v);
-                    }
-                load(p + kAhead * THREADS * V, pack[i], bits[i]);
-            }
-        }
-    }
-    for (int s = 16; s; s >>= 1) {
-        const float v = __shfl_xor_sync(~0u, best.v, s);
-        const int i = __shfl_xor_sync(~0u, best.i, s);
-        better(best, v, i);
-    }
-    best.bad = __any_sync(~0u, best.bad);
-    if ((tid & 31) == 0) wbest[tid >> 5] = best;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < THREADS / 32; ++w) {
-            better(best, wbest[w].v, wbest[w].i);
-            best.bad |= wbest[w].bad;
-        }
-        cbest = best;
-    }
-    cl.sync();
-    if (rank == 0 && tid == 0) {
+    // the best of the row before, whose eight parts are in once its barrier is passed
+    auto join = [&](int r, int slot) {
+        if (rank || tid) return;
+        Best best = row_best[slot][0];
         for (int c = 1; c < kPickCluster; ++c) {
-            const Best* p = cl.map_shared_rank(&cbest, c);
-            better(best, p->v, p->i);
-            best.bad |= p->bad;
+            better(best, row_best[slot][c].v, row_best[slot][c].i);
+            best.bad |= row_best[slot][c].bad;
         }
         a.picked[r] = best.bad || !(best.v > -INFINITY) ? 0xffffffffu : (uint32_t)best.i;
+    };
+    Pack<T, V> pack[kAhead];
+    uint32_t bits[kAhead];
+    const int first = blockIdx.x / kPickCluster;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) Row<T>(a, first).load(place_of((i * THREADS + tid) * V, rank), pack[i], bits[i]);
+    int slot = 0;
+    for (int r = first; r < a.rows; r += step, slot ^= 1) {
+        const Row<T> row(a, r);
+        const int shift = row.shift;
+        const float rep = a.repetition ? a.repetition[r] : 1.f, freq = a.frequency ? a.frequency[r] : 0.f,
+                    pres = a.presence ? a.presence[r] : 0.f;
+        if (touched) {
+            // the word of a token, if it is this CTA's
+            auto word = [&](int id) -> uint32_t* {
+                const int p = id + shift;
+                return (unsigned)id < (unsigned)a.vocab && (p / kChunk) % kPickCluster == rank ? words + p / kRound * kChunk + p % kChunk
+                                                                                             : nullptr;
+            };
+            if (a.bias_ids) {
+                const int nb = clamped(a.bias_lens, r, a.max_bias);
+                for (int j = tid; j < nb; j += THREADS)
+                    if (uint32_t* w = word(a.bias_ids[r * a.bias_stride + j])) atomicMax(w, (uint32_t)(j + 1) << kCountBits);
+                __syncthreads();
+            }
+            if (a.history) {
+                const int nh = clamped(a.history_lens, r, a.max_history);
+                const int* h = a.history + r * a.history_stride;
+                auto count = [&](int id) {
+                    if (uint32_t* w = word(id)) atomicAdd(w, 1u);
+                };
+                int j = tid * 4;
+                if (aligned16(h))
+                    for (; j + 4 <= nh; j += THREADS * 4) {
+                        const int4 q = *reinterpret_cast<const int4*>(h + j);
+                        count(q.x), count(q.y), count(q.z), count(q.w);
+                    }
+                else
+                    for (; j + 4 <= nh; j += THREADS * 4) {
+                        const int q0 = h[j], q1 = h[j + 1], q2 = h[j + 2], q3 = h[j + 3];
+                        count(q0), count(q1), count(q2), count(q3);
+                    }
+                for (int e = j; e < min(j + 4, nh); ++e) count(h[e]);
+            }
+        }
+        if (r != first) {
+            cluster_wait();
+            join(r - step, slot ^ 1);
+        }
+        __syncthreads();
+        Best best{-INFINITY, 0x7fffffff, 0};
+        auto touch = [&](float v, uint32_t w) {
+            const uint32_t c = w & kCountMask, b = w >> kCountBits;
+            if (c) {
+                v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+                v = __fsub_rn(v, __fmul_rn(freq, (float)c));
+                v = __fsub_rn(v, pres);
+            }
+            if (b) v = __fadd_rn(v, a.bias_values[r * a.bias_stride + b - 1]);
+            return v;
+        };
+        for (int w0 = tid * V; place_of(w0, rank) < row.end; w0 += kAhead * THREADS * V) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int at = w0 + i * THREADS * V, p = place_of(at, rank), t = p - shift, later = place_of(at + kAhead * THREADS * V, rank);
+                if (row.whole(p)) {
+                    float v[V];
+#pragma unroll
+                    for (int u = 0; u < V; ++u) v[u] = to_f32(pack[i].v[u]);
+                    uint32_t ok = bits[i];
+                    if (row.allowed) {                                       // the pack's bits, which two words may hold
+                        ok >>= t & 31;
+                        if ((t & 31) + V > 32) ok = __funnelshift_r(bits[i], row.allowed[(t >> 5) + 1], t & 31);
+                    }
+                    row.load(later, pack[i], bits[i]);                       // on its way while this one is worked on
+                    if (touched)
+#pragma unroll
+                        for (int u = 0; u < V; u += 4) {
+                            uint4* word4 = reinterpret_cast<uint4*>(words + at + u);
+                            const uint4 q = *word4;
+                            if (q.x | q.y | q.z | q.w) {
+                                *word4 = make_uint4(0, 0, 0, 0);
+                                if (q.x) v[u] = touch(v[u], q.x);
+                                if (q.y) v[u + 1] = touch(v[u + 1], q.y);
+                                if (q.z) v[u + 2] = touch(v[u + 2], q.z);
+                                if (q.w) v[u + 3] = touch(v[u + 3], q.w);
+                            }
+                        }
+                    float big = -INFINITY;
+                    Pack<T, V> y;
+#pragma unroll
+                    for (int u = 0; u < V; ++u) {
+                        if (!(ok >> u & 1u)) v[u] = -INFINITY;
+                        best.bad |= !(v[u] < INFINITY);
+                        big = fmaxf(big, v[u]);
+                        y.v[u] = from_f32<T>(v[u]);
+                    }
+                    if (big > best.v) {
+                        best.v = big;
+#pragma unroll
+                        for (int u = V - 1; u >= 0; --u)
+                            if (v[u] == big) best.i = t + u;
+                    }
+                    if (row.wide_out) {
+                        *reinterpret_cast<Pack<T, V>*>(row.o + t) = y;
+                    } else if (row.o) {
+#pragma unroll
+                        for (int u = 0; u < V; ++u) row.o[t + u] = y.v[u];
+                    }
+                } else {
+                    if (p < row.end)
+#pragma unroll 1
+                        for (int u = 0; u < V; ++u) {                        // the row's ends
+                            const int e = t + u;
+                            if (e < 0 || e >= a.vocab) continue;
+                            float v = to_f32(row.x[e]);
+                            if (touched && words[at + u]) {
+                                v = touch(v, words[at + u]);
+                                words[at + u] = 0;
+                            }
+                            if (row.allowed && !(row.allowed[e >> 5] >> (e & 31) & 1u)) v = -INFINITY;
+                            best.bad |= !(v < INFINITY);
+                            if (v > best.v) best.v = v, best.i = e;
+                            if (row.o) row.o[e] = from_f32<T>(v);
+                        }
+                    row.load(later, pack[i], bits[i]);
+                }
+            }
+        }
+        if (r + step < a.rows) {                                         // the next row's first packs
+            const Row<T> next(a, r + step);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) next.load(place_of((i * THREADS + tid) * V, rank), pack[i], bits[i]);
+        }
+        for (int s = 16; s; s >>= 1) {
+            const float v = __shfl_xor_sync(~0u, best.v, s);
+            const int i = __shfl_xor_sync(~0u, best.i, s);
+            better(best, v, i);
+        }
+        best.bad = __any_sync(~0u, best.bad);
+        if ((tid & 31) == 0) wbest[tid >> 5] = best;
+        __syncthreads();                                                 // and every word is 0 again
+        if (tid == 0) {
+            for (int w = 1; w < THREADS / 32; ++w) {
+                better(best, wbest[w].v, wbest[w].i);
+                best.bad |= wbest[w].bad;
+            }
+            *cl.map_shared_rank(&row_best[slot][rank], 0) = best;
+        }
+        __syncwarp();
+        cluster_arrive();
     }
-    cl.sync();                                           // the others' words live until they are read
+    cluster_wait();                                                      // the first CTA's memory lives until all have left theirs
+    const int rows = (a.rows - first + step - 1) / step;
+    join(first + (rows - 1) * step, slot ^ 1);
 }
 
 template <class T, int THREADS>
-cudaError_t launch_pick(const PickArgs& a, int rows, cudaStream_t st) {
+cudaError_t launch_pick(const PickArgs& a, cudaStream_t st) {
     const size_t sm = a.history || a.bias_ids ? (size_t)a.slice * 4 : 0;
     cudaError_t e = cudaFuncSetAttribute((const void*)k_pick<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(rows * kPickCluster));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = sm;
     cfg.stream = st;
@@ -239,6 +291,15 @@ cudaError_t launch_pick(const PickArgs& a, int rows, cudaStream_t st) {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
+    int clusters = 1;
+    if (a.rows > 1) {
+        cfg.gridDim = dim3((unsigned)(a.rows * kPickCluster));
+        e = cudaOccupancyMaxActiveClusters(&clusters, k_pick<T, THREADS>, &cfg);
+        if (e != cudaSuccess) return e;
+        if (clusters < 1) clusters = 1;
+        if (clusters > a.rows) clusters = a.rows;
+    }
+    cfg.gridDim = dim3((unsigned)(clusters * kPickCluster));
     return cudaLaunchKernelEx(&cfg, k_pick<T, THREADS>, a);
 }
 
@@ -274,8 +335,9 @@ QX_API int qx_cuda_pick_tokens(const qx_cuda_pick* p, void* stream, char* err, u
     a.out = p->out;
     a.logits_stride = p->logits_stride;
     a.out_stride = p->out_stride;
+    a.rows = (int)p->rows;
     a.vocab = (int)p->vocab;
-    a.slice = (int)((p->vocab + 7 + kPickCluster * 64 - 1) / (kPickCluster * 64) * 64);      // of vocab and up to 7 places before it
+    a.slice = (int)((p->vocab + 7 + kRound - 1) / kRound * kChunk);      // of vocab and up to 7 places before it
     a.max_history = (int)p->max_history;
     a.max_bias = (int)p->max_bias;
     a.history = p->max_history ? p->history : nullptr;
@@ -294,10 +356,9 @@ QX_API int qx_cuda_pick_tokens(const qx_cuda_pick* p, void* stream, char* err, u
     cudaStream_t st = (cudaStream_t)stream;
     // few rows leave SMs to spare: one CTA of 1024 threads each, else two of 512
     const bool few = p->rows * kPickCluster <= 148;
-    const int rows = (int)p->rows;
     cudaError_t e;
-    if (p->dtype == QX_CUDA_F32) e = few ? launch_pick<float, 1024>(a, rows, st) : launch_pick<float, 512>(a, rows, st);
-    else if (p->dtype == QX_CUDA_F16) e = few ? launch_pick<__half, 1024>(a, rows, st) : launch_pick<__half, 512>(a, rows, st);
-    else e = few ? launch_pick<__nv_bfloat16, 1024>(a, rows, st) : launch_pick<__nv_bfloat16, 512>(a, rows, st);
+    if (p->dtype == QX_CUDA_F32) e = few ? launch_pick<float, 1024>(a, st) : launch_pick<float, 512>(a, st);
+    else if (p->dtype == QX_CUDA_F16) e = few ? launch_pick<__half, 1024>(a, st) : launch_pick<__half, 512>(a, st);
+    else e = few ? launch_pick<__nv_bfloat16, 1024>(a, st) : launch_pick<__nv_bfloat16, 512>(a, st);
     return finish(e, err, n);
 }
