@@ -407,97 +407,212 @@ __global__ void __launch_bounds__(kJoinThreads) k_tree_join(const __grid_constan
 
 // ---- what each cache row got ---------------------------------------------------
 
-// mass[t] += sum over the sequence's query rows of 2^(s_t - lse).  A warp owns
-// 16 cache rows of a tile and goes through all query rows of all KV heads, so
-// the sum has one order and no atomics.
+// mass[t] += sum over the sequence's query rows of 2^(x_t - lse), x_t without
+// vs_t.  The steps of 16 cache rows of all sequences, laid end to end, are
+// shared out evenly over the CTAs.  A CTA holds its sequence's queries in
+// shared memory as F16 operands (in several passes where they are too many),
+// and a warp goes through them with a step's keys in registers: it alone adds
+// to the step's rows, in one order, without atomics.
+constexpr int kMassWarps = 16, kMassThreads = kMassWarps * 32;
+template <int HD, int NT>
+struct Held {                                              // a block of 16 query rows
+    static constexpr int kStride = HD + 8, kTerm = 16 * kStride, kFacs = NT * kTerm * 2, kBytes = kFacs + 16 * 8;
+    static constexpr int kMost = 200 * 1024 / kBytes;
+};
+template <int HD>
+struct StepKeys {
+    uint4 k[2][HD / 64];                                   // key tile h: row 4 (n / 2) + 2 h + n % 2 of the step, n = lane / 4
+    float ks[4];                                           // rows 4 j .. 4 j + 3, j = lane % 4
+    __device__ __forceinline__ void load(const int8_t* k0, const float* ks0, int row_bytes, int r0, int last) {
+        const int lane = threadIdx.x & 31, j = lane & 3, n = lane >> 2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c)
+                k[h][c] = *reinterpret_cast<const uint4*>(k0 + (size_t)min(r0 + 4 * (n >> 1) + 2 * h + (n & 1), last) * row_bytes +
+                                                          64 * c + 16 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ks[i] = ks0[min(r0 + 4 * j + i, last)];
+    }
+};
 template <class T, int HD, int NT>
-__global__ void __launch_bounds__(kTreeThreads) k_tree_mass(TreeArgs a) {
-    constexpr int QS = HD + 8;
-    __shared__ __align__(16) __half qs[NT * 16 * QS];
-    __shared__ float qfac[16];
-    __shared__ __align__(16) uint8_t steps[kTreeWarps][Step<HD>::kBytes];
+__global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_constant__ TreeArgs a) {
+    using Block = Held<HD, NT>;
+    extern __shared__ __align__(128) uint8_t dyn[];
     __shared__ int warp_sum[kScanThreads / 32], at_seq, at_first, clash;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
-    // shares here are of tiles alone, one "unit" a sequence
     const int per = (a.d.seqs + kScanThreads - 1) / kScanThreads;
-    const int s0 = min(a.d.seqs, tid * per), s1 = min(a.d.seqs, s0 + per);
+    const int s0 = tid < kScanThreads ? min(a.d.seqs, tid * per) : 0, s1 = tid < kScanThreads ? min(a.d.seqs, s0 + per) : 0;
+    auto steps_of = [&](int s) {
+        const int len = a.d.lens[s], n = a.d.count(s);
+        return n && fits(a.c, a.d, a.d.slots[s], len, n) ? (len + n + 15) / 16 : 0;
+    };
     int mine = 0;
-    for (int s = s0; s < s1; ++s) mine += seq_work(a, s, false).tiles;
+    for (int s = s0; s < s1; ++s) mine += steps_of(s);
     int inc = mine;
+    if (tid < kScanThreads) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(~0u, inc, o);
-        if (lane >= o) inc += t;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(~0u, inc, o);
+            if (lane >= o) inc += t;
+        }
+        if (lane == 31) warp_sum[warp] = inc;
     }
-    if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
     int first = inc - mine, total = 0;
     for (int i = 0; i < kScanThreads / 32; ++i) {
         if (i < warp) first += warp_sum[i];
         total += warp_sum[i];
     }
-    for (int at = blockIdx.x; at < total; at += gridDim.x) {
+    const int each = total / gridDim.x, extra = total % gridDim.x, cta = blockIdx.x;
+    int at = each * cta + min(cta, extra);
+    const int end = at + each + (cta < extra ? 1 : 0), row_bytes = a.c.kv_heads * HD;
+    while (at < end) {
         __syncthreads();
         if (tid == 0) clash = 0;
         int f = first;
         for (int s = s0; s < s1; ++s) {
-            const int t = seq_work(a, s, false).tiles;
+            const int t = steps_of(s);
             if (at >= f && at < f + t) at_seq = s, at_first = f;
             f += t;
         }
         __syncthreads();
-        const int s = at_seq, slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
-        for (int i = tid; i < a.d.seqs; i += kTreeThreads)
-            if (i != s && a.d.slots[i] == slot && seq_work(a, i, false).tiles) clash = 1;
-        const int r0 = (at - at_first) * kTile + 16 * warp, last = len + n - 1;
+        const int s = at_seq, slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s), last = len + n - 1;
+        const int step0 = at - at_first, step1 = min((last + 16) / 16, end - at_first);
+        for (int i = tid; i < a.d.seqs; i += kMassThreads)
+            if (i != s && a.d.slots[i] == slot && steps_of(i)) clash = 1;
+        at += step1 - step0;
         const size_t base_row = (size_t)slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
-        float got[4] = {};
-        for (int g = 0; g < a.c.kv_heads; ++g) {
-            uint8_t* step = steps[warp];
-            __syncwarp();
-            copy_step<HD>(a.c.k + base_row * a.c.kv_heads * HD + g * HD, a.c.v + base_row * a.c.kv_heads * HD + g * HD, a.c.ks + base_row,
-                          a.c.vs + base_row, a.c.kv_heads * HD, min(r0, last), last, (uint32_t)__cvta_generic_to_shared(step));
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            __syncwarp();
-            const float4 ks4 = *reinterpret_cast<const float4*>(step + 2 * Step<HD>::kCodes + 16 * j);
-            const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
-            for (int row0 = 0; row0 < n * a.group; row0 += 16) {
-                const int have = min(16, n * a.group - row0);
-                __syncthreads();
-                stage_queries<T, HD, NT>(a, s, g, row0, 16, have, qs, QS, 16 * QS, qfac);
-                __syncthreads();
-                float acc[2][4];
-                dot_keys<HD, NT>(qs, QS, 16 * QS, step, acc);
+        const int8_t* k0 = a.c.k + base_row * row_bytes;
+        const float* ks0 = a.c.ks + base_row;
+        const int rows = n * a.group, per_head = (rows + 15) / 16, blocks = per_head * a.c.kv_heads;
+        for (int b0 = 0; b0 < blocks; b0 += Block::kMost) {
+            const int b1 = min(blocks, b0 + Block::kMost);
+            StepKeys<HD> next;
+            if (step0 + warp < step1)
+                next.load(k0 + b0 / per_head * HD, ks0, row_bytes, (step0 + warp) * 16, last);
+            __syncthreads();                               // the blocks before have been used
+            if (clash) break;
+            // the queries as F16 terms, with the factor that undoes their power of two and the row's lse; four rows at
+            // a time, for the latency of their loads
+            for (int i0 = 4 * warp; i0 < 16 * (b1 - b0); i0 += 4 * kMassWarps) {
+                const int b = b0 + i0 / 16, g = b / per_head, row0 = b % per_head * 16 + i0 % 16;
+                __half* to = reinterpret_cast<__half*>(dyn + (size_t)(b - b0) * Block::kBytes) + i0 % 16 * Block::kStride;
+                float2* facs = reinterpret_cast<float2*>(dyn + (size_t)(b - b0) * Block::kBytes + Block::kFacs) + i0 % 16;
+                float x[4][HD / 32], big[4], lg[4];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int r = n8 + 8 * u;
-                    if (r >= have) continue;
-                    const int node = (row0 + r) / a.group, h = g * a.group + (row0 + r) % a.group;
-                    const size_t li = (size_t)s * a.d.max_nodes + node;
-                    const unsigned long long* mrow = a.mask ? a.mask + li * a.words : nullptr;
-                    const float lg = a.lse2[li * a.q_heads + h];
+                for (int u = 0; u < 4; ++u) {
+                    const bool real = row0 + u < rows;
+                    const int node = (row0 + u) / a.group, h = g * a.group + (row0 + u) % a.group;
+                    const size_t q = s * a.q.seq + node * a.q.node + h * a.q.head;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int t = r0 + 4 * j + i;
-                        if (t <= last && sees(mrow, node, t, len, n))
-                            got[i] += exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * qfac[r], ks[i], -lg));
+                    for (int i = 0; i < HD / 32; ++i) x[u][i] = real ? load_q<T>(a.q, q + lane + 32 * i) : 0.f;
+                    lg[u] = real ? a.lse2[((size_t)s * a.d.max_nodes + node) * a.q_heads + h] : 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    big[u] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; ++i) big[u] = fmaxf(big[u], isfinite(x[u][i]) ? fabsf(x[u][i]) : 0.f);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) big[u] = fmaxf(big[u], __shfl_xor_sync(~0u, big[u], o));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const RowScale rs(big[u]);
+#pragma unroll
+                    for (int i = 0; i < HD / 32; ++i) {
+                        const float y = x[u][i] * rs.f0 * rs.f1;
+                        const __half hi = __float2half_rn(y);
+                        to[u * Block::kStride + lane + 32 * i] = hi;
+                        if (NT == 2) to[Block::kTerm + u * Block::kStride + lane + 32 * i] = __float2half_rn(y - __half2float(hi));
                     }
+                    if (lane == 0) facs[u] = make_float2(rs.undo(a.scale), lg[u]);
                 }
             }
-        }
-        __syncthreads();
-        if (clash) {
-            if (tid == 0 && a.status) atomicOr(a.status, QX_CUDA_STATUS_SHARED);
-            continue;
-        }
+            __syncthreads();
+            const int g0 = b0 / per_head, g1 = (b1 - 1) / per_head;
+            for (int st = step0 + warp; st < step1; st += kMassWarps) {
+                const int r0 = st * 16;
+                const bool edge = r0 + 16 > len;
+                float got[4] = {};
+                for (int g = g0; g <= g1; ++g) {
+                    const float ks[4] = {next.ks[0], next.ks[1], next.ks[2], next.ks[3]};
+                    uint32_t key[2][HD / 8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            got[i] += __shfl_xor_sync(~0u, got[i], 4);
-            got[i] += __shfl_xor_sync(~0u, got[i], 8);
-            got[i] += __shfl_xor_sync(~0u, got[i], 16);
-            const int t = r0 + 4 * j + i;
-            if (n8 == 0 && t <= last) a.mass[base_row + t] += got[i];
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < HD / 64; ++c) {
+                            const uint32_t w[4] = {next.k[h][c].x, next.k[h][c].y, next.k[h][c].z, next.k[h][c].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t u = w[i] ^ 0x80808080u;
+                                key[h][8 * c + 2 * i] = low_pair(u);
+                                key[h][8 * c + 2 * i + 1] = high_pair(u);
+                            }
+                        }
+                    const bool more = g < g1;
+                    if (more || st + kMassWarps < step1)
+                        next.load(k0 + (more ? g + 1 : g0) * HD, ks0, row_bytes, more ? r0 : r0 + 16 * kMassWarps, last);
+                    const int first_b = max(b0, g * per_head), end_b = min(b1, (g + 1) * per_head);
+                    for (int b = first_b; b < end_b; ++b) {
+                        const uint8_t* block = dyn + (size_t)(b - b0) * Block::kBytes;
+                        const __half* q0 = reinterpret_cast<const __half*>(block) + n8 * Block::kStride + 16 * j;
+                        float acc[2][4] = {};
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int c = 0; c < HD / 64; ++c) {
+                                uint32_t lo[8], hi[8];
+                                const __half* q = q0 + t * Block::kTerm + 64 * c;
+                                *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(q);
+                                *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(q + 8);
+                                *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(q + 8 * Block::kStride);
+                                *reinterpret_cast<uint4*>(hi + 4) = *reinterpret_cast<const uint4*>(q + 8 * Block::kStride + 8);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t af[4] = {lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1]};
+                                    mma16816(acc[0], af, key[0][8 * c + 2 * i], key[0][8 * c + 2 * i + 1]);
+                                    mma16816(acc[1], af, key[1][8 * c + 2 * i], key[1][8 * c + 2 * i + 1]);
+                                }
+                            }
+                        const int row0 = (b - g * per_head) * 16;
+                        const float2* facs = reinterpret_cast<const float2*>(block + Block::kFacs);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int r = row0 + n8 + 8 * u;
+                            const float2 fl = facs[n8 + 8 * u];
+                            uint32_t seen = 15u;
+                            if (r >= rows) {
+                                seen = 0;
+                            } else if (edge) {
+                                const int node = r / a.group;
+                                const unsigned long long* mrow =
+                                    a.mask ? a.mask + ((size_t)s * a.d.max_nodes + node) * a.words : nullptr;
+                                seen = (uint32_t)sees64(mrow, a.words, node, r0 + 4 * j, len, n);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float e = exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * fl.x, ks[i], -fl.y));
+                                got[i] += seen >> i & 1u ? e : 0.f;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    got[i] += __shfl_xor_sync(~0u, got[i], 4);
+                    got[i] += __shfl_xor_sync(~0u, got[i], 8);
+                    got[i] += __shfl_xor_sync(~0u, got[i], 16);
+                }
+                const float x = n8 == 0 ? got[0] : n8 == 1 ? got[1] : n8 == 2 ? got[2] : got[3];
+                const int t = r0 + 4 * j + n8;
+                if (n8 < 4 && t <= last) a.mass[base_row + t] += x;
+            }
         }
+        if (clash && tid == 0 && a.status) atomicOr(a.status, QX_CUDA_STATUS_SHARED);
     }
 }
 
@@ -557,7 +672,10 @@ cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t
     cfg.numAttrs = 1;
     e = tc ? cudaLaunchKernelEx(&cfg, k_tree_join<T, HD, 8>, a) : cudaLaunchKernelEx(&cfg, k_tree_join<T, HD, 2>, a);
     if (e != cudaSuccess || !a.mass) return e;
-    k_tree_mass<T, HD, NT><<<sms * 4, kTreeThreads, 0, st>>>(a);
+    constexpr int kHeld = Held<HD, NT>::kMost * Held<HD, NT>::kBytes;
+    e = cudaFuncSetAttribute((const void*)k_tree_mass<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld);
+    if (e != cudaSuccess) return e;
+    k_tree_mass<T, HD, NT><<<sms, kMassThreads, kHeld, st>>>(a);
     return cudaGetLastError();
 }
 
