@@ -23,24 +23,35 @@ struct Heads {
     size_t seq, node, head;
 };
 
-struct RopeArgs {
-    Cache c;
-    Drafts d;
-    int layer, q_heads, rd, interleaved;
-    const double* inv_freq;
-    double amplitude;
-    Heads q, qo, k, v;
-    const int* positions;
-    uint32_t* status;
-};
 
-// The items of a head: `pairs` items of V rotated pairs (half layout: V values
-// at i and V at rd / 2 + i; interleaved: 2 V consecutive values), then items
-// of V values that pass through.
+// A tensor's items for V-wide accesses: first every head's `pairs` items of V
+// rotated pairs (half layout: V values at i and V at rd / 2 + i; interleaved:
+// 2 V consecutive values), then every head's `pass` items of V values that go
+// through, so that a warp mostly has items of one kind.
+struct Over {                                            // division by d: the product is at most one too high
+    uint32_t d, by;
+    __host__ __device__ __forceinline__ explicit Over(uint32_t d) : d(d), by(d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+        const uint32_t q = d > 1 ? __umulhi(x, by) : x;
+        return q - (q * d > x);
+    }
+};
+struct Items {
+    Over pairs, pass;
+    int rotated;                                         // in all heads
+    // head, item within it
+    __device__ __forceinline__ bool at(int w, int& h, int& it) const {
+        const bool rot = w < rotated;
+        const Over& o = rot ? pairs : pass;
+        const uint32_t x = rot ? w : w - rotated;
+        h = (int)o(x);
+        it = (int)(x - h * o.d);
+        return rot;
+    }
+};
 template <class T, int V, bool IL>
-__device__ __forceinline__ void load_item(const T* h, int item, int pairs, int rd, T (&a)[V], T (&b)[V], bool& rot) {
-    rot = item < pairs;
-    const int i0 = rot ? (IL ? 2 * V * item : V * item) : rd + V * (item - pairs);
+__device__ __forceinline__ void load_item(const T* h, int item, int rd, bool rot, T (&a)[V], T (&b)[V]) {
+    const int i0 = rot ? (IL ? 2 * V * item : V * item) : rd + V * item;
     const int i1 = IL ? i0 + V : rd / 2 + i0;
     const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(h + i0);
 #pragma unroll
@@ -52,13 +63,44 @@ __device__ __forceinline__ void load_item(const T* h, int item, int pairs, int r
     }
 }
 
-// One CTA per drafted token: a token's 36 heads of 128 are 10 KB, read once
+struct RopeArgs {
+    Cache c;
+    Drafts d;
+    int layer, q_heads, rd, interleaved;
+    const double* inv_freq;
+    double amplitude;
+    Heads q, qo, k, v;
+    Items q_items, k_items;
+    Over v_packs;                                        // V-wide packs of a head
+    const int* positions;
+    uint32_t* status;
+};
+
+// rint(x / scale), clamped, for |x| <= 127.5 scale.  The product with 1 / scale
+// is within 2^-21 of the quotient's size, so below 2^-14 of it, and rounds to
+// the same integer unless that near a half; then the quotient itself decides.
+__device__ __forceinline__ int code_of(float x, float scale, float inv) {
+    if (!isfinite(x)) return 0;
+    const float q = x * inv;
+    float r = rintf(q);
+    if (!(fabsf(q - r) < 0.5f - 0x1p-14f)) r = rintf(__fdiv_rn(x, scale));
+    return max(-127, min(127, (int)r));
+}
+
+// One CTA per drafted token: a token's 40 heads of 128 are 10 KB, read once
 // into registers (queries) or shared memory as F32 (keys and values, which
 // need their row's largest magnitude before they can be quantized).
+//
+// A prompt of 4096 tokens moves 76 MB, 12 us at the memory's rate, and takes
+// 28 us fully rotated, 24 us with half of each head rotated in pairs.  What is left are instructions: the
+// scheduler issues in 62 of 100 cycles, a quarter of them sines and keys in
+// double.  8 CTAs to an SM and one item ahead did best: 2 items 33 us, 3 items
+// and 5 CTAs 40 us, 256 threads 37 us.
 template <class T, int V, bool IL>
-__global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
     extern __shared__ __align__(16) float kvrow[];       // [2][kv]: rotated key, value
     __shared__ double cs_d[2][256 + 1];
+    __shared__ float cs_f[2][256 + 1];
     __shared__ float wmax[2][kRopeThreads / 32];
     __shared__ int clash;
     const int node = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
@@ -72,11 +114,36 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
     if (node >= n) return;
     if (tid == 0) clash = 0;
     const int pos = a.positions ? a.positions[(size_t)s * a.d.max_nodes + node] : len + node;
+    const T* qp = (const T*)a.q.p + s * a.q.seq + node * a.q.node;
+    const T* kp = (const T*)a.k.p + s * a.k.seq + node * a.k.node;
+    const T* vp = (const T*)a.v.p + s * a.v.seq + node * a.v.node;
+    const int per_head = (IL ? rd / (2 * V) : half / V) + (D - rd) / V;
+    const int k_items = a.k.p ? a.c.kv_heads * per_head : 0, v_packs = a.k.p ? KV / V : 0, q_items = a.q.p ? a.q_heads * per_head : 0;
+    auto load_k = [&](int w, T (&x)[V], T (&y)[V]) {
+        int h, it;
+        const bool rot = a.k_items.at(w, h, it);
+        load_item<T, V, IL>(kp + h * a.k.head, it, rd, rot, x, y);
+    };
+    auto load_q = [&](int w, T (&x)[V], T (&y)[V]) {
+        int h, it;
+        const bool rot = a.q_items.at(w, h, it);
+        load_item<T, V, IL>(qp + h * a.q.head, it, rd, rot, x, y);
+    };
+    auto load_v = [&](int w) {
+        const int h = (int)a.v_packs(w);
+        return *reinterpret_cast<const Pack<T, V>*>(vp + h * a.v.head + (w * V - h * D));
+    };
+    // a thread's first items are on their way before the sines are worked out
+    T kx[V], ky[V], qx[V], qy[V];
+    Pack<T, V> vx;
+    if (tid < k_items) load_k(tid, kx, ky);
+    if (tid < v_packs) vx = load_v(tid);
+    if (tid < q_items) load_q(tid, qx, qy);
     for (int i = tid; i < half; i += kRopeThreads) {
         double sn, cn;
         sincos(__dmul_rn((double)pos, a.inv_freq[i]), &sn, &cn);
-        cs_d[0][i] = __dmul_rn(cn, a.amplitude);
-        cs_d[1][i] = __dmul_rn(sn, a.amplitude);
+        cs_f[0][i] = (float)(cs_d[0][i] = __dmul_rn(cn, a.amplitude));
+        cs_f[1][i] = (float)(cs_d[1][i] = __dmul_rn(sn, a.amplitude));
     }
     __syncthreads();
     if (a.k.p)                                           // another sequence of the call that appends to this slot
@@ -85,16 +152,11 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
                 const int m = a.d.count(j);
                 if (m > 0 && fits(a.c, a.d, slot, a.d.lens[j], m)) clash = 1;
             }
-    const int pairs = IL ? rd / (2 * V) : half / V, items = pairs + (D - rd) / V;
     float ka = 0.f, va = 0.f;
     if (a.k.p) {
-        const T* kp = (const T*)a.k.p + s * a.k.seq + node * a.k.node;
-        const T* vp = (const T*)a.v.p + s * a.v.seq + node * a.v.node;
-        for (int w = tid; w < a.c.kv_heads * items; w += kRopeThreads) {
-            const int h = w / items, it = w % items;
-            T x[V], y[V];
-            bool rot;
-            load_item<T, V, IL>(kp + h * a.k.head, it, pairs, rd, x, y, rot);
+        auto key = [&](int w, const T (&x)[V], const T (&y)[V]) {
+            int h, it;
+            const bool rot = a.k_items.at(w, h, it);
             float* o = kvrow + h * D;
             if (rot) {
 #pragma unroll
@@ -115,21 +177,28 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
 #pragma unroll
                 for (int u = 0; u < V; ++u) {
                     const float r = to_f32(x[u]);
-                    o[rd + V * (it - pairs) + u] = r;
+                    o[rd + V * it + u] = r;
                     ka = fmaxf(ka, isfinite(r) ? fabsf(r) : 0.f);
                 }
             }
-        }
-        for (int w = tid; w < KV / V; w += kRopeThreads) {
-            const int h = w * V / D, i = w * V % D;
-            const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(vp + h * a.v.head + i);
+        };
+        auto value = [&](int w, const Pack<T, V>& x) {
 #pragma unroll
             for (int u = 0; u < V; ++u) {
                 const float r = to_f32(x.v[u]);
                 kvrow[KV + w * V + u] = r;
                 va = fmaxf(va, isfinite(r) ? fabsf(r) : 0.f);
             }
+        };
+        if (tid < k_items) key(tid, kx, ky);
+        for (int w = tid + kRopeThreads; w < k_items; w += kRopeThreads) {
+            T x[V], y[V];
+            load_k(w, x, y);
+            key(w, x, y);
         }
+        if (tid < v_packs) value(tid, vx);
+        for (int w = tid + kRopeThreads; w < v_packs; w += kRopeThreads)
+            value(w, load_v(w));
         for (int o = 16; o; o >>= 1) {
             ka = fmaxf(ka, __shfl_xor_sync(~0u, ka, o));
             va = fmaxf(va, __shfl_xor_sync(~0u, va, o));
@@ -142,13 +211,10 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
         return;
     }
     if (a.q.p) {
-        const T* qp = (const T*)a.q.p + s * a.q.seq + node * a.q.node;
         T* qo = (T*)const_cast<void*>(a.qo.p) + s * a.qo.seq + node * a.qo.node;
-        for (int w = tid; w < a.q_heads * items; w += kRopeThreads) {
-            const int h = w / items, it = w % items;
-            T x[V], y[V];
-            bool rot;
-            load_item<T, V, IL>(qp + h * a.q.head, it, pairs, rd, x, y, rot);
+        auto query = [&](int w, const T (&x)[V], const T (&y)[V]) {
+            int h, it;
+            const bool rot = a.q_items.at(w, h, it);
             T* o = qo + h * a.qo.head;
             Pack<T, V> ox, oy;
             if (rot) {
@@ -157,7 +223,7 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
                     const int p = V * it + u;
                     const float x0 = IL ? (2 * u < V ? to_f32(x[(2 * u) % V]) : to_f32(y[(2 * u) % V])) : to_f32(x[u]);
                     const float x1 = IL ? (2 * u + 1 < V ? to_f32(x[(2 * u + 1) % V]) : to_f32(y[(2 * u + 1) % V])) : to_f32(y[u]);
-                    const float c = (float)cs_d[0][p], sn = (float)cs_d[1][p];
+                    const float c = cs_f[0][p], sn = cs_f[1][p];
                     const T r0 = from_f32<T>(x0 * c - x1 * sn), r1 = from_f32<T>(x0 * sn + x1 * c);
                     if (IL) {
                         if (2 * u < V) ox.v[(2 * u) % V] = r0; else oy.v[(2 * u) % V] = r0;
@@ -173,8 +239,14 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
             } else {
 #pragma unroll
                 for (int u = 0; u < V; ++u) ox.v[u] = x[u];
-                *reinterpret_cast<Pack<T, V>*>(o + rd + V * (it - pairs)) = ox;
+                *reinterpret_cast<Pack<T, V>*>(o + rd + V * it) = ox;
             }
+        };
+        if (tid < q_items) query(tid, qx, qy);
+        for (int w = tid + kRopeThreads; w < q_items; w += kRopeThreads) {
+            T x[V], y[V];
+            load_q(w, x, y);
+            query(w, x, y);
         }
     }
     if (!a.k.p) return;
@@ -190,13 +262,12 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
     for (int w = tid; w < 2 * KV / 4; w += kRopeThreads) {
         const bool isv = w >= KV / 4;
         const float4 x = *reinterpret_cast<const float4*>(kvrow + 4 * w);
-        const float sc = isv ? vsc : ksc;
+        const float sc = isv ? vsc : ksc, inv = 1.0f / sc;
         uint32_t word = 0;
         const float e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int code = isfinite(e[u]) ? max(-127, min(127, __float2int_rn(__fdiv_rn(e[u], sc)))) : 0;
-            word |= (uint32_t)(uint8_t)(int8_t)code << (8 * u);
+            word |= (uint32_t)(uint8_t)(int8_t)code_of(e[u], sc, inv) << (8 * u);
         }
         reinterpret_cast<uint32_t*>((isv ? a.c.v : a.c.k) + row * KV)[isv ? w - KV / 4 : w] = word;
     }
@@ -207,7 +278,11 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(RopeArgs a) {
 }
 
 template <class T, int V>
-cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
+cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
+    const uint32_t pairs = (uint32_t)a.rd / (2 * V), pass = (uint32_t)(a.c.head_dim - a.rd) / V;
+    a.q_items = {Over(pairs), Over(pass ? pass : 1), (int)(a.q_heads * pairs)};
+    a.k_items = {Over(pairs), Over(pass ? pass : 1), (int)(a.c.kv_heads * pairs)};
+    a.v_packs = Over((uint32_t)a.c.head_dim / V);
     const dim3 grid((unsigned)a.d.max_nodes, (unsigned)a.d.seqs);
     const size_t sm = a.k.p ? (size_t)2 * a.c.kv_heads * a.c.head_dim * 4 : 0;
     auto fn = a.interleaved ? k_rope_append<T, V, true> : k_rope_append<T, V, false>;
@@ -299,7 +374,7 @@ QX_API int qx_cuda_rope_append(const qx_cuda_kv_cache* cache, uint32_t layer, co
     };
     RopeArgs a{cache_of(cache), drafts_of(drafts), (int)layer, (int)q_heads, (int)rd, rotary->interleaved ? 1 : 0,
                rotary->inv_freq, rotary->amplitude, heads(q, has_q), heads(q_out, has_q), heads(k, has_k),
-               heads(v, has_k), positions, status};
+               heads(v, has_k), {Over(1), Over(1), 0}, {Over(1), Over(1), 0}, Over(1), positions, status};
     // 16-byte accesses where pointers, strides and the rotated part allow; else
     // element by element (odd strides or parts, which a view of a larger
     // projection can have)
