@@ -160,57 +160,99 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
     for (int r = tid; r < a.recent; r += kSelThreads) kept[a.budget - a.recent + r] = last + r;
 }
 
-// Moves the kept rows of one column slice, `rows` rows at a time and
-// kMoveDepth of those in flight; every thread of the CTA calls it.
+// Moves the kept rows of one column slice, kMoveDepth rows of `rows` threads'
+// each to a chunk; every thread of the CTA calls it.  The next chunk's loads
+// and the indexes of the one after are on their way while a chunk is stored.
 template <class W>
 __device__ __forceinline__ void move_columns(const W* src, W* dst, size_t row_words, int col, int row_in_chunk,
                                              int rows, const int* kept, int keep, bool live) {
-    for (int r0 = 0; r0 < keep; r0 += rows * kMoveDepth) {
-        W w[kMoveDepth];
-        int from[kMoveDepth];
+    const int chunk = rows * kMoveDepth;
+    W w[kMoveDepth], w_next[kMoveDepth];
+    int from[kMoveDepth], from_next[kMoveDepth];
+    auto index = [&](int r0, int (&f)[kMoveDepth]) {
 #pragma unroll
         for (int u = 0; u < kMoveDepth; ++u) {
             const int r = r0 + u * rows + row_in_chunk;
-            from[u] = live && r < keep ? kept[r] : -1;
-            if (from[u] >= 0) w[u] = src[(size_t)from[u] * row_words + col];
+            f[u] = live && r < keep ? kept[r] : -1;
         }
+    };
+    auto load = [&](const int (&f)[kMoveDepth], W (&x)[kMoveDepth]) {
+#pragma unroll
+        for (int u = 0; u < kMoveDepth; ++u)
+            if (f[u] >= 0) x[u] = src[(size_t)f[u] * row_words + col];
+    };
+    index(0, from);
+    load(from, w);
+    index(chunk, from_next);
+    for (int r0 = 0; r0 < keep; r0 += chunk) {
+        int from_last[kMoveDepth];
+        load(from_next, w_next);
+        index(r0 + 2 * chunk, from_last);
         __syncthreads();                                 // every load of the chunk has arrived
 #pragma unroll
         for (int u = 0; u < kMoveDepth; ++u) {
             const int r = r0 + u * rows + row_in_chunk;
             if (from[u] >= 0) dst[(size_t)r * row_words + col] = w[u];
+            w[u] = w_next[u];
+            from[u] = from_next[u];
+            from_next[u] = from_last[u];
         }
     }
 }
 
-// grid: (sequence, layer, slice); slices of 128 bytes of K, then of V, then
-// one for the scales and the mass.
-__global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a) {
+// Bound by the memory where there is much to move: 48 layers of 8 sequences of
+// 4096 rows, half of them kept, are 1.6 GB, 250 us at the memory's rate, and take 307 us.  A single
+// sequence is bound by the chain of index, load and store per chunk: slices of
+// 32 bytes make 128 rows of 256 threads' accesses instead of 32, and four times the CTAs (8192
+// rows of one layer, with the selection: 20 us, against 74 us for slices of 128 bytes without
+// the loads ahead).
+//
+// grid: (sequence, layer, slice); slices of 16 LANES bytes of K, then of V,
+// then the key scales, the value scales and the mass.
+template <int LANES>
+__global__ void __launch_bounds__(kMoveThreads) k_evict_move(const __grid_constant__ EvictArgs a) {
     const int s = blockIdx.x, l = blockIdx.y, tid = threadIdx.x;
     const int* kept = a.kept + ((size_t)l * a.seqs + s) * a.budget;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the selection still runs
     if (!evict_fits(a, s)) return;
     const int len = a.lens[s], slot = a.slots[s], dst = a.dst_slots ? a.dst_slots[s] : slot, keep = min(len, a.budget);
     if (keep == 0 || kept[0] < 0) return;                // nothing there, or left out
     if (dst == slot && len <= a.budget) return;
     const size_t from = (size_t)slot * a.c.slot_rows + (size_t)l * a.c.layer_rows;
     const size_t to = (size_t)dst * a.c.slot_rows + (size_t)l * a.c.layer_rows;
-    const int KV = a.c.kv_heads * a.c.head_dim, slices = (KV + 127) / 128;
+    const int KV = a.c.kv_heads * a.c.head_dim, slices = (KV / 16 + LANES - 1) / LANES;
     int slice = blockIdx.z;
     if (slice < 2 * slices) {
         const bool isv = slice >= slices;
         if (isv) slice -= slices;
-        const int words = min(8, KV / 16 - slice * 8), rows = kMoveThreads / 8;
         int8_t* base = isv ? a.c.v : a.c.k;
-        const int col = tid & 7;
-        const bool live = col < words;
-        move_columns<uint4>((const uint4*)(base + from * KV), (uint4*)(base + to * KV), (size_t)KV / 16,
-                            slice * 8 + (live ? col : 0), tid >> 3, rows, kept, keep, live);
+        const int col = tid % LANES + slice * LANES;
+        const bool live = col < KV / 16;
+        move_columns<uint4>((const uint4*)(base + from * KV), (uint4*)(base + to * KV), (size_t)KV / 16, live ? col : 0,
+                            tid / LANES, kMoveThreads / LANES, kept, keep, live);
         return;
     }
-    float* cols[3] = {a.c.ks, a.c.vs, a.mass};
-    for (int j = 0; j < 3; ++j) move_columns<float>(cols[j] + from, cols[j] + to, 1, 0, tid, kMoveThreads, kept, keep, true);
-    __syncthreads();
-    for (int r = keep + tid; r < len; r += kMoveThreads) a.mass[to + r] = 0.f;
+    float* col = slice == 2 * slices ? a.c.ks : slice == 2 * slices + 1 ? a.c.vs : a.mass;
+    move_columns<float>(col + from, col + to, 1, 0, tid, kMoveThreads, kept, keep, true);
+    if (slice == 2 * slices + 2) {
+        __syncthreads();
+        for (int r = keep + tid; r < len; r += kMoveThreads) a.mass[to + r] = 0.f;
+    }
+}
+
+template <int LANES>
+cudaError_t launch_move(const EvictArgs& a, cudaStream_t st) {
+    const unsigned slices = (unsigned)(a.c.kv_heads * a.c.head_dim / 16 + LANES - 1) / LANES;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)a.seqs, (unsigned)a.c.layers, 2 * slices + 3);
+    cfg.blockDim = dim3(kMoveThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_evict_move<LANES>, a);
 }
 
 }  // namespace
@@ -235,7 +277,8 @@ QX_API int qx_cuda_kv_evict(const qx_cuda_kv_cache* cache, uint32_t seqs, const 
     k_evict_select<<<dim3(seqs, cache->layers), kSelThreads, 0, st>>>(a);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return finish(e, err, n);
-    const unsigned slices = (cache->kv_heads * cache->head_dim + 127) / 128;
-    k_evict_move<<<dim3(seqs, cache->layers, 2 * slices + 1), kMoveThreads, 0, st>>>(a);
-    return finish(cudaSuccess, err, n);
+    const uint64_t slices = ((uint64_t)cache->kv_heads * cache->head_dim + 127) / 128;
+    // slices of 32 bytes while those of 128 would leave SMs without two CTAs
+    const bool few = (uint64_t)seqs * cache->layers * 2 * slices < 2 * 148;
+    return finish(few ? launch_move<2>(a, st) : launch_move<8>(a, st), err, n);
 }
