@@ -3,7 +3,7 @@
 //
 // A cluster of CTAs takes row after row; each CTA owns a slice of the
 // vocabulary (every eighth 64 tokens: frequent tokens lie together, and one CTA
-// with all of them held the others up, 131 us against XX for 256 rows of
+// with all of them held the others up, 131 us against 107 for 256 rows of
 // 151936) and keeps one 32-bit word per token of it in shared memory: the
 // token's count in the history (low 20 bits) and the last bias entry that names
 // it, plus one (high 12 bits).  Every CTA reads the whole history and counts
@@ -16,6 +16,14 @@
 // cluster's first CTA, which joins a row's eight while the next is counted: no
 // workspace, one launch, and no wait between rows that the next row's first
 // loads do not overlap.
+//
+// 256 rows of 151936 F32 logits with a mask, 64 biases and histories of 4096
+// move 311 MB, 49 us at the memory's rate, and take 110 us, bound by
+// instructions: of each 128 tokens a warp looks at, three or four are in the
+// history, and each of the four lanes' words costs its branch.  Dearer were: a queue
+// of such tokens per warp, emptied 32 at a time (134 us: its scans), and a second
+// walk over the history that changes them after the pass (134 us: it reads
+// every id again in every CTA).
 //
 // Rows need not start on 16-byte boundaries: a row's tokens are numbered from
 // the boundary before it ("places"), and slices and packs are of places.

@@ -69,15 +69,15 @@ __device__ __forceinline__ void finish_step(uint8_t* step) {
     __syncwarp();
 }
 
-// q . k for 16 query rows (staged at qs) and a step's rows: acc[h] is the
-// accumulator of key tile h.
-template <int HD, int NT>
-__device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qterm, const uint8_t* step, float (&acc)[2][4]) {
+// q . k for MT times 16 query rows (staged at qs) and a step's rows: acc[m][h]
+// is the accumulator of query tile m and key tile h.
+template <int HD, int NT, int MT>
+__device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qterm, const uint8_t* step, float (&acc)[MT][2][4]) {
     const int lane = threadIdx.x & 31, j = lane & 3, n = lane >> 2;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[h][i] = 0.f;
+        for (int i = 0; i < 8; ++i) acc[m][i >> 2][i & 3] = 0.f;
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) {
         uint32_t b[2][8];
@@ -94,20 +94,22 @@ __device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qter
             }
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const __half* q0 = qs + t * qterm + n * qstride + 64 * c + 16 * j;
-            uint32_t lo[8], hi[8];
-            *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(q0);
-            *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(q0 + 8);
-            *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride);
-            *reinterpret_cast<uint4*>(hi + 4) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride + 8);
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t af[4] = {lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1]};
-                mma16816(acc[0], af, b[0][2 * i], b[0][2 * i + 1]);
-                mma16816(acc[1], af, b[1][2 * i], b[1][2 * i + 1]);
+            for (int t = 0; t < NT; ++t) {
+                const __half* q0 = qs + t * qterm + (16 * m + n) * qstride + 64 * c + 16 * j;
+                uint32_t lo[8], hi[8];
+                *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(q0);
+                *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(q0 + 8);
+                *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride);
+                *reinterpret_cast<uint4*>(hi + 4) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride + 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t af[4] = {lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1]};
+                    mma16816(acc[m][0], af, b[0][2 * i], b[0][2 * i + 1]);
+                    mma16816(acc[m][1], af, b[1][2 * i], b[1][2 * i + 1]);
+                }
             }
-        }
     }
 }
 
@@ -147,27 +149,27 @@ __device__ __forceinline__ void stage_queries(const TreeArgs& a, int s, int g, i
 
 // ---- the kernel for small trees ------------------------------------------------
 
-// Blocks of 16 query rows; each of the 4 warps takes 16 of a tile's 64 cache
+// Blocks of 16 MT query rows; each of the 4 warps takes 16 of a tile's 64 cache
 // rows, kRing - 1 tiles ahead, keeps its own m, sum and o, and the four are
 // joined when the unit's part ends.
 constexpr int kRing = 3;
-template <int HD, int NT>
+template <int HD, int NT, int MT>
 struct Small {
-    static constexpr int kQ = NT * 16 * (HD + 8) * 2, kRingBytes = kTreeWarps * kRing * Step<HD>::kBytes;
-    static constexpr int kO = kTreeWarps * 16 * (HD + 4) * 4;             // the warps' o, over the ring
+    static constexpr int kQ = NT * MT * 16 * (HD + 8) * 2, kRingBytes = kTreeWarps * kRing * Step<HD>::kBytes;
+    static constexpr int kO = kTreeWarps * MT * 16 * (HD + 4) * 4;           // the warps' o, over the ring
     static constexpr int kBytes = kQ + (kRingBytes > kO ? kRingBytes : kO);
 };
-template <class T, int HD, int NT>
-__global__ void __launch_bounds__(kTreeThreads, 3) k_tree_small(const __grid_constant__ TreeArgs a) {
-    constexpr int BM = 16, QS = HD + 8, NV = HD / 8;
+template <class T, int HD, int NT, int MT>
+__global__ void __launch_bounds__(kTreeThreads, MT == 1 ? 3 : 2) k_tree_small(const __grid_constant__ TreeArgs a) {
+    constexpr int BM = 16 * MT, QS = HD + 8, NV = HD / 8;
     extern __shared__ __align__(128) uint8_t dyn[];
     __half* qs = reinterpret_cast<__half*>(dyn);
-    float (*wo)[BM][HD + 4] = reinterpret_cast<float (*)[BM][HD + 4]>(dyn + Small<HD, NT>::kQ);
+    float (*wo)[BM][HD + 4] = reinterpret_cast<float (*)[BM][HD + 4]>(dyn + Small<HD, NT, MT>::kQ);
     __shared__ float qfac[BM];
     __shared__ float wm[kTreeWarps][BM], wl[kTreeWarps][BM];
     __shared__ PieceList list;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
-    uint8_t* ring = dyn + Small<HD, NT>::kQ + warp * kRing * Step<HD>::kBytes;
+    uint8_t* ring = dyn + Small<HD, NT, MT>::kQ + warp * kRing * Step<HD>::kBytes;
     const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(ring);
     const int row_bytes = a.c.kv_heads * HD;
     int batch = 0, at = 0;
@@ -186,19 +188,25 @@ __global__ void __launch_bounds__(kTreeThreads, 3) k_tree_small(const __grid_con
         for (int i = 0; i < kRing - 1; ++i) copy(r0 + i * kTile, i);
         stage_queries<T, HD, NT>(a, p.s, p.g, p.row0, BM, p.have, qs, QS, BM * QS, qfac);
         __syncthreads();
-        float m[2], l[2], o[NV][4], fac[2];
-        const unsigned long long* mrow[2];
-        int node[2];
+        // row [t][u] of a lane is the block's row 16 t + 8 u + lane / 4
+        // (top: what raises m; ref: what the exponents are relative to)
+        float m[MT][2], l[MT][2], o[MT][NV][4], fac[MT][2], top[MT][2], ref[MT][2];
+        const unsigned long long* mrow[MT][2];
+        int node[MT][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int r = n8 + 8 * u;
-            m[u] = -INFINITY, l[u] = 0.f;
-            fac[u] = qfac[r];
-            node[u] = r < p.have ? (p.row0 + r) / a.group : -1;
-            mrow[u] = a.mask && r < p.have ? a.mask + ((size_t)p.s * a.d.max_nodes + node[u]) * a.words : nullptr;
-        }
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int d = 0; d < NV; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+            for (int u = 0; u < 2; ++u) {
+                const int r = 16 * t + n8 + 8 * u;
+                m[t][u] = top[t][u] = -INFINITY, l[t][u] = ref[t][u] = 0.f;
+                fac[t][u] = qfac[r];
+                node[t][u] = r < p.have ? (p.row0 + r) / a.group : -1;
+                mrow[t][u] = a.mask && r < p.have ? a.mask + ((size_t)p.s * a.d.max_nodes + node[t][u]) * a.words : nullptr;
+            }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int d = 0; d < NV; ++d) o[t][d][0] = o[t][d][1] = o[t][d][2] = o[t][d][3] = 0.f;
         for (; r0 < stop; r0 += kTile) {
             __syncwarp();                                              // the slot to fill has been read
             copy(r0 + (kRing - 1) * kTile, slot == 0 ? kRing - 1 : slot - 1);
@@ -212,50 +220,65 @@ __global__ void __launch_bounds__(kTreeThreads, 3) k_tree_small(const __grid_con
             *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(f + 4 * j);
             *reinterpret_cast<float4*>(lv) = *reinterpret_cast<const float4*>(f + 32 + 4 * j);
             *reinterpret_cast<float4*>(iv) = *reinterpret_cast<const float4*>(f + 48 + 4 * j);
-            const bool edge = r0 + 16 > p.len;
-            float acc[2][4];
-            dot_keys<HD, NT>(qs, QS, BM * QS, step, acc);
-            // acc[h][2 u + c]: query row n8 + 8 u, cache row r0 + 4 j + 2 h + c
-            float x[2][4], up[2];
-            bool grew = false;
+            float acc[MT][2][4];
+            dot_keys<HD, NT, MT>(qs, QS, BM * QS, step, acc);
+            // acc[t][h][2 u + c]: row [t][u], cache row r0 + 4 j + 2 h + c
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[u][i] = fmaf(acc[i >> 1][2 * u + (i & 1)] * fac[u], ks[i], lv[i]);
-                    if (edge && (node[u] < 0 || !sees(mrow[u], node[u], r0 + 4 * j + i, p.len, p.n))) x[u][i] = -INFINITY;
+                for (int e = 0; e < 8; ++e) {
+                    const int u = e >> 1 & 1, i = (e >> 2) * 2 + (e & 1);
+                    acc[t][e >> 2][e & 3] = fmaf(acc[t][e >> 2][e & 3] * fac[t][u], ks[i], lv[i]);
                 }
-                float mx = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
-                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-                up[u] = mx > m[u] + kSlack || m[u] == -INFINITY ? fmaxf(mx, m[u]) : m[u];
-                grew |= up[u] > m[u];
+            if (r0 + 16 > p.len) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        uint32_t seen = 0;
+                        if (node[t][u] >= 0) seen = (uint32_t)sees64(mrow[t][u], a.words, node[t][u], r0 + 4 * j, p.len, p.n);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!(seen >> i & 1u)) acc[t][i >> 1][2 * u + (i & 1)] = -INFINITY;
+                    }
             }
-            if (__any_sync(~0u, grew)) {
+            uint32_t w[MT][NT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                float mx[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const float f = up[u] > m[u] ? exp2_fast(m[u] - up[u]) : 1.f;
-                    l[u] *= f;
-#pragma unroll
-                    for (int d = 0; d < NV; ++d) o[d][2 * u] *= f, o[d][2 * u + 1] *= f;
-                    m[u] = up[u];
+                    mx[u] = fmaxf(fmaxf(acc[t][0][2 * u], acc[t][0][2 * u + 1]), fmaxf(acc[t][1][2 * u], acc[t][1][2 * u + 1]));
+                    mx[u] = fmaxf(mx[u], __shfl_xor_sync(~0u, mx[u], 1));
+                    mx[u] = fmaxf(mx[u], __shfl_xor_sync(~0u, mx[u], 2));
                 }
-            }
-            uint32_t w[NT][4];
+                if (__any_sync(~0u, mx[0] > top[t][0] || mx[1] > top[t][1])) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float ref = m[u] == -INFINITY ? 0.f : m[u] - kPBias;
-                float e[4];
+                    for (int u = 0; u < 2; ++u) {
+                        if (!(mx[u] > top[t][u])) mx[u] = m[t][u];
+                        const float f = mx[u] > m[t][u] ? exp2_fast(m[t][u] - mx[u]) : 1.f;
+                        l[t][u] *= f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[i] = exp2_fast(x[u][i] - ref);
-                    l[u] = fmaf(e[i], iv[i], l[u]);
+                        for (int d = 0; d < NV; ++d) o[t][d][2 * u] *= f, o[t][d][2 * u + 1] *= f;
+                        m[t][u] = mx[u];
+                        top[t][u] = mx[u] + kSlack;
+                        ref[t][u] = mx[u] == -INFINITY ? 0.f : mx[u] - kPBias;
+                    }
                 }
-                w[0][u] = pack_half(e[0], e[1]);
-                w[0][2 + u] = pack_half(e[2], e[3]);
-                if (NT == 2) {
-                    w[NT - 1][u] = rest_half(e[0], e[1], w[0][u]);
-                    w[NT - 1][2 + u] = rest_half(e[2], e[3], w[0][2 + u]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        e[i] = exp2_fast(acc[t][i >> 1][2 * u + (i & 1)] - ref[t][u]);
+                        l[t][u] = fmaf(e[i], iv[i], l[t][u]);
+                    }
+                    w[t][0][u] = pack_half(e[0], e[1]);
+                    w[t][0][2 + u] = pack_half(e[2], e[3]);
+                    if (NT == 2) {
+                        w[t][NT - 1][u] = rest_half(e[0], e[1], w[t][0][u]);
+                        w[t][NT - 1][2 + u] = rest_half(e[2], e[3], w[t][0][2 + u]);
+                    }
                 }
             }
             // values: dims (lane / 4) * NV + d of rows 4 j .. 4 j + 3 are column lane / 4 of value tile d
@@ -282,25 +305,30 @@ __global__ void __launch_bounds__(kTreeThreads, 3) k_tree_small(const __grid_con
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
-                    for (int q = 0; q < NT; ++q) mma16816(o[4 * d4 + d], w[q], b0[d], b1[d]);
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int q = 0; q < NT; ++q) mma16816(o[t][4 * d4 + d], w[t][q], b0[d], b1[d]);
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();                                               // every warp's steps are read: its o may go over them
         // join the four warps
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            l[u] += __shfl_xor_sync(~0u, l[u], 1);
-            l[u] += __shfl_xor_sync(~0u, l[u], 2);
-            if (j == 0) wm[warp][n8 + 8 * u] = m[u], wl[warp][n8 + 8 * u] = l[u];
-            // columns 2 j, 2 j + 1 of value tile d are dims 2 j NV + d and (2 j + 1) NV + d
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int u = 0; u < 2; ++u) {
+                const int r = 16 * t + n8 + 8 * u;
+                l[t][u] += __shfl_xor_sync(~0u, l[t][u], 1);
+                l[t][u] += __shfl_xor_sync(~0u, l[t][u], 2);
+                if (j == 0) wm[warp][r] = m[t][u], wl[warp][r] = l[t][u];
+                // columns 2 j, 2 j + 1 of value tile d are dims 2 j NV + d and (2 j + 1) NV + d
 #pragma unroll
-                for (int d = 0; d < NV; d += 4)
-                    *reinterpret_cast<float4*>(&wo[warp][n8 + 8 * u][(2 * j + c) * NV + d]) =
-                        make_float4(o[d][2 * u + c], o[d + 1][2 * u + c], o[d + 2][2 * u + c], o[d + 3][2 * u + c]);
-        }
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int d = 0; d < NV; d += 4)
+                        *reinterpret_cast<float4*>(&wo[warp][r][(2 * j + c) * NV + d]) = make_float4(
+                            o[t][d][2 * u + c], o[t][d + 1][2 * u + c], o[t][d + 2][2 * u + c], o[t][d + 3][2 * u + c]);
+            }
         __syncthreads();
         float* part = part_of(a, blockIdx.x, p.begins);
         for (int i = tid; i < BM * (HD / 8); i += kTreeThreads) {
@@ -624,13 +652,17 @@ struct Plan {
     uint64_t parts, joins, lse2;     // bytes of workspace
     uint64_t all() const { return (parts + joins + lse2 + 255) / 256 * 256; }
 };
+// the most CTAs that a call with blocks of so many rows has: they set what the workspace holds
+constexpr int most_ctas(int block_rows) { return block_rows == 128 ? kMaxCtas / 8 : block_rows == 32 ? kMaxCtas / 4 : kMaxCtas; }
 Plan plan_of(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim) {
     Plan p{};
     const uint64_t rows = (uint64_t)max_nodes * (q_heads / kv_heads);
     p.tc = rows > 32;
-    p.block_rows = p.tc ? 128 : 16;
+    // 64 sequences of 4096 rows, BF16: 16 query rows to a KV head 74 us in blocks of 16; 32 rows 126 us in blocks of 32,
+    // 146 us in two of 16; 64 rows 139 us on tcgen05, whose time hardly depends on how many of the 128 rows there are.
+    p.block_rows = p.tc ? 128 : rows > 16 ? 32 : 16;
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
-    p.parts = (uint64_t)2 * (p.tc ? kMaxCtas / 8 : kMaxCtas) * p.block_rows * (kPartHead + head_dim) * 4;
+    p.parts = (uint64_t)2 * most_ctas(p.block_rows) * p.block_rows * (kPartHead + head_dim) * 4;
     p.joins = (uint64_t)(kMaxCtas * sizeof(Join) + 255) / 256 * 256;
     p.lse2 = (uint64_t)seqs * max_nodes * q_heads * 4;
     return p;
@@ -644,22 +676,24 @@ const char* check_shape(uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, 
     return nullptr;
 }
 
+template <class T, int HD, int NT, int MT>
+cudaError_t launch_small(TreeArgs& a, int sms, cudaStream_t st) {
+    int per = 0;
+    constexpr int kBytes = Small<HD, NT, MT>::kBytes;
+    const auto kernel = k_tree_small<T, HD, NT, MT>;
+    cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kTreeThreads, kBytes);
+    if (e != cudaSuccess) return e;
+    a.ctas = sms * (per < 1 ? 1 : per);
+    if (a.ctas > most_ctas(16 * MT)) a.ctas = most_ctas(16 * MT);
+    kernel<<<a.ctas, kTreeThreads, kBytes, st>>>(a);
+    return cudaGetLastError();
+}
 template <class T, int HD, int NT>
 cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t st) {
-    cudaError_t e;
-    if (tc) {
-        e = launch_tree_tc(a, type, sms, st);
-    } else {
-        int per = 0;
-        constexpr int kBytes = Small<HD, NT>::kBytes;
-        e = cudaFuncSetAttribute((const void*)k_tree_small<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_tree_small<T, HD, NT>, kTreeThreads, kBytes);
-        if (e != cudaSuccess) return e;
-        a.ctas = sms * (per < 1 ? 1 : per);
-        if (a.ctas > kMaxCtas) a.ctas = kMaxCtas;
-        k_tree_small<T, HD, NT><<<a.ctas, kTreeThreads, kBytes, st>>>(a);
-        e = cudaGetLastError();
-    }
+    cudaError_t e = tc                   ? launch_tree_tc(a, type, sms, st)
+                    : a.block_rows == 16 ? launch_small<T, HD, NT, 1>(a, sms, st)
+                                         : launch_small<T, HD, NT, 2>(a, sms, st);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)(a.block_rows / (tc ? 8 : 2)));

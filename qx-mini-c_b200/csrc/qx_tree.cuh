@@ -282,14 +282,7 @@ __device__ __forceinline__ float inv_vs(float vs) {
 
 // ---- visibility ----------------------------------------------------------------
 
-// Whether a node sees row t of its sequence (mrow: its mask words, or null).
-__device__ __forceinline__ bool sees(const unsigned long long* mrow, int node, int t, int len, int n) {
-    if (t < len) return true;
-    const int b = t - len;
-    if (b >= n) return false;
-    return mrow ? (mrow[b >> 6] >> (b & 63)) & 1ull : b <= node;
-}
-// The same for the 64 rows from t0 on, as bits.
+// Which of the 64 rows from t0 on a node sees, as bits (mrow: its mask words, or null).
 __device__ __forceinline__ unsigned long long sees64(const unsigned long long* mrow, int words, int node, int t0, int len,
                                                      int n) {
     const unsigned long long all = ~0ull;
