@@ -19,8 +19,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <class T>
-__device__ __forceinline__ float load_q(const Tensor& q, size_t at) { return to_f32(((const T*)q.p)[at]); }
 
 // ---- one warp's 16 cache rows --------------------------------------------------
 
@@ -69,82 +67,99 @@ __device__ __forceinline__ void finish_step(uint8_t* step) {
     __syncwarp();
 }
 
-// q . k for MT times 16 query rows (staged at qs) and a step's rows: acc[m][h]
-// is the accumulator of query tile m and key tile h.
-template <int HD, int NT, int MT>
-__device__ __forceinline__ void dot_keys(const __half* qs, int qstride, int qterm, const uint8_t* step, float (&acc)[MT][2][4]) {
-    const int lane = threadIdx.x & 31, j = lane & 3, n = lane >> 2;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[m][i >> 2][i & 3] = 0.f;
-#pragma unroll
-    for (int c = 0; c < HD / 64; ++c) {
-        uint32_t b[2][8];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int row = 4 * (n >> 1) + 2 * h + (n & 1);
-            const uint4 k = *reinterpret_cast<const uint4*>(step + row * HD + 16 * Step<HD>::k_chunk(row, 4 * c + j));
-            const uint32_t w[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t u = w[i] ^ 0x80808080u;
-                b[h][2 * i] = low_pair(u);
-                b[h][2 * i + 1] = high_pair(u);
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const __half* q0 = qs + t * qterm + (16 * m + n) * qstride + 64 * c + 16 * j;
-                uint32_t lo[8], hi[8];
-                *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(q0);
-                *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(q0 + 8);
-                *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride);
-                *reinterpret_cast<uint4*>(hi + 4) = *reinterpret_cast<const uint4*>(q0 + 8 * qstride + 8);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t af[4] = {lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1]};
-                    mma16816(acc[m][0], af, b[0][2 * i], b[0][2 * i + 1]);
-                    mma16816(acc[m][1], af, b[1][2 * i], b[1][2 * i + 1]);
-                }
-            }
-    }
-}
+// A block of 16 query rows as the products' A operand, in the order in which the
+// lanes take it: 16 bytes a lane (rows n and n + 8 of dims d, d + 1, then of d + 2,
+// d + 3; n = lane / 4, d = 64 c + 16 j + 4 i, j = lane % 4) for each c, i and F16 term.
+template <int HD, int NT>
+struct QBlock {
+    static constexpr int kFrag = 512 + 32;                 // the gap keeps the staging's stores apart
+    static constexpr int kTerm = HD / 16 * kFrag, kBytes = NT * kTerm;
+};
 
-// Stage `rows` query rows (from row0 on, `have` of them real) as F16 terms and
-// the factor that undoes their power of two; whole CTA.
+// Stages rows 2 part, 2 part + 1 and those 8 further of the block at row0 of KV
+// head g, `rows` rows in all; undo: the factors that undo their powers of two.
+// Whole warp, four rows at a time for the latency of their loads.
 template <class T, int HD, int NT>
-__device__ __forceinline__ void stage_queries(const TreeArgs& a, int s, int g, int row0, int rows, int have, __half* qs,
-                                              int qstride, int qterm, float* qfac) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    for (int r = w; r < rows; r += nw) {
-        float x[HD / 32];
-        float big = 0.f;
-        if (r < have) {
-            const int node = (row0 + r) / a.group, h = g * a.group + (row0 + r) % a.group;
-            const size_t at = s * a.q.seq + node * a.q.node + h * a.q.head;
+__device__ __forceinline__ void stage_rows(const TreeArgs& a, int s, int g, int row0, int rows, int part, uint8_t* block,
+                                           float (&undo)[4]) {
+    constexpr int E = HD / 32;                             // dims of a lane
+    const int lane = threadIdx.x & 31;
+    Pack<T, E> x[4];
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-                x[i] = load_q<T>(a.q, at + lane + 32 * i);
-                big = fmaxf(big, isfinite(x[i]) ? fabsf(x[i]) : 0.f);
-            }
+    for (int u = 0; u < 4; ++u) {
+        const int r = row0 + 2 * part + (u >> 1) + 8 * (u & 1);
+        const T* q = (const T*)a.q.p + s * a.q.seq + (size_t)(r / a.group) * a.q.node +
+                     (size_t)(g * a.group + r % a.group) * a.q.head + lane * E;
+        if (r < rows && a.wide) {
+            x[u] = *reinterpret_cast<const Pack<T, E>*>(q);
         } else {
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) x[i] = 0.f;
+            for (int e = 0; e < E; ++e) x[u].v[e] = r < rows ? q[e] : from_f32<T>(0.f);
         }
-        for (int o = 16; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
-        const RowScale rs(big);
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-            const float y = x[i] * rs.f0 * rs.f1;
-            const __half hi = __float2half_rn(y);
-            qs[r * qstride + lane + 32 * i] = hi;
-            if (NT == 2) qs[qterm + r * qstride + lane + 32 * i] = __float2half_rn(y - __half2float(hi));
-        }
-        if (lane == 0) qfac[r] = rs.undo(a.scale);
     }
+    float big[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        big[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float y = to_f32(x[u].v[e]);
+            big[u] = fmaxf(big[u], isfinite(y) ? fabsf(y) : 0.f);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) big[u] = fmaxf(big[u], __shfl_xor_sync(~0u, big[u], o));
+    uint32_t w[NT][4][E / 2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const RowScale rs(big[u]);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const float y0 = to_f32(x[u].v[e]) * rs.f0 * rs.f1, y1 = to_f32(x[u].v[e + 1]) * rs.f0 * rs.f1;
+            w[0][u][e / 2] = pack_half(y0, y1);
+            if (NT == 2) w[NT - 1][u][e / 2] = rest_half(y0, y1, w[0][u][e / 2]);
+        }
+        undo[u] = rs.undo(a.scale);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            uint8_t* to = block + t * QBlock<HD, NT>::kTerm + (2 * part + v) * 64;
+            if (HD == 128)
+                *reinterpret_cast<uint4*>(to + ((lane >> 4) * 4 + (lane & 3)) * QBlock<HD, NT>::kFrag + (lane >> 2 & 3) * 16) =
+                    make_uint4(w[t][2 * v][0], w[t][2 * v + 1][0], w[t][2 * v][E / 2 - 1], w[t][2 * v + 1][E / 2 - 1]);
+            else
+                *reinterpret_cast<uint2*>(to + (lane >> 1 & 3) * QBlock<HD, NT>::kFrag + (lane >> 3) * 16 + (lane & 1) * 8) =
+                    make_uint2(w[t][2 * v][0], w[t][2 * v + 1][0]);
+        }
+}
+
+// Key codes as the B operand: 16 bytes of a lane are eight words.
+__device__ __forceinline__ void key_halves(const uint4& k, uint32_t* b) {
+    const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = w[i] ^ 0x80808080u;
+        b[2 * i] = low_pair(u);
+        b[2 * i + 1] = high_pair(u);
+    }
+}
+// acc[h] += q . k of a staged block and key tile h, dims 64 c to 64 c + 63 (b: their key_halves).
+template <int HD, int NT>
+__device__ __forceinline__ void dot_block(const uint8_t* block, int c, const uint32_t* b0, const uint32_t* b1, float (&acc)[2][4]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 q = *reinterpret_cast<const uint4*>(block + t * QBlock<HD, NT>::kTerm + (4 * c + i) * QBlock<HD, NT>::kFrag +
+                                                            16 * (threadIdx.x & 31));
+            const uint32_t af[4] = {q.x, q.y, q.z, q.w};
+            mma16816(acc[0], af, b0[2 * i], b0[2 * i + 1]);
+            mma16816(acc[1], af, b1[2 * i], b1[2 * i + 1]);
+        }
 }
 
 // ---- the kernel for small trees ------------------------------------------------
@@ -155,15 +170,14 @@ __device__ __forceinline__ void stage_queries(const TreeArgs& a, int s, int g, i
 constexpr int kRing = 3;
 template <int HD, int NT, int MT>
 struct Small {
-    static constexpr int kQ = NT * MT * 16 * (HD + 8) * 2, kRingBytes = kTreeWarps * kRing * Step<HD>::kBytes;
+    static constexpr int kQ = MT * QBlock<HD, NT>::kBytes, kRingBytes = kTreeWarps * kRing * Step<HD>::kBytes;
     static constexpr int kO = kTreeWarps * MT * 16 * (HD + 4) * 4;           // the warps' o, over the ring
     static constexpr int kBytes = kQ + (kRingBytes > kO ? kRingBytes : kO);
 };
 template <class T, int HD, int NT, int MT>
 __global__ void __launch_bounds__(kTreeThreads, MT == 1 ? 3 : 2) k_tree_small(const __grid_constant__ TreeArgs a) {
-    constexpr int BM = 16 * MT, QS = HD + 8, NV = HD / 8;
+    constexpr int BM = 16 * MT, NV = HD / 8;
     extern __shared__ __align__(128) uint8_t dyn[];
-    __half* qs = reinterpret_cast<__half*>(dyn);
     float (*wo)[BM][HD + 4] = reinterpret_cast<float (*)[BM][HD + 4]>(dyn + Small<HD, NT, MT>::kQ);
     __shared__ float qfac[BM];
     __shared__ float wm[kTreeWarps][BM], wl[kTreeWarps][BM];
@@ -186,7 +200,12 @@ __global__ void __launch_bounds__(kTreeThreads, MT == 1 ? 3 : 2) k_tree_small(co
         };
 #pragma unroll
         for (int i = 0; i < kRing - 1; ++i) copy(r0 + i * kTile, i);
-        stage_queries<T, HD, NT>(a, p.s, p.g, p.row0, BM, p.have, qs, QS, BM * QS, qfac);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            float undo[4];
+            stage_rows<T, HD, NT>(a, p.s, p.g, p.row0 + 16 * t, p.row0 + p.have, warp, dyn + t * QBlock<HD, NT>::kBytes, undo);
+            if (lane < 4) qfac[16 * t + 2 * warp + (lane >> 1) + 8 * (lane & 1)] = lane == 0 ? undo[0] : lane == 1 ? undo[1] : lane == 2 ? undo[2] : undo[3];
+        }
         __syncthreads();
         // row [t][u] of a lane is the block's row 16 t + 8 u + lane / 4
         // (top: what raises m; ref: what the exponents are relative to)
@@ -220,8 +239,18 @@ __global__ void __launch_bounds__(kTreeThreads, MT == 1 ? 3 : 2) k_tree_small(co
             *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(f + 4 * j);
             *reinterpret_cast<float4*>(lv) = *reinterpret_cast<const float4*>(f + 32 + 4 * j);
             *reinterpret_cast<float4*>(iv) = *reinterpret_cast<const float4*>(f + 48 + 4 * j);
-            float acc[MT][2][4];
-            dot_keys<HD, NT, MT>(qs, QS, BM * QS, step, acc);
+            float acc[MT][2][4] = {};
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {
+                uint32_t b[2][8];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = 4 * (n8 >> 1) + 2 * h + (n8 & 1);
+                    key_halves(*reinterpret_cast<const uint4*>(step + row * HD + 16 * Step<HD>::k_chunk(row, 4 * c + j)), b[h]);
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) dot_block<HD, NT>(dyn + t * QBlock<HD, NT>::kBytes, c, b[0], b[1], acc[t]);
+            }
             // acc[t][h][2 u + c]: row [t][u], cache row r0 + 4 j + 2 h + c
 #pragma unroll
             for (int t = 0; t < MT; ++t)
@@ -443,9 +472,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_tree_join(const __grid_constan
 // to the step's rows, in one order, without atomics.
 constexpr int kMassWarps = 16, kMassThreads = kMassWarps * 32;
 template <int HD, int NT>
-struct Held {                                              // a block of 16 query rows
-    static constexpr int kStride = HD + 8, kTerm = 16 * kStride, kFacs = NT * kTerm * 2, kBytes = kFacs + 16 * 8;
-    static constexpr int kMost = 200 * 1024 / kBytes;
+struct Held {                                              // a QBlock, and its rows' factors and lse
+    static constexpr int kFacs = QBlock<HD, NT>::kBytes, kBytes = kFacs + 16 * 8, kMost = 200 * 1024 / kBytes;
 };
 template <int HD>
 struct StepKeys {
@@ -521,44 +549,16 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_cons
                 next.load(k0 + b0 / per_head * HD, ks0, row_bytes, (step0 + warp) * 16, last);
             __syncthreads();                               // the blocks before have been used
             if (clash) break;
-            // the queries as F16 terms, with the factor that undoes their power of two and the row's lse; four rows at
-            // a time, for the latency of their loads
-            for (int i0 = 4 * warp; i0 < 16 * (b1 - b0); i0 += 4 * kMassWarps) {
-                const int b = b0 + i0 / 16, g = b / per_head, row0 = b % per_head * 16 + i0 % 16;
-                __half* to = reinterpret_cast<__half*>(dyn + (size_t)(b - b0) * Block::kBytes) + i0 % 16 * Block::kStride;
-                float2* facs = reinterpret_cast<float2*>(dyn + (size_t)(b - b0) * Block::kBytes + Block::kFacs) + i0 % 16;
-                float x[4][HD / 32], big[4], lg[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const bool real = row0 + u < rows;
-                    const int node = (row0 + u) / a.group, h = g * a.group + (row0 + u) % a.group;
-                    const size_t q = s * a.q.seq + node * a.q.node + h * a.q.head;
-#pragma unroll
-                    for (int i = 0; i < HD / 32; ++i) x[u][i] = real ? load_q<T>(a.q, q + lane + 32 * i) : 0.f;
-                    lg[u] = real ? a.lse2[((size_t)s * a.d.max_nodes + node) * a.q_heads + h] : 0.f;
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    big[u] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < HD / 32; ++i) big[u] = fmaxf(big[u], isfinite(x[u][i]) ? fabsf(x[u][i]) : 0.f);
-                }
-#pragma unroll
-                for (int o = 16; o; o >>= 1)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) big[u] = fmaxf(big[u], __shfl_xor_sync(~0u, big[u], o));
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const RowScale rs(big[u]);
-#pragma unroll
-                    for (int i = 0; i < HD / 32; ++i) {
-                        const float y = x[u][i] * rs.f0 * rs.f1;
-                        const __half hi = __float2half_rn(y);
-                        to[u * Block::kStride + lane + 32 * i] = hi;
-                        if (NT == 2) to[Block::kTerm + u * Block::kStride + lane + 32 * i] = __float2half_rn(y - __half2float(hi));
-                    }
-                    if (lane == 0) facs[u] = make_float2(rs.undo(a.scale), lg[u]);
-                }
+            for (int i = warp; i < 4 * (b1 - b0); i += kMassWarps) {
+                const int b = b0 + i / 4, part = i % 4, g = b / per_head, row0 = b % per_head * 16;
+                uint8_t* block = dyn + (size_t)(b - b0) * Block::kBytes;
+                const int row = 2 * part + (lane >> 1 & 1) + 8 * (lane & 1), r = row0 + row;
+                const float lg = lane < 4 && r < rows ? a.lse2[((size_t)s * a.d.max_nodes + r / a.group) * a.q_heads + g * a.group + r % a.group] : 0.f;
+                float undo[4];
+                stage_rows<T, HD, NT>(a, s, g, row0, rows, part, block, undo);
+                if (lane < 4)
+                    reinterpret_cast<float2*>(block + Block::kFacs)[row] =
+                        make_float2(lane == 0 ? undo[0] : lane == 1 ? undo[1] : lane == 2 ? undo[2] : undo[3], lg);
             }
             __syncthreads();
             const int g0 = b0 / per_head, g1 = (b1 - 1) / per_head;
@@ -572,61 +572,41 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_cons
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int c = 0; c < HD / 64; ++c) {
-                            const uint32_t w[4] = {next.k[h][c].x, next.k[h][c].y, next.k[h][c].z, next.k[h][c].w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t u = w[i] ^ 0x80808080u;
-                                key[h][8 * c + 2 * i] = low_pair(u);
-                                key[h][8 * c + 2 * i + 1] = high_pair(u);
-                            }
-                        }
+                        for (int c = 0; c < HD / 64; ++c) key_halves(next.k[h][c], key[h] + 8 * c);
                     const bool more = g < g1;
                     if (more || st + kMassWarps < step1)
                         next.load(k0 + (more ? g + 1 : g0) * HD, ks0, row_bytes, more ? r0 : r0 + 16 * kMassWarps, last);
                     const int first_b = max(b0, g * per_head), end_b = min(b1, (g + 1) * per_head);
                     for (int b = first_b; b < end_b; ++b) {
                         const uint8_t* block = dyn + (size_t)(b - b0) * Block::kBytes;
-                        const __half* q0 = reinterpret_cast<const __half*>(block) + n8 * Block::kStride + 16 * j;
                         float acc[2][4] = {};
 #pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int c = 0; c < HD / 64; ++c) {
-                                uint32_t lo[8], hi[8];
-                                const __half* q = q0 + t * Block::kTerm + 64 * c;
-                                *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(q);
-                                *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(q + 8);
-                                *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(q + 8 * Block::kStride);
-                                *reinterpret_cast<uint4*>(hi + 4) = *reinterpret_cast<const uint4*>(q + 8 * Block::kStride + 8);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const uint32_t af[4] = {lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1]};
-                                    mma16816(acc[0], af, key[0][8 * c + 2 * i], key[0][8 * c + 2 * i + 1]);
-                                    mma16816(acc[1], af, key[1][8 * c + 2 * i], key[1][8 * c + 2 * i + 1]);
-                                }
-                            }
+                        for (int c = 0; c < HD / 64; ++c) dot_block<HD, NT>(block, c, key[0] + 8 * c, key[1] + 8 * c, acc);
                         const int row0 = (b - g * per_head) * 16;
                         const float2* facs = reinterpret_cast<const float2*>(block + Block::kFacs);
+                        float e[2][4];
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            const int r = row0 + n8 + 8 * u;
                             const float2 fl = facs[n8 + 8 * u];
-                            uint32_t seen = 15u;
-                            if (r >= rows) {
-                                seen = 0;
-                            } else if (edge) {
-                                const int node = r / a.group;
-                                const unsigned long long* mrow =
-                                    a.mask ? a.mask + ((size_t)s * a.d.max_nodes + node) * a.words : nullptr;
-                                seen = (uint32_t)sees64(mrow, a.words, node, r0 + 4 * j, len, n);
-                            }
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float e = exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * fl.x, ks[i], -fl.y));
-                                got[i] += seen >> i & 1u ? e : 0.f;
+                            for (int i = 0; i < 4; ++i)
+                                e[u][i] = exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * fl.x, ks[i], -fl.y));
+                        }
+                        if (edge || row0 + 16 > rows) {
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const int r = row0 + n8 + 8 * u, node = r / a.group;
+                                uint32_t seen = r < rows ? 15u : 0u;
+                                if (edge && r < rows)
+                                    seen = (uint32_t)sees64(a.mask ? a.mask + ((size_t)s * a.d.max_nodes + node) * a.words : nullptr,
+                                                            a.words, node, r0 + 4 * j, len, n);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (!(seen >> i & 1u)) e[u][i] = 0.f;
                             }
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) got[i] += e[0][i] + e[1][i];
                     }
                 }
 #pragma unroll
