@@ -12,8 +12,8 @@ using namespace qx::ops;
 
 constexpr int kTreeThreads = 128, kTreeWarps = 4;
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // not volatile: products may be interleaved
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -579,9 +579,12 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_cons
                     const int first_b = max(b0, g * per_head), end_b = min(b1, (g + 1) * per_head);
                     for (int b = first_b; b < end_b; ++b) {
                         const uint8_t* block = dyn + (size_t)(b - b0) * Block::kBytes;
-                        float acc[2][4] = {};
+                        float part[HD / 64][2][4] = {}, acc[2][4];   // apart, for shorter chains of products
 #pragma unroll
-                        for (int c = 0; c < HD / 64; ++c) dot_block<HD, NT>(block, c, key[0] + 8 * c, key[1] + 8 * c, acc);
+                        for (int c = 0; c < HD / 64; ++c) dot_block<HD, NT>(block, c, key[0] + 8 * c, key[1] + 8 * c, part[c]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            acc[i >> 2][i & 3] = HD == 128 ? part[0][i >> 2][i & 3] + part[HD / 64 - 1][i >> 2][i & 3] : part[0][i >> 2][i & 3];
                         const int row0 = (b - g * per_head) * 16;
                         const float2* facs = reinterpret_cast<const float2*>(block + Block::kFacs);
                         float e[2][4];
