@@ -138,6 +138,17 @@ struct alignas(sizeof(T) * N) Pack {
     T v[N];
 };
 
+// Division by a number that the host knows.  (2^32 / d + 1) x / 2^32 is too
+// large by less than x / 2^32 < 1, so the quotient by one at most.
+struct Over {
+    uint32_t d, by;
+    Over(uint32_t d = 1) : d(d), by(d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+        const uint32_t q = d > 1 ? __umulhi(x, by) : x;
+        return q - (q * d > x);
+    }
+};
+
 // Where the rows of a sequence lie.
 struct Cache {
     int8_t *k, *v;

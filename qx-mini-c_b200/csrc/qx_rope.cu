@@ -28,14 +28,6 @@ struct Heads {
 // rotated pairs (half layout: V values at i and V at rd / 2 + i; interleaved:
 // 2 V consecutive values), then every head's `pass` items of V values that go
 // through, so that a warp mostly has items of one kind.
-struct Over {                                            // division by d: the product is at most one too high
-    uint32_t d, by;
-    __host__ __device__ __forceinline__ explicit Over(uint32_t d) : d(d), by(d > 1 ? (uint32_t)((1ull << 32) / d + 1) : 0) {}
-    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
-        const uint32_t q = d > 1 ? __umulhi(x, by) : x;
-        return q - (q * d > x);
-    }
-};
 struct Items {
     Over pairs, pass;
     int rotated;                                         // in all heads

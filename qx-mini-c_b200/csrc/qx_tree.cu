@@ -669,6 +669,7 @@ cudaError_t launch_small(TreeArgs& a, int sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     a.ctas = sms * (per < 1 ? 1 : per);
     if (a.ctas > most_ctas(16 * MT)) a.ctas = most_ctas(16 * MT);
+    a.per_cta = Over((uint32_t)a.ctas);
     kernel<<<a.ctas, kTreeThreads, kBytes, st>>>(a);
     return cudaGetLastError();
 }
@@ -746,6 +747,8 @@ QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer,
     a.group = (int)(q_heads / cache->kv_heads);
     a.block_rows = p.block_rows;
     a.row_blocks = p.row_blocks;
+    a.per_block = Over((uint32_t)p.block_rows);
+    a.per_heads = Over(cache->kv_heads);
     a.q = {q->data, (size_t)q->seq_stride, (size_t)q->node_stride, (size_t)q->head_stride};
     a.out = {out->data, (size_t)out->seq_stride, (size_t)out->node_stride, (size_t)out->head_stride};
     a.mask = (const unsigned long long*)mask;

@@ -62,6 +62,7 @@ struct TreeArgs {
     float* parts;                                         // [2 * ctas][block_rows][kPartHead + head_dim]
     Join* joins;                                          // [ctas]
     int ctas;
+    Over per_block, per_heads, per_cta;                   // division by block_rows, kv_heads, ctas
     uint32_t* status;
 };
 
@@ -91,7 +92,7 @@ __device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool repor
         return {0, 0};
     }
     if (n == 0) return {0, 0};
-    return {(len + n + kTile - 1) / kTile, a.c.kv_heads * ((n * a.group + a.block_rows - 1) / a.block_rows)};
+    return {(len + n + kTile - 1) / kTile, a.c.kv_heads * (int)a.per_block(n * a.group + a.block_rows - 1)};
 }
 
 // The tiles of all units laid end to end, cut into shares that differ by one
@@ -100,14 +101,14 @@ struct Shares {
     int busy, each, extra;
     __device__ __forceinline__ Shares(const TreeArgs& a, int total) {
         busy = min(a.ctas, total);
-        each = busy ? total / busy : 0;
-        extra = busy ? total - each * busy : 0;
+        each = total < a.ctas ? 1 : (int)a.per_cta(total);
+        extra = total < a.ctas ? 0 : total - each * busy;
     }
     __device__ __forceinline__ int begin(int c) const { return each * c + min(c, extra); }
     // the CTA that has tile t
     __device__ __forceinline__ int of(int t) const {
         const int longer = extra * (each + 1);
-        return t < longer ? t / (each + 1) : extra + (t - longer) / each;
+        return each == 1 && t >= longer ? extra + t - longer : t < longer ? t / (each + 1) : extra + (t - longer) / each;
     }
 };
 
@@ -193,8 +194,9 @@ static __device__ __noinline__ void list_pieces(const TreeArgs& a, PieceList& sh
                     Piece& p = sh.piece[at];
                     p.s = s;
                     p.len = a.d.lens[s], p.n = a.d.count(s);
-                    p.g = u % a.c.kv_heads;
-                    p.row0 = u / a.c.kv_heads * a.block_rows;
+                    const int block = (int)a.per_heads(u);
+                    p.g = u - block * a.c.kv_heads;
+                    p.row0 = block * a.block_rows;
                     p.have = min(a.block_rows, p.n * a.group - p.row0);
                     p.tile0 = max(begin, f) - f;
                     p.tile1 = min(k.tiles, end - f);

@@ -769,6 +769,7 @@ cudaError_t cache_maps(const Cache& c, Maps& m) {
 template <class T, int HD, int NT>
 cudaError_t run(TreeArgs& a, int sms, cudaStream_t st) {
     a.ctas = sms < kMaxCtas / 8 ? sms : kMaxCtas / 8;
+    a.per_cta = Over((uint32_t)a.ctas);
     Maps maps;
     cudaError_t e = cache_maps(a.c, maps);
     if (e != cudaSuccess) return e;
