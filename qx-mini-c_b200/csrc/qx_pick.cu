@@ -3,7 +3,7 @@
 //
 // A cluster of CTAs takes row after row; each CTA owns a slice of the
 // vocabulary (every eighth 64 tokens: frequent tokens lie together, and one CTA
-// with all of them held the others up, 131 us against 107 for 256 rows of
+// with all of them held the others up, 131 us against 113 for 256 rows of
 // 151936) and keeps one 32-bit word per token of it in shared memory: the
 // token's count in the history (low 20 bits) and the last bias entry that names
 // it, plus one (high 12 bits).  Every CTA reads the whole history and counts
@@ -18,7 +18,7 @@
 // loads do not overlap.
 //
 // 256 rows of 151936 F32 logits with a mask, 64 biases and histories of 4096
-// move 311 MB, 49 us at the memory's rate, and take 110 us, bound by
+// move 311 MB, 49 us at the memory's rate, and take 113 us, bound by
 // instructions: of each 128 tokens a warp looks at, three or four are in the
 // history, and each of the four lanes' words costs its branch.  Dearer were: a queue
 // of such tokens per warp, emptied 32 at a time (134 us: its scans), and a second
