@@ -282,6 +282,6 @@ QX_API int qx_cuda_kv_evict(const qx_cuda_kv_cache* cache, uint32_t seqs, const 
     if (e != cudaSuccess) return finish(e, err, n);
     const uint64_t slices = ((uint64_t)cache->kv_heads * cache->head_dim + 127) / 128;
     // slices of 32 bytes while those of 128 would leave SMs without two CTAs
-    const bool few = (uint64_t)seqs * cache->layers * 2 * slices < 2 * 148;
+    const bool few = seqs * (uint64_t)cache->layers * 2 * slices < 2 * 148;
     return finish(few ? launch_move<2>(a, st) : launch_move<8>(a, st), err, n);
 }

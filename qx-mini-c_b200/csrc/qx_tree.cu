@@ -747,7 +747,9 @@ QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer,
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < p.all())
         return refuse(err, n, "the workspace is missing, misaligned or too small");
     const uint64_t tiles = ((uint64_t)cache->ctx_tokens + kTile - 1) / kTile;
-    if ((uint64_t)drafts->seqs * cache->kv_heads * p.row_blocks * tiles > 0x7fffffffull)
+    // (what each row got is summed in steps of 16 rows)
+    if ((uint64_t)drafts->seqs * cache->kv_heads * p.row_blocks * tiles > 0x7fffffffull ||
+        (mass && drafts->seqs * tiles * (kTile / 16) > 0x7fffffffull))
         return refuse(err, n, "more rows and cache than one call can take");
     if (cache_rows(cache_of(cache)) > 0x7fffffffull - kTile) return refuse(err, n, "the cache has more rows than the operator supports");
     DeviceOf dev(cache->k, err, n);

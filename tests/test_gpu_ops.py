@@ -172,6 +172,46 @@ def test_rope_append_of_non_finite_and_zero_rows():
     assert c.v[0, 0, 0, 0, 3:7].tolist() == [0, 0, -127, 64] and c.v_scales[0, 0, 2] == 1 and not c.k[0, 0, :3].any()
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -6, 0.013, 1e-30, 3e-38, 7e-41, 3e30])
+def test_codes_of_values_next_to_a_half(scale):
+    """Quotients that are a half, or a few units of the last place from it, round like the definition's; whole rows of tiny,
+    denormal and huge scales too."""
+    halves = np.arange(-126, 127, dtype=np.float64) + 0.5
+    rows = [np.float32(127 * scale) * np.ones(256, np.float32) for _ in range(5)]
+    step = rows[0][0] / np.float32(127)
+    for i, row in enumerate(rows):
+        x = (halves * float(step)).astype(np.float32)
+        for _ in range(abs(i - 2)):
+            x = np.nextafter(x, np.float32(math.copysign(math.inf, i - 2)))
+        row[1:1 + len(x)] = x
+        assert np.abs(row).max() == row[0]
+    v = torch.from_numpy(np.stack(rows)).to(DEV).view(1, 5, 2, 128)
+    c = make_cache(gen(3), 1, 1, 8, 2, 128)
+    inv = torch.from_numpy(qxops.rope_frequencies(128)[0]).to(DEV)
+    # at position 0 keys turn by nothing, so both halves of the cache hold the same
+    qxops.rope_append(c, 0, ints([0]), ints([1]), None, v.clone(), v, inv, positions=ints([[0] * 5]))
+    codes, scales = codes_of(v.reshape(5, 256))
+    for got, s in ((c.k, c.k_scales), (c.v, c.v_scales)):
+        assert torch.equal(got[0, 0, 1:6].reshape(5, 256), codes) and torch.equal(s[0, 0, 1:6], scales)
+
+
+def test_rope_append_of_many_wide_heads():
+    """More items of each kind than threads, in heads that turn in part: 40 query and 24 KV heads of 136 values, 48 of them turned."""
+    g = gen(31)
+    c = make_cache(g, 2, 1, 9, 24, 136)
+    before = copies(c)
+    q, k, v = (torch.randn(2, 3, h, 136, generator=g, device=DEV).bfloat16() for h in (40, 24, 24))
+    inv = torch.from_numpy(qxops.rope_frequencies(48)[0]).to(DEV)
+    slots, lens, nodes = ints([1, 0]), ints([2, 6]), ints([3, 3])
+    for il in (False, True):
+        out = torch.zeros_like(q)
+        pos = ints([[5, 6, 900], [70000, 1, 0]])
+        for x, b in zip((c.k, c.v, c.k_scales, c.v_scales), before):
+            x.copy_(b)
+        qxops.rope_append(c, 0, slots, lens, q, k, v, inv, positions=pos, interleaved=il, q_out=out)
+        check_rope(c, before, 0, slots, lens, nodes, q, k, v, inv, pos, 1.0, 48, il, out, torch.zeros_like(q))
+
+
 def test_rope_append_leaves_out_what_does_not_fit():
     g = gen(8)
     c = make_cache(g, 3, 1, 6, 1, 64)
@@ -397,6 +437,57 @@ def test_tree_attention_leaves_out_what_does_not_fit(n):
     assert int(status) == qxops.STATUS_SHARED and not mass[0].any() and bool((mass[1, 0, :20] > 0).all())
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,hd", [(3, 64), (4, 128)])
+def test_poison_in_trees_of_seventeen_to_thirty_two_rows(kind, n, hd):
+    g = gen(19)
+    c = make_cache(g, 2, 1, 96, 2, hd)
+    q = torch.randn(2, n, 16, hd, generator=g, device=DEV).to(TYPES[kind])
+    mask = torch.zeros(2, n, 1, dtype=torch.int64, device=DEV)
+    mask[0, 0, 0] = 1                                           # sequence 0, empty cache: node 0 sees itself, the others nothing
+    mask[1, :, 0] = 1
+    c.k_scales[0, 0, 1:], c.v_scales[0, 0, 1:] = math.nan, math.inf
+    c.k_scales[1, 0, 41:], c.v_scales[1, 0, 41:] = math.inf, math.nan
+    out, lse, _ = check_tree(c, 0, ints([0, 1]), ints([0, 40]), None, q, mask, 0.2)
+    assert bool((out[0, 1:] == 0).all()) and bool((lse[0, 1:] == -math.inf).all())
+    mask[1, 1, 0] = 3                                           # now node 1 sees the poisoned row 41
+    again = qxops.tree_attention(c, 0, ints([0, 1]), ints([0, 40]), q, mask=mask, scale=0.2)
+    assert bool(torch.isnan(again[1, 1]).all())
+    keep = [i for i in range(n) if i != 1]
+    assert torch.equal(again[1, keep], out[1, keep]) and torch.equal(again[0], out[0])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("heads,hd,n", [((12, 3), 128, 97), ((12, 3), 64, 150), ((24, 8), 128, 5)])
+def test_mass_of_more_queries_than_one_pass_holds(kind, heads, hd, n):
+    """Query blocks that are held in several passes, cut inside a KV head and between heads; lengths that end inside a step."""
+    g = gen(n)
+    qh, kvh = heads
+    c = make_cache(g, 4, 1, 400, kvh, hd)
+    q = torch.randn(4, n, qh, hd, generator=g, device=DEV).to(TYPES[kind])
+    check_tree(c, 0, ints([2, 0, 3, 1]), ints([200, 0, 17, 400 - n]), ints([n, n, 0, n - 1]), q, random_tree(4, n, 5), hd ** -0.5)
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call has scratch of its own: the bits are those of the calls alone."""
+    g = gen(23)
+    c = make_cache(g, 6, 1, 3000, 2, 128)
+    slots, lens = ints([0, 1, 2, 3, 4, 5]), ints([2900, 1500, 7, 0, 2000, 100])
+    qs = [torch.randn(6, n, 16, 128, generator=g, device=DEV).bfloat16() for n in (1, 3, 12)]
+    want = [(qxops.tree_attention(c, 0, slots, lens, q, mass=m), m) for q in qs for m in [torch.zeros_like(c.k_scales)]]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                m = torch.zeros_like(c.k_scales)
+                got.append((qxops.tree_attention(c, 0, slots, lens, q, mass=m), m))
+    torch.cuda.synchronize()
+    for i, (out, m) in enumerate(got):
+        assert torch.equal(out, want[i % 3][0]) and torch.equal(m, want[i % 3][1]), i
+
+
 def test_the_same_call_gives_the_same_bits():
     g = gen(13)
     c = make_cache(g, 8, 1, 1000, 4, 128)
@@ -457,6 +548,23 @@ def test_evict(in_place, kvh, hd, budget, sink, recent):
     assert int(status) == 0
     assert torch.equal(kept.cpu(), want[2]) and torch.equal(new.cpu(), want[3])
     assert torch.equal(mass.cpu(), want[1])
+    for got, e, what in zip((c.k, c.v, c.k_scales, c.v_scales), want[0], ("k", "v", "k scales", "v scales")):
+        assert torch.equal(got.cpu(), e), what
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("kvh,hd", [(4, 128), (2, 136), (1, 16)])
+def test_evict_of_many_layers(in_place, kvh, hd):
+    """Enough sequences and layers for the wide slices, and rows that end inside one."""
+    g = gen(kvh)
+    layers, ctx, seqs = 48, 150, 4
+    c = make_cache(g, 2 * seqs, layers, ctx, kvh, hd)
+    mass = torch.rand(c.k_scales.shape, generator=g, device=DEV)
+    slots, lens = [0, 3, 1, 2], [150, 140, 90, 31]
+    dst = slots if in_place else [4, 5, 6, 7]
+    want = evicted(copies(c), mass, slots, dst, lens, 70, 2, 8)
+    kept, new = qxops.evict(c, ints(slots), ints(lens), mass, 70, 2, 8, dst_slots=None if in_place else ints(dst))
+    assert torch.equal(kept.cpu(), want[2]) and torch.equal(new.cpu(), want[3]) and torch.equal(mass.cpu(), want[1])
     for got, e, what in zip((c.k, c.v, c.k_scales, c.v_scales), want[0], ("k", "v", "k scales", "v scales")):
         assert torch.equal(got.cpu(), e), what
 

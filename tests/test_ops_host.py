@@ -106,6 +106,15 @@ def test_tree_attention_refusals(args, message):
     assert tree(**args) == (0, message)
 
 
+def test_tree_attention_refuses_more_steps_than_it_counts():
+    """4096 sequences of 2^24 rows: 2^30 tiles of 64 rows, but 2^32 steps of 16 for the mass."""
+    wide = cache(slots=1, layers=1, ctx_tokens=1 << 24, kv_heads=1, slot_rows=1 << 24, layer_rows=1 << 24)
+    d, q = drafts(seqs=4096, max_nodes=1), heads(seq=64, node=64)
+    args = dict(c=wide, d=d, qh=1, q=q, out=q)
+    assert tree(mass=BASE, **args) == (0, "more rows and cache than one call can take")
+    assert tree(**args)[1] != "more rows and cache than one call can take"      # refused later, for its made-up addresses
+
+
 def evict(c=None, seqs=2, slots=BASE, dst=None, lens=BASE, mass=BASE, budget=8, sink=2, recent=2, kept=BASE, new=BASE + 64,
           status=None):
     return said(opsabi.lib().qx_cuda_kv_evict, C.byref(c or cache()), seqs, slots, dst, lens, mass, budget, sink, recent, kept,
