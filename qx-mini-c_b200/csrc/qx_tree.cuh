@@ -82,17 +82,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // A sequence's share of the work: `units` units of `tiles` tiles each.  (The
 // host refuses calls whose tiles could pass 2^31.)
 struct SeqWork {
-    int tiles, units;
+    int tiles, units, slot, len, n;
     __device__ __forceinline__ int all() const { return tiles * units; }
 };
 __device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool report) {
     const int slot = a.d.slots[s], len = a.d.lens[s], n = a.d.count(s);
     if (!fits(a.c, a.d, slot, len, n)) {
         if (report && a.status) atomicOr(a.status, QX_CUDA_STATUS_RANGE);
-        return {0, 0};
+        return {};
     }
-    if (n == 0) return {0, 0};
-    return {(len + n + kTile - 1) / kTile, a.c.kv_heads * (int)a.per_block(n * a.group + a.block_rows - 1)};
+    if (n == 0) return {};
+    return {(len + n + kTile - 1) / kTile, a.c.kv_heads * (int)a.per_block(n * a.group + a.block_rows - 1), slot, len, n};
 }
 
 // The tiles of all units laid end to end, cut into shares that differ by one
@@ -137,7 +137,7 @@ static __device__ __noinline__ void list_pieces(const TreeArgs& a, PieceList& sh
     const bool scans = threadIdx.x < kScanThreads;
     const int s0 = scans ? min(a.d.seqs, (int)threadIdx.x * per) : 0, s1 = scans ? min(a.d.seqs, s0 + per) : 0;
     int tiles = 0, units = 0;
-    SeqWork one{0, 0};                                    // kept where a thread has one sequence
+    SeqWork one{};                                        // kept where a thread has one sequence
     for (int s = s0; s < s1; ++s) {
         one = seq_work(a, s, blockIdx.x == 0 && batch == 0);
         tiles += one.all();
@@ -193,7 +193,7 @@ static __device__ __noinline__ void list_pieces(const TreeArgs& a, PieceList& sh
                     const int f = first + u * k.tiles;
                     Piece& p = sh.piece[at];
                     p.s = s;
-                    p.len = a.d.lens[s], p.n = a.d.count(s);
+                    p.len = k.len, p.n = k.n;
                     const int block = (int)a.per_heads(u);
                     p.g = u - block * a.c.kv_heads;
                     p.row0 = block * a.block_rows;
@@ -202,7 +202,7 @@ static __device__ __noinline__ void list_pieces(const TreeArgs& a, PieceList& sh
                     p.tile1 = min(k.tiles, end - f);
                     p.begins = p.tile0 == 0;
                     p.whole = p.begins && p.tile1 == k.tiles;
-                    p.base_row = (size_t)a.d.slots[s] * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
+                    p.base_row = (size_t)k.slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows;
                     // of the CTAs that share a unit, the second sees to its joining
                     if (at == 0 && batch == 0 && !p.begins && cut.begin(c - 1) <= f)
                         a.joins[c] = {cut.of(f + k.tiles - 1) - c + 2, s, p.g, p.row0, p.have};
@@ -263,13 +263,16 @@ struct RowScale {
     int up;
     float f0, f1;
     __device__ __forceinline__ explicit RowScale(float big) {
-        up = 13 - (big > 0.f ? ilogbf(big) : 0);
+        const int b = __float_as_int(big);
+        const int e = b < 0x00800000 ? b ? 31 - __clz(b) - 149 : 0 : (b >> 23) - 127;
+        up = 13 - e;
         const int u0 = up / 2;
-        f0 = __uint_as_float((uint32_t)(127 + u0) << 23);
-        f1 = __uint_as_float((uint32_t)(127 + up - u0) << 23);
+        f0 = pow2(u0);
+        f1 = pow2(up - u0);
     }
+    __device__ __forceinline__ static float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
     // what turns the integer dot product of scaled queries and codes into a base-2 score, but for ks_t
-    __device__ __forceinline__ float undo(float scale) const { return ldexpf(scale * kLog2e, -up); }
+    __device__ __forceinline__ float undo(float scale) const { return scale * kLog2e * pow2(-(up / 2)) * pow2(up / 2 - up); }
 };
 
 // log2(vs) for the exponent, and 1 / vs for the sum of weights.
