@@ -400,73 +400,161 @@ __global__ void __launch_bounds__(kTreeThreads, MT == 1 ? 3 : 2) k_tree_small(co
     }
 }
 
-// Adds the parts of the units that several CTAs worked on, by the records
-// they left.  grid: (CTA of the kernel before, R of the unit's rows); G groups
-// of threads take a share of the parts each (many for the small kernel's units,
-// which can be spread over hundreds of CTAs; one for those of 128 rows), and are added in order.
-constexpr int kJoinThreads = 256;
-template <class T, int HD, int R>
-__global__ void __launch_bounds__(kJoinThreads) k_tree_join(const __grid_constant__ TreeArgs a) {
-    constexpr int kLanes = HD / 4, G = kJoinThreads / (R * kLanes), kPer = kJoinThreads / R, kMost = R == 8 ? kMaxCtas / 8 : kMaxCtas;
-    __shared__ float weight[R][kMost], red[2][kJoinThreads / 32], tops[R];
-    __shared__ float4 shares[G][R][kLanes];
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the kernel before still runs
-    const Join j = a.joins[blockIdx.x];
-    const int row0 = blockIdx.y * R, tid = threadIdx.x;
-    if (row0 >= (j.parts ? j.have : 0)) return;
-    // the first part begins the unit, the others are what their CTAs began with
-    const size_t row_floats = kPartHead + HD, step = 2 * (size_t)a.block_rows * row_floats;
-    const float* parts = part_of(a, blockIdx.x - 1, false);
-    auto part = [&](int i, int row) { return parts + i * step + (i == 0 ? step / 2 : 0) + row * row_floats; };
-    // the parts' factors: kPer threads (whole warps) to a row
-    const int wr = tid / kPer, wi = tid % kPer, wrow = min(row0 + wr, j.have - 1);
-    float mx = -INFINITY, sum = 0.f;
-    for (int i = wi; i < j.parts; i += kPer) mx = fmaxf(mx, part(i, wrow)[0]);
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
-    if (kPer > 32) {
-        if ((tid & 31) == 0) red[0][tid >> 5] = mx;
-        __syncthreads();
-        for (int i = 0; i < kPer / 32; ++i) mx = fmaxf(mx, red[0][wr * (kPer / 32) + i]);
+// Adds the parts of the units that several CTAs worked on, by the records they
+// left.  A unit of few parts is joined by a warp a row, one of many by a CTA a
+// row, whose warps take every eighth part: items of eight rows or one, counted
+// from the records by every CTA for itself.  A row's first parts are asked for before
+// their factors are known.  What it adds to a call: 9 us for 64 x 16 nodes over 4096 rows (147
+// units of two or three parts, 20 MB), 7 us for 13 nodes over 32768 rows (4 units of 37 parts).  A CTA for each
+// record and eight rows, most of them with nothing to do, added 10 and 15 us.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kFewParts = 8, kJoinAhead = 4, kJoinList = 64;
+struct JoinItem {
+    Join j;
+    int c, local;                                          // the record, and the item among its own
+};
+template <class T, int HD>
+__global__ void __launch_bounds__(kJoinThreads, 4) k_tree_join(const __grid_constant__ TreeArgs a) {
+    constexpr int kLanes = HD / 4, S = 32 / kLanes;        // lanes of a part's row, parts a warp reads at a time
+    __shared__ int warp_sum[kJoinWarps];
+    __shared__ JoinItem list[kJoinList];
+    __shared__ float4 shares[kJoinWarps][kLanes];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / kLanes, d = lane % kLanes;
+    asm volatile("griddepcontrol.wait;" ::: "memory");     // launched while the kernel before still runs
+    const int per = (a.ctas + kJoinThreads - 1) / kJoinThreads, c0 = min(a.ctas, tid * per), c1 = min(a.ctas, c0 + per);
+    auto items_of = [&](const Join& j) { return j.parts == 0 ? 0 : j.parts <= kFewParts ? (j.have + kJoinWarps - 1) / kJoinWarps : j.have; };
+    Join one{};                                            // kept where a thread has one record
+    int mine = 0;
+    for (int c = c0; c < c1; ++c) {
+        one = a.joins[c];
+        mine += items_of(one);
     }
-    for (int i = wi; i < j.parts; i += kPer) {
-        const float2 ml = *reinterpret_cast<const float2*>(part(i, wrow));
-        const float f = part_weight(ml.x, ml.y, mx);
-        weight[wr][i] = f;
-        sum = fmaf(f, ml.y, sum);
-    }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if ((tid & 31) == 0) red[1][tid >> 5] = sum;
-    if (wi == 0) tops[wr] = mx;
-    __syncthreads();
-    const int d = tid % kLanes, r = tid / kLanes % R, g = tid / (kLanes * R), row = row0 + r;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < j.have) {
-        const int each = (j.parts + G - 1) / G, first = g * each, end = min(j.parts, first + each);
-#pragma unroll 8
-        for (int i = first; i < end; ++i) {
-            const float4 v = *reinterpret_cast<const float4*>(part(i, row) + kPartHead + 4 * d);
-            const float f = weight[r][i];
-            y = make_float4(fmaf(f, v.x, y.x), fmaf(f, v.y, y.y), fmaf(f, v.z, y.z), fmaf(f, v.w, y.w));
-        }
-    }
-    if (G > 1) {
-        shares[g][r][d] = y;
-        __syncthreads();
-    }
-    if (g || row >= j.have) return;
-    for (int i = 1; i < G; ++i) {
-        const float4 z = shares[i][r][d];
-        y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
-    }
-    sum = 0.f;
-    for (int i = 0; i < kPer / 32; ++i) sum += red[1][r * (kPer / 32) + i];
-    const float by = sum == 0.f ? 0.f : 1.f / sum;
-    const int nd = (j.row0 + row) / a.group, h = j.g * a.group + (j.row0 + row) % a.group;
-    T* dst = (T*)a.out.p + j.s * a.out.seq + nd * a.out.node + h * a.out.head + 4 * d;
-    const float out[4] = {y.x * by, y.y * by, y.z * by, y.w * by};
+    int upto = mine;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dst[e] = from_f32<T>(sum == 0.f ? 0.f : out[e]);
-    if (d == 0) write_lse(a, j.s, nd, h, tops[r], sum);
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += t;
+    }
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        if (w < warp) upto += warp_sum[w];
+        total += warp_sum[w];
+    }
+    const int row_floats = kPartHead + HD, step = 2 * a.block_rows * row_floats;   // all parts are below 2^24 floats
+    const int each = (total + gridDim.x - 1) / gridDim.x, end = min(total, (int)(blockIdx.x + 1) * each);
+    for (int i0 = blockIdx.x * each; i0 < end; i0 += kJoinList) {
+        const int i1 = min(end, i0 + kJoinList);
+        int b = upto - mine;
+        if (b < i1 && upto > i0)
+            for (int c = c0; c < c1; ++c) {
+                const Join j = per == 1 ? one : a.joins[c];
+                const int n = items_of(j);
+                for (int i = max(b, i0); i < min(b + n, i1); ++i) list[i - i0] = {j, c, i - b};
+                b += n;
+            }
+        __syncthreads();
+        for (int item = 0; item < i1 - i0; ++item) {
+            const Join& j = list[item].j;
+            const int parts_n = j.parts, local = list[item].local;
+            const bool few = parts_n <= kFewParts;
+            const int row = few ? local * kJoinWarps + warp : local;
+            if (row >= j.have) continue;                   // (never in part of a CTA that joins a row together)
+            // the first part begins the unit, the others are what their CTAs began with
+            const float* parts = part_of(a, list[item].c - 1, false) + row * row_floats;
+            auto part = [&](int i) { return parts + max(i * step, step / 2); };
+            float4 v[kJoinAhead], y = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto add = [&](float f, const float4& x) {
+                y = make_float4(fmaf(f, x.x, y.x), fmaf(f, x.y, y.y), fmaf(f, x.z, y.z), fmaf(f, x.w, y.w));
+            };
+            float mx, sum;
+            if (few) {
+                // lanes i, i + 8, .. have part i's factor
+#pragma unroll
+                for (int u = 0; u < kJoinAhead; ++u)
+                    if (u * S < parts_n) v[u] = *reinterpret_cast<const float4*>(part(min(u * S + sub, parts_n - 1)) + kPartHead + 4 * d);
+                const int mine = lane & (kFewParts - 1);
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (mine < parts_n) ml = *reinterpret_cast<const float2*>(part(mine));
+                mx = ml.x;
+#pragma unroll
+                for (int o = kFewParts / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+                const float f = part_weight(ml.x, ml.y, mx);
+                sum = f * ml.y;
+#pragma unroll
+                for (int o = kFewParts / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+#pragma unroll
+                for (int u = 0; u < kFewParts / S; ++u)
+                    if (u * S < parts_n) {
+                        const float fu = __shfl_sync(~0u, f, u * S + sub);
+                        if (u >= kJoinAhead) v[u % kJoinAhead] = *reinterpret_cast<const float4*>(part(min(u * S + sub, parts_n - 1)) + kPartHead + 4 * d);
+                        if (u * S + sub < parts_n) add(fu, v[u % kJoinAhead]);
+                    }
+            } else {
+                const int first = warp * S + sub, by = kJoinWarps * S;
+#pragma unroll
+                for (int u = 0; u < kJoinAhead; ++u)
+                    if (first + u * by < parts_n) v[u] = *reinterpret_cast<const float4*>(part(first + u * by) + kPartHead + 4 * d);
+                mx = -INFINITY, sum = 0.f;
+                for (int i = lane; i < parts_n; i += 32) mx = fmaxf(mx, part(i)[0]);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+                for (int i = lane; i < parts_n; i += 32) {
+                    const float2 ml = *reinterpret_cast<const float2*>(part(i));
+                    sum = fmaf(part_weight(ml.x, ml.y, mx), ml.y, sum);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+                for (int i = first; i < parts_n; i += kJoinAhead * by) {
+                    if (i != first)
+#pragma unroll
+                        for (int u = 0; u < kJoinAhead; ++u)
+                            if (i + u * by < parts_n) v[u] = *reinterpret_cast<const float4*>(part(i + u * by) + kPartHead + 4 * d);
+#pragma unroll
+                    for (int u = 0; u < kJoinAhead; ++u)
+                        if (i + u * by < parts_n) {
+                            const float2 ml = *reinterpret_cast<const float2*>(part(i + u * by));
+                            add(part_weight(ml.x, ml.y, mx), v[u]);
+                        }
+                }
+            }
+            if (S == 2) {
+                __syncwarp();
+                y.x += __shfl_xor_sync(~0u, y.x, 16), y.y += __shfl_xor_sync(~0u, y.y, 16);
+                y.z += __shfl_xor_sync(~0u, y.z, 16), y.w += __shfl_xor_sync(~0u, y.w, 16);
+            }
+            if (!few) {
+                if (sub == 0) shares[warp][d] = y;
+                __syncthreads();
+                if (warp == 0) {
+#pragma unroll
+                    for (int w = 1; w < kJoinWarps; ++w) {
+                        const float4 z = shares[w][d];
+                        y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+                    }
+                }
+                __syncthreads();                               // the next item's shares may go over these
+                if (warp) continue;
+            }
+            if (sub) continue;
+            const float scale = sum == 0.f ? 0.f : 1.f / sum;
+            const int nd = (int)a.per_group(j.row0 + row), h = j.g * a.group + (j.row0 + row) - nd * a.group;
+            T* dst = (T*)a.out.p + j.s * a.out.seq + nd * a.out.node + h * a.out.head + 4 * d;
+            const float out[4] = {y.x * scale, y.y * scale, y.z * scale, y.w * scale};
+            Pack<T, 4> z;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z.v[e] = from_f32<T>(sum == 0.f ? 0.f : out[e]);
+            if (a.wide) {
+                *reinterpret_cast<Pack<T, 4>*>(dst) = z;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dst[e] = z.v[e];
+            }
+            if (d == 0) write_lse(a, j.s, nd, h, mx, sum);
+        }
+        __syncthreads();                                   // the list has been read
+    }
 }
 
 // ---- what each cache row got ---------------------------------------------------
@@ -693,7 +781,7 @@ cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t
                                          : launch_small<T, HD, NT, 2>(a, sms, st);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)(a.block_rows / (tc ? 8 : 2)));
+    cfg.gridDim = dim3((unsigned)sms * 4);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at{};
@@ -701,7 +789,7 @@ cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = tc ? cudaLaunchKernelEx(&cfg, k_tree_join<T, HD, 8>, a) : cudaLaunchKernelEx(&cfg, k_tree_join<T, HD, 2>, a);
+    e = cudaLaunchKernelEx(&cfg, k_tree_join<T, HD>, a);
     if (e != cudaSuccess || !a.mass) return e;
     constexpr int kHeld = Held<HD, NT>::kMost * Held<HD, NT>::kBytes;
     e = cudaFuncSetAttribute((const void*)k_tree_mass<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld);
@@ -764,6 +852,7 @@ QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer,
     a.row_blocks = p.row_blocks;
     a.per_block = Over((uint32_t)p.block_rows);
     a.per_heads = Over(cache->kv_heads);
+    a.per_group = Over((uint32_t)a.group);
     a.q = {q->data, (size_t)q->seq_stride, (size_t)q->node_stride, (size_t)q->head_stride};
     a.out = {out->data, (size_t)out->seq_stride, (size_t)out->node_stride, (size_t)out->head_stride};
     a.mask = (const unsigned long long*)mask;

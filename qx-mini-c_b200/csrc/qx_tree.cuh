@@ -62,7 +62,7 @@ struct TreeArgs {
     float* parts;                                         // [2 * ctas][block_rows][kPartHead + head_dim]
     Join* joins;                                          // [ctas]
     int ctas;
-    Over per_block, per_heads, per_cta;                   // division by block_rows, kv_heads, ctas
+    Over per_block, per_heads, per_group, per_cta;        // division by block_rows, kv_heads, group, ctas
     uint32_t* status;
 };
 
