@@ -242,45 +242,63 @@ __device__ __noinline__ void stage_queries(const TreeArgs& a, const Piece& p, in
     constexpr int V = 16 / sizeof(T), kSteps = HD / 32, kPacks = 8 / V;
     const int lane = threadIdx.x & 31, r8 = lane & 7, c4 = lane >> 3, row = row0 + r8, r = p.row0 + row;
     const bool real = row < p.have;
-    const T* src = (const T*)a.q.p + p.s * a.q.seq + (real ? r / a.group : 0) * a.q.node +
-                   (size_t)(p.g * a.group + (real ? r % a.group : 0)) * a.q.head + c4 * 8;
-    Pack<T, V> x[kSteps][kPacks];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-        for (int k = 0; k < kPacks; ++k) {
-#pragma unroll
-            for (int u = 0; u < V; ++u) x[i][k].v[u] = from_f32<T>(0.f);
-            if (real && a.wide) x[i][k] = *reinterpret_cast<const Pack<T, V>*>(src + 32 * i + V * k);
-        }
-    if (real && !a.wide)
+    const int node = real ? (int)a.per_group(r) : 0;
+    const T* src = (const T*)a.q.p + p.s * a.q.seq + node * a.q.node +
+                   (size_t)(p.g * a.group + (real ? r - node * a.group : 0)) * a.q.head + c4 * 8;
+    float big = 0.f;
+    auto largest = [&](T v) {
+        const float y = fabsf(to_f32(v));
+        big = fmaxf(big, y <= 3.402823466e38f ? y : 0.f);
+    };
+    Pack<T, V> all[kSteps][kPacks] = {};
+    if (real && a.wide) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e / V].v[e % V] = src[32 * i + e];
-    float big = 0.f;
+            for (int k = 0; k < kPacks; ++k) all[i][k] = *reinterpret_cast<const Pack<T, V>*>(src + 32 * i + V * k);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float y = fabsf(to_f32(x[i][e / V].v[e % V]));
-            big = fmaxf(big, y <= 3.402823466e38f ? y : 0.f);
-        }
+            for (int e = 0; e < 8; ++e) largest(all[i][e / V].v[e % V]);
+    } else if (real) {
+#pragma unroll 1
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) largest(src[32 * i + e]);
+    }
     big = fmaxf(big, __shfl_xor_sync(~0u, big, 8));
     big = fmaxf(big, __shfl_xor_sync(~0u, big, 16));
     const RowScale rs(big);
     uint8_t* to = qt + (row >> 3) * (HD / 8 * 128) + r8 * 16 + c4 * 128;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
+    auto store = [&](int i, const Pack<T, V> (&x)[kPacks]) {
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = to_f32(x[i][e / V].v[e % V]) * rs.f0 * rs.f1;
+        for (int e = 0; e < 8; ++e) y[e] = to_f32(x[e / V].v[e % V]) * rs.f0 * rs.f1;
         const uint4 hi = make_uint4(pack_half(y[0], y[1]), pack_half(y[2], y[3]), pack_half(y[4], y[5]), pack_half(y[6], y[7]));
         *reinterpret_cast<uint4*>(to + i * 512) = hi;
         if (NT == 2)
             *reinterpret_cast<uint4*>(to + Shape<HD, NT>::kQBytes + i * 512) =
                 make_uint4(rest_half(y[0], y[1], hi.x), rest_half(y[2], y[3], hi.y), rest_half(y[4], y[5], hi.z),
                            rest_half(y[6], y[7], hi.w));
+    };
+    // Queries of two bytes are read a second time, from L1, in a loop that is a quarter of the code to fetch (64 x 16
+    // nodes 154 -> 151 us); F32 ones would not all be there still (174 -> 181 us).
+    if (NT == 2 && (a.wide || !real)) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) store(i, all[i]);
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < kSteps; ++i) {
+            Pack<T, V> x[kPacks] = {};
+            if (real && a.wide) {
+#pragma unroll
+                for (int k = 0; k < kPacks; ++k) x[k] = *reinterpret_cast<const Pack<T, V>*>(src + 32 * i + V * k);
+            } else if (real) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e / V].v[e % V] = src[32 * i + e];
+            }
+            store(i, x);
+        }
     }
     if (c4 == 0) fac[row] = rs.undo(a.scale);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
