@@ -38,7 +38,6 @@ namespace {
 using namespace qx::ops;
 namespace cg = cooperative_groups;
 
-constexpr int kPickCluster = 8;                        // CTAs a row
 constexpr uint32_t kMaxVocab = 393216, kCountBits = 20, kCountMask = (1u << kCountBits) - 1;
 
 struct PickArgs {
@@ -73,10 +72,11 @@ __device__ __forceinline__ int clamped(const int* lens, int r, int most) {
     return lens ? max(0, min(lens[r], most)) : most;
 }
 
-// Place p is word p / 512 * 64 + p % 64 of the CTA p / 64 % 8 of the cluster.
-constexpr int kChunk = 64, kRound = kChunk * kPickCluster;
+// Of a cluster of CL CTAs, place p is word p / (64 CL) * 64 + p % 64 of CTA p / 64 % CL.
+constexpr int kChunk = 64;
+template <int CL>
 __device__ __forceinline__ int place_of(int word, int rank) {
-    return word / kChunk * kRound + rank * kChunk + word % kChunk;
+    return word / kChunk * (kChunk * CL) + rank * kChunk + word % kChunk;
 }
 
 // A row's addresses, and where its tokens are.
@@ -106,13 +106,16 @@ struct Row {
     }
 };
 
-template <class T, int THREADS>
+// Words of a CTA: of vocab and up to 7 places before it.
+inline int slice_of(int vocab, int ctas) { return (vocab + 7 + kChunk * ctas - 1) / (kChunk * ctas) * kChunk; }
+
+template <class T, int THREADS, int CL>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_constant__ PickArgs a) {
-    constexpr int V = 16 / sizeof(T), kAhead = V == 4 ? 4 : 2;         // packs a thread has in flight
+    constexpr int V = 16 / sizeof(T), kAhead = V == 4 ? 3 : 1, kRound = kChunk * CL;   // kAhead: packs a thread has in flight
     extern __shared__ __align__(16) uint32_t words[];
-    __shared__ Best wbest[THREADS / 32], row_best[2][kPickCluster];     // row_best: in the cluster's first CTA
+    __shared__ Best wbest[THREADS / 32], row_best[2][CL];     // row_best: in the cluster's first CTA
     cg::cluster_group cl = cg::this_cluster();
-    const int rank = (int)cl.block_rank(), step = gridDim.x / kPickCluster, tid = threadIdx.x;
+    const int rank = (int)cl.block_rank(), step = gridDim.x / CL, tid = threadIdx.x;
     const bool touched = a.history || a.bias_ids;
     if (touched) {
         for (int i = tid * 4; i < a.slice; i += THREADS * 4) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
     auto join = [&](int r, int slot) {
         if (rank || tid) return;
         Best best = row_best[slot][0];
-        for (int c = 1; c < kPickCluster; ++c) {
+        for (int c = 1; c < CL; ++c) {
             better(best, row_best[slot][c].v, row_best[slot][c].i);
             best.bad |= row_best[slot][c].bad;
         }
@@ -130,9 +133,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
     };
     Pack<T, V> pack[kAhead];
     uint32_t bits[kAhead];
-    const int first = blockIdx.x / kPickCluster;
+    const int first = blockIdx.x / CL;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) Row<T>(a, first).load(place_of((i * THREADS + tid) * V, rank), pack[i], bits[i]);
+    for (int i = 0; i < kAhead; ++i) Row<T>(a, first).load(place_of<CL>((i * THREADS + tid) * V, rank), pack[i], bits[i]);
     int slot = 0;
     for (int r = first; r < a.rows; r += step, slot ^= 1) {
         const Row<T> row(a, r);
@@ -143,7 +146,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
             // the word of a token, if it is this CTA's
             auto word = [&](int id) -> uint32_t* {
                 const int p = id + shift;
-                return (unsigned)id < (unsigned)a.vocab && (p / kChunk) % kPickCluster == rank ? words + p / kRound * kChunk + p % kChunk
+                return (unsigned)id < (unsigned)a.vocab && (p / kChunk) % CL == rank ? words + p / kRound * kChunk + p % kChunk
                                                                                              : nullptr;
             };
             if (a.bias_ids) {
@@ -188,10 +191,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
             if (b) v = __fadd_rn(v, a.bias_values[r * a.bias_stride + b - 1]);
             return v;
         };
-        for (int w0 = tid * V; place_of(w0, rank) < row.end; w0 += kAhead * THREADS * V) {
+        for (int w0 = tid * V; place_of<CL>(w0, rank) < row.end; w0 += kAhead * THREADS * V) {
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int at = w0 + i * THREADS * V, p = place_of(at, rank), t = p - shift, later = place_of(at + kAhead * THREADS * V, rank);
+                const int at = w0 + i * THREADS * V, p = place_of<CL>(at, rank), t = p - shift, later = place_of<CL>(at + kAhead * THREADS * V, rank);
                 if (row.whole(p)) {
                     float v[V];
 #pragma unroll
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
         if (r + step < a.rows) {                                         // the next row's first packs
             const Row<T> next(a, r + step);
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) next.load(place_of((i * THREADS + tid) * V, rank), pack[i], bits[i]);
+            for (int i = 0; i < kAhead; ++i) next.load(place_of<CL>((i * THREADS + tid) * V, rank), pack[i], bits[i]);
         }
         for (int s = 16; s; s >>= 1) {
             const float v = __shfl_xor_sync(~0u, best.v, s);
@@ -284,10 +287,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
     join(first + (rows - 1) * step, slot ^ 1);
 }
 
-template <class T, int THREADS>
-cudaError_t launch_pick(const PickArgs& a, cudaStream_t st) {
+template <class T, int THREADS, int CL>
+cudaError_t launch_pick(PickArgs a, cudaStream_t st) {
+    a.slice = slice_of(a.vocab, CL);
     const size_t sm = a.history || a.bias_ids ? (size_t)a.slice * 4 : 0;
-    cudaError_t e = cudaFuncSetAttribute((const void*)k_pick<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    cudaError_t e = cudaFuncSetAttribute((const void*)k_pick<T, THREADS, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(THREADS);
@@ -295,20 +299,30 @@ cudaError_t launch_pick(const PickArgs& a, cudaStream_t st) {
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = kPickCluster;
+    at.val.clusterDim.x = CL;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
     int clusters = 1;
     if (a.rows > 1) {
-        cfg.gridDim = dim3((unsigned)(a.rows * kPickCluster));
-        e = cudaOccupancyMaxActiveClusters(&clusters, k_pick<T, THREADS>, &cfg);
+        cfg.gridDim = dim3((unsigned)(a.rows * CL));
+        e = cudaOccupancyMaxActiveClusters(&clusters, k_pick<T, THREADS, CL>, &cfg);
         if (e != cudaSuccess) return e;
         if (clusters < 1) clusters = 1;
         if (clusters > a.rows) clusters = a.rows;
     }
-    cfg.gridDim = dim3((unsigned)(clusters * kPickCluster));
-    return cudaLaunchKernelEx(&cfg, k_pick<T, THREADS>, a);
+    cfg.gridDim = dim3((unsigned)(clusters * CL));
+    return cudaLaunchKernelEx(&cfg, k_pick<T, THREADS, CL>, a);
+}
+
+template <class T>
+cudaError_t run_pick(const PickArgs& a, cudaStream_t st) {
+    // Few rows leave SMs to spare: one CTA of 1024 threads each.  Else two of 512 (rows of 50257, 64 of them: XX).
+    if (a.rows * 8 <= 148) return launch_pick<T, 1024, 8>(a, st);
+    // More rows than there are clusters of eight: clusters of four read the histories half as often, if two of their
+    // larger slices fit an SM.
+    if (a.rows * 8 > 2 * 148 && slice_of(a.vocab, 4) * 4 <= 100 * 1024) return launch_pick<T, 512, 4>(a, st);
+    return launch_pick<T, 512, 8>(a, st);
 }
 
 }  // namespace
@@ -345,7 +359,6 @@ QX_API int qx_cuda_pick_tokens(const qx_cuda_pick* p, void* stream, char* err, u
     a.out_stride = p->out_stride;
     a.rows = (int)p->rows;
     a.vocab = (int)p->vocab;
-    a.slice = (int)((p->vocab + 7 + kRound - 1) / kRound * kChunk);      // of vocab and up to 7 places before it
     a.max_history = (int)p->max_history;
     a.max_bias = (int)p->max_bias;
     a.history = p->max_history ? p->history : nullptr;
@@ -362,11 +375,9 @@ QX_API int qx_cuda_pick_tokens(const qx_cuda_pick* p, void* stream, char* err, u
     a.allowed_stride = p->allowed_stride;
     a.picked = p->picked;
     cudaStream_t st = (cudaStream_t)stream;
-    // few rows leave SMs to spare: one CTA of 1024 threads each, else two of 512
-    const bool few = p->rows * kPickCluster <= 148;
     cudaError_t e;
-    if (p->dtype == QX_CUDA_F32) e = few ? launch_pick<float, 1024>(a, st) : launch_pick<float, 512>(a, st);
-    else if (p->dtype == QX_CUDA_F16) e = few ? launch_pick<__half, 1024>(a, st) : launch_pick<__half, 512>(a, st);
-    else e = few ? launch_pick<__nv_bfloat16, 1024>(a, st) : launch_pick<__nv_bfloat16, 512>(a, st);
+    if (p->dtype == QX_CUDA_F32) e = run_pick<float>(a, st);
+    else if (p->dtype == QX_CUDA_F16) e = run_pick<__half>(a, st);
+    else e = run_pick<__nv_bfloat16>(a, st);
     return finish(e, err, n);
 }
