@@ -2,8 +2,8 @@
 // row (qx_cuda_pick_tokens).
 //
 // A cluster of CTAs takes row after row; each CTA owns a slice of the
-// vocabulary (every eighth 64 tokens: frequent tokens lie together, and one CTA
-// with all of them held the others up, 131 us against 113 for 256 rows of
+// vocabulary (of eight CTAs every eighth 64 tokens: frequent tokens lie together, and one CTA
+// with all of them held the others up, 131 us against 112 for 256 rows of
 // 151936) and keeps one 32-bit word per token of it in shared memory: the
 // token's count in the history (low 20 bits) and the last bias entry that names
 // it, plus one (high 12 bits).  Every CTA reads the whole history and counts
@@ -13,12 +13,12 @@
 // where this way took 135).  Integer atomics, so the order they land in changes
 // nothing.  Then each CTA streams its slice of the logits once, putting the
 // words it finds back to 0 for the next row, and leaves its best with the
-// cluster's first CTA, which joins a row's eight while the next is counted: no
+// cluster's first CTA, which joins a row's parts while the next is counted: no
 // workspace, one launch, and no wait between rows that the next row's first
 // loads do not overlap.
 //
 // 256 rows of 151936 F32 logits with a mask, 64 biases and histories of 4096
-// move 311 MB, 49 us at the memory's rate, and take 113 us, bound by
+// move 311 MB, 49 us at the memory's rate, and take 112 us, bound by
 // instructions: of each 128 tokens a warp looks at, three or four are in the
 // history, and each of the four lanes' words costs its branch.  Dearer were: a queue
 // of such tokens per warp, emptied 32 at a time (134 us: its scans), and a second
@@ -317,10 +317,12 @@ cudaError_t launch_pick(PickArgs a, cudaStream_t st) {
 
 template <class T>
 cudaError_t run_pick(const PickArgs& a, cudaStream_t st) {
-    // Few rows leave SMs to spare: one CTA of 1024 threads each.  Else two of 512 (rows of 50257, 64 of them: XX).
+    // Few rows leave SMs to spare: one CTA of 1024 threads each.  Else two of 512.
     if (a.rows * 8 <= 148) return launch_pick<T, 1024, 8>(a, st);
-    // More rows than there are clusters of eight: clusters of four read the histories half as often, if two of their
-    // larger slices fit an SM.
+    // More rows than there are clusters: smaller ones read the histories less often and wait for fewer, if two of their
+    // larger slices fit an SM (256 rows of 32000 took 33 us by clusters of four, take 25 by two; 64 rows of 50257 took
+    // 17 us by eight, take 11 by four; one CTA of 1024 threads with a slice of a quarter was no faster for rows of 151936).
+    if (a.rows * 4 > 2 * 148 && slice_of(a.vocab, 2) * 4 <= 100 * 1024) return launch_pick<T, 512, 2>(a, st);
     if (a.rows * 8 > 2 * 148 && slice_of(a.vocab, 4) * 4 <= 100 * 1024) return launch_pick<T, 512, 4>(a, st);
     return launch_pick<T, 512, 8>(a, st);
 }

@@ -704,6 +704,14 @@ def test_pick_tokens_of_strided_rows(stride, in_place):
     run_pick(stride, 5, 5000, "bf16", 64, 12, True, stride=stride, in_place=in_place, lens=False)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(25, 30011), (45, 151936), (60, 60001), (90, 4099), (170, 33), (170, 30011)])
+def test_pick_tokens_of_more_rows_than_fit_at_once(kind, rows, vocab):
+    """Each way of sharing rows and vocabulary out, with rows that follow one another in the same CTAs."""
+    run_pick(rows + vocab, rows, vocab, kind, 200, 17, True)
+    run_pick(rows, rows, vocab, kind, 0, 0, False)
+
+
 def test_pick_tokens_of_a_large_vocabulary_and_history():
     run_pick(8, 2, 393216, "bf16", 70000, 4095, True)
 
