@@ -3,7 +3,7 @@
 //
 // A cluster of CTAs takes row after row; each CTA owns a slice of the
 // vocabulary (of eight CTAs every eighth 64 tokens: frequent tokens lie together, and one CTA
-// with all of them held the others up, 131 us against 112 for 256 rows of
+// with all of them held the others up, 131 us against 111 for 256 rows of
 // 151936) and keeps one 32-bit word per token of it in shared memory: the
 // token's count in the history (low 20 bits) and the last bias entry that names
 // it, plus one (high 12 bits).  Every CTA reads the whole history and counts
@@ -18,9 +18,9 @@
 // loads do not overlap.
 //
 // 256 rows of 151936 F32 logits with a mask, 64 biases and histories of 4096
-// move 311 MB, 49 us at the memory's rate, and take 112 us, bound by
-// instructions: of each 128 tokens a warp looks at, three or four are in the
-// history, and each of the four lanes' words costs its branch.  Dearer were: a queue
+// move 311 MB, 49 us at the memory's rate, and take 111 us, bound by
+// instructions and the latency of a row's steps: of each 128 tokens a warp looks at, three or four are in the
+// history (a branch for each of a lane's four words instead of a loop over those that are: 113 us).  Dearer were: a queue
 // of such tokens per warp, emptied 32 at a time (134 us: its scans), and a second
 // walk over the history that changes them after the pass (134 us: it reads
 // every id again in every CTA).
@@ -212,10 +212,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
                             const uint4 q = *word4;
                             if (q.x | q.y | q.z | q.w) {
                                 *word4 = make_uint4(0, 0, 0, 0);
-                                if (q.x) v[u] = touch(v[u], q.x);
-                                if (q.y) v[u + 1] = touch(v[u + 1], q.y);
-                                if (q.z) v[u + 2] = touch(v[u + 2], q.z);
-                                if (q.w) v[u + 3] = touch(v[u + 3], q.w);
+                                uint32_t left = (q.x ? 1u : 0u) | (q.y ? 2u : 0u) | (q.z ? 4u : 0u) | (q.w ? 8u : 0u);
+                                do {                                         // most lanes that have one have no other
+                                    const bool hi = !(left & 3u), odd = !(left & (hi ? 4u : 1u));
+                                    const uint32_t w = hi ? (odd ? q.w : q.z) : (odd ? q.y : q.x);
+                                    const float x = touch(hi ? (odd ? v[u + 3] : v[u + 2]) : (odd ? v[u + 1] : v[u]), w);
+                                    if (!hi && !odd) v[u] = x;
+                                    if (!hi && odd) v[u + 1] = x;
+                                    if (hi && !odd) v[u + 2] = x;
+                                    if (hi && odd) v[u + 3] = x;
+                                    left &= left - 1;
+                                } while (left);
                             }
                         }
                     float big = -INFINITY;

@@ -166,9 +166,9 @@ __device__ __forceinline__ void dot_block(const uint8_t* block, int c, const uin
 
 // For trees with few query rows to a KV head, where reading the cache is most
 // of the work.  64 sequences of one token over 4096 rows (BF16, 4 KV heads of
-// 128; 271 MB, 41 us at the memory's rate) take 69 us, F32 82 us; with 32 query rows 111
+// 128; 271 MB, 41 us at the memory's rate) take 68 us, F32 81 us; with 32 query rows 103
 // us.  Bound by instructions and their latency: turning the codes to F16 costs as many as
-// the products, and registers allow 12 warps an SM (8 with 32 rows).  One token over 32768 rows takes 28 us,
+// the products, and registers allow 12 warps an SM (8 with 32 rows).  One token over 32768 rows takes 26 us,
 // over 513 rows 12 us, which is launching, finding one's tiles and joining parts.
 //
 // Blocks of 16 MT query rows; each of the 4 warps takes 16 of a tile's 64 cache
@@ -566,9 +566,9 @@ __global__ void __launch_bounds__(kJoinThreads, 4) k_tree_join(const __grid_cons
 // and a warp goes through them with a step's keys in registers: it alone adds
 // to the step's rows, in one order, without atomics.
 //
-// For 64 ragged sequences of one token over up to 4096 rows it is 30 us of the
-// call's 64; for 64 trees of 16 nodes (512 query rows) over 4096 rows 188 of
-// 343, bound by mma.sync, whose pipe 16 products of 16 x 8 x 16 a block keep busy
+// For 64 ragged sequences of one token over up to 4096 rows it is 27 us of the
+// call's 63; for 64 trees of 16 nodes (512 query rows) over 4096 rows 187 of
+// 338, bound by mma.sync, whose pipe 16 products of 16 x 8 x 16 a block keep busy
 // (staging the queries anew for every tile and block took 1150 us).
 constexpr int kMassWarps = 16, kMassThreads = kMassWarps * 32;
 template <int HD, int NT>
@@ -741,9 +741,9 @@ Plan plan_of(uint32_t seqs, uint32_t max_nodes, uint32_t q_heads, uint32_t kv_he
     Plan p{};
     const uint64_t rows = (uint64_t)max_nodes * (q_heads / kv_heads);
     p.tc = rows > 32;
-    // 64 sequences of 4096 rows, BF16, 4 KV heads of 128: 16 query rows to a KV head take 75 us in blocks of 16; 32 rows
-    // 111 us in blocks of 32, 147 us in two of 16; 64 rows 138 us on tcgen05, whose time depends little on how many of
-    // its 128 rows there are (128: 155 us).
+    // 64 sequences of 4096 rows, BF16, 4 KV heads of 128: 16 query rows to a KV head take 71 us in blocks of 16; 32 rows
+    // 103 us in blocks of 32, 147 us in two of 16; 64 rows 136 us on tcgen05, whose time depends little on how many of
+    // its 128 rows there are (128: 151 us).
     p.block_rows = p.tc ? 128 : rows > 16 ? 32 : 16;
     p.row_blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
     p.parts = (uint64_t)2 * most_ctas(p.block_rows) * p.block_rows * (kPartHead + head_dim) * 4;
