@@ -253,6 +253,8 @@ def attention(c, layer, slots, lens, nodes, q, mask, scale):
     tol_mass = torch.zeros_like(mass)
     for s in range(seqs):
         sl, a, m = int(slots[s]), int(lens[s]), int(nodes[s])
+        if not m:
+            continue                                            # no row to compare
         t = a + m
         ks, vs = c.k_scales[sl, layer, :t].double(), c.v_scales[sl, layer, :t].double().clamp(min=2.0 ** -90)
         k, v = c.k[sl, layer, :t].double(), c.v[sl, layer, :t].double()
@@ -351,6 +353,19 @@ def test_tree_attention_splits(kind, seqs, n, ctx):
     q = torch.randn(seqs, n, 8, 128, generator=g, device=DEV).to(TYPES[kind])
     lens = ints([ctx - (i * 7) % min(ctx, 250) for i in range(seqs)])
     check_tree(c, 0, ints(list(range(seqs))), lens, None, q, random_tree(seqs, n, 3), 0.1)
+
+
+@pytest.mark.parametrize("kind,n", [("bf16", 1), ("f32", 3), ("f16", 9)])
+def test_tree_attention_of_hundreds_of_sequences(kind, n):
+    """More sequences than threads that look them up, some without nodes, in each of the kernels."""
+    g = gen(n)
+    seqs = 300
+    c = make_cache(g, seqs, 1, 90 + n, 1, 64)
+    q = torch.randn(seqs, n, 8, 64, generator=g, device=DEV).to(TYPES[kind])
+    lens = torch.randint(0, 91, (seqs,), generator=g, device=DEV, dtype=torch.int32)
+    nodes = torch.randint(0, n + 1, (seqs,), generator=g, device=DEV, dtype=torch.int32)
+    slots = torch.randperm(seqs, generator=g, device=DEV).to(torch.int32)
+    check_tree(c, 0, slots, lens, nodes, q, random_tree(seqs, n, 8), 0.125)
 
 
 def test_tree_attention_of_a_chain_of_many_rows():
