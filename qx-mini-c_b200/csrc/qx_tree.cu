@@ -566,9 +566,9 @@ __global__ void __launch_bounds__(kJoinThreads, 4) k_tree_join(const __grid_cons
 // and a warp goes through them with a step's keys in registers: it alone adds
 // to the step's rows, in one order, without atomics.
 //
-// For 64 ragged sequences of one token over up to 4096 rows it is 27 us of the
-// call's 63; for 64 trees of 16 nodes (512 query rows) over 4096 rows 187 of
-// 338, bound by mma.sync, whose pipe 16 products of 16 x 8 x 16 a block keep busy
+// For 64 ragged sequences of one token over up to 4096 rows it is 25 us of the
+// call's 61, bound by instructions and by steps that come out uneven (25 for 16 warps); for 64 trees of 16 nodes (512
+// query rows) over 4096 rows 183 of 334, bound by mma.sync, whose pipe 16 products of 16 x 8 x 16 a block keep busy
 // (staging the queries anew for every tile and block took 1150 us).
 constexpr int kMassWarps = 16, kMassThreads = kMassWarps * 32;
 template <int HD, int NT>
@@ -591,9 +591,12 @@ struct StepKeys {
         for (int i = 0; i < 4; ++i) ks[i] = ks0[min(r0 + 4 * j + i, last)];
     }
 };
-template <class T, int HD, int NT>
+// ONE: a KV head's query rows are one block at most.  Its keys are needed once, and those of three steps are on their
+// way (64 ragged sequences of one token: 63 us for the call with one, 61 with three).
+template <class T, int HD, int NT, bool ONE>
 __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_constant__ TreeArgs a) {
     using Block = Held<HD, NT>;
+    constexpr int kAhead = ONE ? 3 : 1;
     extern __shared__ __align__(128) uint8_t dyn[];
     __shared__ int warp_sum[kScanThreads / 32], at_seq, at_first, clash;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 3, n8 = lane >> 2;
@@ -644,9 +647,16 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_cons
         const int rows = n * a.group, per_head = (rows + 15) / 16, blocks = per_head * a.c.kv_heads;
         for (int b0 = 0; b0 < blocks; b0 += Block::kMost) {
             const int b1 = min(blocks, b0 + Block::kMost);
-            StepKeys<HD> next;
-            if (step0 + warp < step1)
-                next.load(k0 + b0 / per_head * HD, ks0, row_bytes, (step0 + warp) * 16, last);
+            const int g0 = b0 / per_head, g1 = (b1 - 1) / per_head;
+            StepKeys<HD> next[kAhead];
+            int next_st = step0 + warp, next_g = g0;
+            auto fetch = [&](StepKeys<HD>& k) {            // the warp's next step and head
+                if (next_st >= step1) return;
+                k.load(k0 + next_g * HD, ks0, row_bytes, next_st * 16, last);
+                if (++next_g > g1) next_g = g0, next_st += kMassWarps;
+            };
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) fetch(next[i]);
             __syncthreads();                               // the blocks before have been used
             if (clash) break;
             for (int i = warp; i < 4 * (b1 - b0); i += kMassWarps) {
@@ -661,57 +671,39 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_cons
                         make_float2(lane == 0 ? undo[0] : lane == 1 ? undo[1] : lane == 2 ? undo[2] : undo[3], lg);
             }
             __syncthreads();
-            const int g0 = b0 / per_head, g1 = (b1 - 1) / per_head;
-            for (int st = step0 + warp; st < step1; st += kMassWarps) {
-                const int r0 = st * 16;
+            float got[4] = {};
+            // the weights of the block's rows for rows r0 + 4 j .. + 3 of the cache, from their products
+            auto weigh = [&](const float (&part)[HD / 64][2][4], const float (&ks)[4], const uint8_t* block, int row0, int r0) {
+                const float2* facs = reinterpret_cast<const float2*>(block + Block::kFacs);
                 const bool edge = r0 + 16 > len;
-                float got[4] = {};
-                for (int g = g0; g <= g1; ++g) {
-                    const float ks[4] = {next.ks[0], next.ks[1], next.ks[2], next.ks[3]};
-                    uint32_t key[2][HD / 8];
+                float e[2][4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                for (int u = 0; u < 2; ++u) {
+                    const float2 fl = facs[n8 + 8 * u];
 #pragma unroll
-                        for (int c = 0; c < HD / 64; ++c) key_halves(next.k[h][c], key[h] + 8 * c);
-                    const bool more = g < g1;
-                    if (more || st + kMassWarps < step1)
-                        next.load(k0 + (more ? g + 1 : g0) * HD, ks0, row_bytes, more ? r0 : r0 + 16 * kMassWarps, last);
-                    const int first_b = max(b0, g * per_head), end_b = min(b1, (g + 1) * per_head);
-                    for (int b = first_b; b < end_b; ++b) {
-                        const uint8_t* block = dyn + (size_t)(b - b0) * Block::kBytes;
-                        float part[HD / 64][2][4] = {}, acc[2][4];   // apart, for shorter chains of products
-#pragma unroll
-                        for (int c = 0; c < HD / 64; ++c) dot_block<HD, NT>(block, c, key[0] + 8 * c, key[1] + 8 * c, part[c]);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            acc[i >> 2][i & 3] = HD == 128 ? part[0][i >> 2][i & 3] + part[HD / 64 - 1][i >> 2][i & 3] : part[0][i >> 2][i & 3];
-                        const int row0 = (b - g * per_head) * 16;
-                        const float2* facs = reinterpret_cast<const float2*>(block + Block::kFacs);
-                        float e[2][4];
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const float2 fl = facs[n8 + 8 * u];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                e[u][i] = exp2_fast(fmaf(acc[i >> 1][2 * u + (i & 1)] * fl.x, ks[i], -fl.y));
-                        }
-                        if (edge || row0 + 16 > rows) {
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const int r = row0 + n8 + 8 * u, node = r / a.group;
-                                uint32_t seen = r < rows ? 15u : 0u;
-                                if (edge && r < rows)
-                                    seen = (uint32_t)sees64(a.mask ? a.mask + ((size_t)s * a.d.max_nodes + node) * a.words : nullptr,
-                                                            a.words, node, r0 + 4 * j, len, n);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (!(seen >> i & 1u)) e[u][i] = 0.f;
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) got[i] += e[0][i] + e[1][i];
+                    for (int i = 0; i < 4; ++i) {
+                        float x = part[0][i >> 1][2 * u + (i & 1)];
+                        if (HD == 128) x += part[HD / 64 - 1][i >> 1][2 * u + (i & 1)];
+                        e[u][i] = exp2_fast(fmaf(x * fl.x, ks[i], -fl.y));
                     }
                 }
+                if (edge || row0 + 16 > rows) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int r = row0 + n8 + 8 * u, node = (int)a.per_group(r);
+                        uint32_t seen = r < rows ? 15u : 0u;
+                        if (edge && r < rows)
+                            seen = (uint32_t)sees64(a.mask ? a.mask + ((size_t)s * a.d.max_nodes + node) * a.words : nullptr,
+                                                    a.words, node, r0 + 4 * j, len, n);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!(seen >> i & 1u)) e[u][i] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) got[i] += e[0][i] + e[1][i];
+            };
+            auto put = [&](int r0) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     got[i] += __shfl_xor_sync(~0u, got[i], 4);
@@ -721,6 +713,51 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_cons
                 const float x = n8 == 0 ? got[0] : n8 == 1 ? got[1] : n8 == 2 ? got[2] : got[3];
                 const int t = r0 + 4 * j + n8;
                 if (n8 < 4 && t <= last) a.mass[base_row + t] += x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) got[i] = 0.f;
+            };
+            int st = step0 + warp, g = g0;
+            while (ONE && st < step1)
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (st >= step1) break;
+                    const uint8_t* block = dyn + (size_t)(g - g0) * Block::kBytes;
+                    const float ks[4] = {next[i].ks[0], next[i].ks[1], next[i].ks[2], next[i].ks[3]};
+                    float part[HD / 64][2][4] = {};                  // apart, for shorter chains of products
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c) {
+                        uint32_t key[2][8];
+                        key_halves(next[i].k[0][c], key[0]);
+                        key_halves(next[i].k[1][c], key[1]);
+                        dot_block<HD, NT>(block, c, key[0], key[1], part[c]);
+                    }
+                    fetch(next[i]);
+                    weigh(part, ks, block, 0, st * 16);
+                    if (++g > g1) {
+                        put(st * 16);
+                        st += kMassWarps;
+                        g = g0;
+                    }
+                }
+            for (; !ONE && st < step1; st += kMassWarps) {
+                for (g = g0; g <= g1; ++g) {
+                    const float ks[4] = {next[0].ks[0], next[0].ks[1], next[0].ks[2], next[0].ks[3]};
+                    uint32_t key[2][HD / 8];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int c = 0; c < HD / 64; ++c) key_halves(next[0].k[h][c], key[h] + 8 * c);
+                    fetch(next[0]);
+                    const int first_b = max(b0, g * per_head), end_b = min(b1, (g + 1) * per_head);
+                    for (int b = first_b; b < end_b; ++b) {
+                        const uint8_t* block = dyn + (size_t)(b - b0) * Block::kBytes;
+                        float part[HD / 64][2][4] = {};
+#pragma unroll
+                        for (int c = 0; c < HD / 64; ++c) dot_block<HD, NT>(block, c, key[0] + 8 * c, key[1] + 8 * c, part[c]);
+                        weigh(part, ks, block, (b - g * per_head) * 16, st * 16);
+                    }
+                }
+                put(st * 16);
             }
         }
         if (clash && tid == 0 && a.status) atomicOr(a.status, QX_CUDA_STATUS_SHARED);
@@ -792,9 +829,10 @@ cudaError_t run_typed(TreeArgs& a, bool tc, uint32_t type, int sms, cudaStream_t
     e = cudaLaunchKernelEx(&cfg, k_tree_join<T, HD>, a);
     if (e != cudaSuccess || !a.mass) return e;
     constexpr int kHeld = Held<HD, NT>::kMost * Held<HD, NT>::kBytes;
-    e = cudaFuncSetAttribute((const void*)k_tree_mass<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld);
+    const auto kernel = a.block_rows == 16 ? k_tree_mass<T, HD, NT, true> : k_tree_mass<T, HD, NT, false>;
+    e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld);
     if (e != cudaSuccess) return e;
-    k_tree_mass<T, HD, NT><<<sms, kMassThreads, kHeld, st>>>(a);
+    kernel<<<sms, kMassThreads, kHeld, st>>>(a);
     return cudaGetLastError();
 }
 
