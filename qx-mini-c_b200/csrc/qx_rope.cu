@@ -16,7 +16,6 @@ namespace {
 
 using namespace qx::ops;
 
-constexpr int kRopeThreads = 128;
 
 struct Heads {
     const void* p;
@@ -87,13 +86,13 @@ __device__ __forceinline__ int code_of(float x, float scale, float inv) {
 // 28 us fully rotated, 24 us with half of each head rotated in pairs.  What is left are instructions: the
 // scheduler issues in 62 of 100 cycles, a quarter of them sines and keys in
 // double.  8 CTAs to an SM and one item ahead did best: 2 items 33 us, 3 items
-// and 5 CTAs 40 us, 256 threads 37 us.
-template <class T, int V, bool IL>
-__global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
+// and 5 CTAs 40 us.
+template <class T, int V, bool IL, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_rope_append(RopeArgs a) {
     extern __shared__ __align__(16) float kvrow[];       // [2][kv]: rotated key, value
     __shared__ double cs_d[2][256 + 1];
     __shared__ float cs_f[2][256 + 1];
-    __shared__ float wmax[2][kRopeThreads / 32];
+    __shared__ float wmax[2][THREADS / 32];
     __shared__ int clash;
     const int node = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
     const int D = a.c.head_dim, KV = a.c.kv_heads * D, rd = a.rd, half = rd / 2;
@@ -131,7 +130,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
     if (tid < k_items) load_k(tid, kx, ky);
     if (tid < v_packs) vx = load_v(tid);
     if (tid < q_items) load_q(tid, qx, qy);
-    for (int i = tid; i < half; i += kRopeThreads) {
+    for (int i = tid; i < half; i += THREADS) {
         double sn, cn;
         sincos(__dmul_rn((double)pos, a.inv_freq[i]), &sn, &cn);
         cs_f[0][i] = (float)(cs_d[0][i] = __dmul_rn(cn, a.amplitude));
@@ -139,7 +138,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
     }
     __syncthreads();
     if (a.k.p)                                           // another sequence of the call that appends to this slot
-        for (int j = tid; j < a.d.seqs; j += kRopeThreads)
+        for (int j = tid; j < a.d.seqs; j += THREADS)
             if (j != s && a.d.slots[j] == slot) {
                 const int m = a.d.count(j);
                 if (m > 0 && fits(a.c, a.d, slot, a.d.lens[j], m)) clash = 1;
@@ -183,13 +182,13 @@ __global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
             }
         };
         if (tid < k_items) key(tid, kx, ky);
-        for (int w = tid + kRopeThreads; w < k_items; w += kRopeThreads) {
+        for (int w = tid + THREADS; w < k_items; w += THREADS) {
             T x[V], y[V];
             load_k(w, x, y);
             key(w, x, y);
         }
         if (tid < v_packs) value(tid, vx);
-        for (int w = tid + kRopeThreads; w < v_packs; w += kRopeThreads)
+        for (int w = tid + THREADS; w < v_packs; w += THREADS)
             value(w, load_v(w));
         for (int o = 16; o; o >>= 1) {
             ka = fmaxf(ka, __shfl_xor_sync(~0u, ka, o));
@@ -235,7 +234,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
             }
         };
         if (tid < q_items) query(tid, qx, qy);
-        for (int w = tid + kRopeThreads; w < q_items; w += kRopeThreads) {
+        for (int w = tid + THREADS; w < q_items; w += THREADS) {
             T x[V], y[V];
             load_q(w, x, y);
             query(w, x, y);
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
     }
     if (!a.k.p) return;
     ka = va = 0.f;
-    for (int w = 0; w < kRopeThreads / 32; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
         ka = fmaxf(ka, wmax[0][w]);
         va = fmaxf(va, wmax[1][w]);
     }
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) k_rope_append(RopeArgs a) {
     if (!(ksc > 0.f)) ksc = 1.0f;                        // a row of zeros, or one whose quotient underflows
     if (!(vsc > 0.f)) vsc = 1.0f;
     const size_t row = (size_t)slot * a.c.slot_rows + (size_t)a.layer * a.c.layer_rows + (size_t)(len + node);
-    for (int w = tid; w < 2 * KV / 4; w += kRopeThreads) {
+    for (int w = tid; w < 2 * KV / 4; w += THREADS) {
         const bool isv = w >= KV / 4;
         const float4 x = *reinterpret_cast<const float4*>(kvrow + 4 * w);
         const float sc = isv ? vsc : ksc, inv = 1.0f / sc;
@@ -277,11 +276,15 @@ cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
     a.v_packs = Over((uint32_t)a.c.head_dim / V);
     const dim3 grid((unsigned)a.d.max_nodes, (unsigned)a.d.seqs);
     const size_t sm = a.k.p ? (size_t)2 * a.c.kv_heads * a.c.head_dim * 4 : 0;
-    auto fn = a.interleaved ? k_rope_append<T, V, true> : k_rope_append<T, V, false>;
+    // 256 threads a token while all of them run at once (one token 5.6 -> 5.0 us, 64 trees of 16 nodes 7.5 -> 6.9 us; a
+    // prompt of 4096 tokens 28 -> 37 us)
+    const bool few = (uint64_t)a.d.max_nodes * a.d.seqs <= 148 * 8;
+    auto fn = a.interleaved ? (few ? k_rope_append<T, V, true, 256> : k_rope_append<T, V, true, 128>)
+                            : (few ? k_rope_append<T, V, false, 256> : k_rope_append<T, V, false, 128>);
     cudaError_t e = cudaSuccess;
     if (sm > 40 * 1024) e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
     if (e != cudaSuccess) return e;
-    fn<<<grid, kRopeThreads, sm, st>>>(a);
+    fn<<<grid, few ? 256 : 128, sm, st>>>(a);
     return cudaGetLastError();
 }
 

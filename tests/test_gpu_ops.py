@@ -212,6 +212,21 @@ def test_rope_append_of_many_wide_heads():
         check_rope(c, before, 0, slots, lens, nodes, q, k, v, inv, pos, 1.0, 48, il, out, torch.zeros_like(q))
 
 
+@pytest.mark.parametrize("kind,interleaved", [("f32", True), ("bf16", False), ("f16", True)])
+def test_rope_append_of_long_prompts(kind, interleaved):
+    """More tokens than run at once: chunks of up to 700 of three sequences, one ragged, one with nothing to append."""
+    g = gen(41)
+    c = make_cache(g, 3, 1, 720, 2, 64)
+    before = copies(c)
+    q, k, v = (torch.randn(3, 700, h, 64, generator=g, device=DEV).to(TYPES[kind]) for h in (6, 2, 2))
+    inv = torch.from_numpy(qxops.rope_frequencies(40)[0]).to(DEV)
+    slots, lens, nodes = ints([2, 0, 1]), ints([20, 3, 700]), ints([700, 411, 0])
+    pos = (lens[:, None] + torch.arange(700, device=DEV, dtype=torch.int32)).contiguous()
+    out = torch.full_like(q, 5)
+    qxops.rope_append(c, 0, slots, lens, q, k, v, inv, nodes=nodes, interleaved=interleaved, q_out=out)
+    check_rope(c, before, 0, slots, lens, nodes, q, k, v, inv, pos, 1.0, 40, interleaved, out, torch.full_like(q, 5))
+
+
 def test_rope_append_leaves_out_what_does_not_fit():
     g = gen(8)
     c = make_cache(g, 3, 1, 6, 1, 64)
