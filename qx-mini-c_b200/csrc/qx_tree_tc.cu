@@ -612,6 +612,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                     }
                 }
             }
+            pc = qc;                                             // every piece of the list with tiles has its queries
         } else if (warp == 10) {
             // ---- ask for the codes ----
             const uint32_t raw_a = smem_addr(raw_s);
