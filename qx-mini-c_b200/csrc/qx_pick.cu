@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
     cg::cluster_group cl = cg::this_cluster();
     const int rank = (int)cl.block_rank(), step = gridDim.x / CL, tid = threadIdx.x;
     const bool touched = a.history || a.bias_ids;
+    cluster_arrive();                                        // this CTA has started: its memory may be written by the others
     if (touched) {
         for (int i = tid * 4; i < a.slice; i += THREADS * 4) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
@@ -175,10 +176,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_pick(const __grid_c
                 for (int e = j; e < min(j + 4, nh); ++e) count(h[e]);
             }
         }
-        if (r != first) {
-            cluster_wait();
-            join(r - step, slot ^ 1);
-        }
+        cluster_wait();                                                  // first row: every CTA has started
+        if (r != first) join(r - step, slot ^ 1);
         __syncthreads();
         Best best{-INFINITY, 0x7fffffff, 0};
         auto touch = [&](float v, uint32_t w) {

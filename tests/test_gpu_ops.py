@@ -746,6 +746,26 @@ def test_pick_tokens_of_a_large_vocabulary_and_history():
     run_pick(8, 2, 393216, "bf16", 70000, 4095, True)
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 300), (18, 5000), (30, 40001), (100, 9000)])
+def test_pick_tokens_call_after_call(rows, vocab):
+    """Hundreds of short calls on two streams at once, each way of sharing rows out: CTAs of a cluster start one after the other
+    while others still run, and the first of each joins what the others leave with it."""
+    x = torch.randn(64, rows, vocab, generator=gen(rows), device=DEV)
+    want = x.argmax(-1).to(torch.int32)
+    tok = torch.zeros(2, 64, rows, dtype=torch.int32, device=DEV)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        tok.fill_(-2)
+        torch.cuda.synchronize()
+        for i in range(64):
+            for s, t in zip(streams, tok):
+                with torch.cuda.stream(s):
+                    qxops.pick_tokens(x[i], picked=t[i])
+        torch.cuda.synchronize()
+        assert torch.equal(tok[0], want) and torch.equal(tok[1], want)
+
+
 def test_pick_without_output():
     x = torch.randn(3, 777, device=DEV)
     args = opsabi.Pick(x.data_ptr(), None, 777, 0, 3, 777, 0, 0, 0, 0, *([None] * 9), 0, 0, 0, 0)
