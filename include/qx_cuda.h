@@ -330,6 +330,18 @@ int qx_cuda_rope_append(const qx_cuda_kv_cache *cache, uint32_t layer, const qx_
                         const qx_cuda_heads *q_out, const qx_cuda_heads *k, const qx_cuda_heads *v,
                         const int32_t *positions, uint32_t *status, void *stream, char *err, uint64_t err_len);
 
+/* The same, for a cache whose rows' weights are collected: mass (of
+ * qx_cuda_tree_attention; F32, one value per row at the index of the row's
+ * scales; NULL: as above) becomes 0 for every row that is appended, so that a
+ * token does not start with what a rejected node, or whatever else was in its
+ * row before, had gathered.  Needs k and v.  A caller that writes rows in
+ * another way (an engine's prefill) sets their mass to 0 itself. */
+int qx_cuda_rope_append_mass(const qx_cuda_kv_cache *cache, uint32_t layer, const qx_cuda_drafts *drafts,
+                             const qx_cuda_rotary *rotary, uint32_t dtype, uint32_t q_heads, const qx_cuda_heads *q,
+                             const qx_cuda_heads *q_out, const qx_cuda_heads *k, const qx_cuda_heads *v,
+                             const int32_t *positions, float *mass, uint32_t *status, void *stream, char *err,
+                             uint64_t err_len);
+
 /* Attention of the drafted tokens over layer `layer` of the cache.  Node j of
  * sequence i sees the committed rows and those tree rows whose bit is set in
  * its mask: bit b of mask[(i * max_nodes + j) * words + b / 64], words =
@@ -344,8 +356,9 @@ int qx_cuda_rope_append(const qx_cuda_kv_cache *cache, uint32_t layer, const qx_
  *   lse[seqs][max_nodes][q_heads] (F32, may be NULL): log of the softmax sum.
  *   mass (F32, one value per row at the index of the row's scales, may be
  *   NULL): adds, for each row, the weights that all nodes and heads of the
- *   call gave it - what qx_cuda_kv_evict goes by.  Sequences of one call then
- *   need distinct slots.
+ *   call gave it, drafted rows included - what qx_cuda_kv_evict goes by.  Rows
+ *   that are written anew have to start from 0 (qx_cuda_rope_append_mass).
+ *   Sequences of one call then need distinct slots.
  * Rows of out and lse past a sequence's nodes stay as they were.  Sequences
  * may share a slot when mass is NULL.  The same call gives the same bits every
  * time; how a sequence's rows are split over the GPU, and so its rounding,
@@ -367,8 +380,9 @@ int qx_cuda_tree_attention_workspace(uint32_t seqs, uint32_t max_nodes, uint32_t
  * keeps the lower row, NaN counts as less than any number.  Sequences of at
  * most `budget` rows keep all.  The kept rows' codes, scales and mass move to
  * rows 0.. of slot dst_slots[i] (NULL: in place), the mass of the rows behind
- * them up to lens[i] becomes 0, and other rows stay as they were.  A
- * destination slot must be no other sequence's source or destination.
+ * them up to lens[i] becomes 0, and other rows stay as they were (a
+ * destination's rows behind lens[i] keep the mass they had until
+ * qx_cuda_rope_append_mass writes them anew).  A destination slot must be no other sequence's source or destination.
  *   kept[layers][seqs][budget] (int32): the rows kept, -1 past the last;
  *   all -1 for a sequence left out.
  *   new_lens[seqs] (int32, not lens itself): min(lens[i], budget); lens[i] for

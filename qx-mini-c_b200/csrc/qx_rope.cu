@@ -64,6 +64,7 @@ struct RopeArgs {
     Items q_items, k_items;
     Over v_packs;                                        // V-wide packs of a head
     const int* positions;
+    float* mass;                                         // 0 for an appended row, or null
     uint32_t* status;
 };
 
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_rope_append(RopeArg
     if (tid == 0) {
         a.c.ks[row] = ksc;
         a.c.vs[row] = vsc;
+        if (a.mass) a.mass[row] = 0.f;
     }
 }
 
@@ -335,6 +337,15 @@ QX_API int qx_cuda_rope_append(const qx_cuda_kv_cache* cache, uint32_t layer, co
                                const qx_cuda_rotary* rotary, uint32_t dtype, uint32_t q_heads, const qx_cuda_heads* q,
                                const qx_cuda_heads* q_out, const qx_cuda_heads* k, const qx_cuda_heads* v,
                                const int32_t* positions, uint32_t* status, void* stream, char* err, uint64_t n) {
+    return qx_cuda_rope_append_mass(cache, layer, drafts, rotary, dtype, q_heads, q, q_out, k, v, positions, nullptr, status,
+                                    stream, err, n);
+}
+
+QX_API int qx_cuda_rope_append_mass(const qx_cuda_kv_cache* cache, uint32_t layer, const qx_cuda_drafts* drafts,
+                                    const qx_cuda_rotary* rotary, uint32_t dtype, uint32_t q_heads, const qx_cuda_heads* q,
+                                    const qx_cuda_heads* q_out, const qx_cuda_heads* k, const qx_cuda_heads* v,
+                                    const int32_t* positions, float* mass, uint32_t* status, void* stream, char* err,
+                                    uint64_t n) {
     const char* m = check_cache(cache);
     if (!m) m = check_drafts(drafts);
     if (m) return refuse(err, n, m);
@@ -348,6 +359,8 @@ QX_API int qx_cuda_rope_append(const qx_cuda_kv_cache* cache, uint32_t layer, co
     const bool has_q = q && q->data, has_k = k && k->data;
     if (has_q != (q_out && q_out->data) || has_k != (v && v->data)) return refuse(err, n, "q goes with q_out, k with v");
     if (!has_q && !has_k) return refuse(err, n, "nothing to rotate");
+    if (mass && !has_k) return refuse(err, n, "mass goes with k and v");
+    if (!aligned(mass, 4)) return refuse(err, n, "mass must be 4-byte aligned");
     if (has_q) {
         if (!q_heads || q_heads > kMaxHeads) return refuse(err, n, "1 to 1024 query heads");
         m = check_heads(q, drafts->seqs, drafts->max_nodes, q_heads, D, dtype, false);
@@ -369,7 +382,7 @@ QX_API int qx_cuda_rope_append(const qx_cuda_kv_cache* cache, uint32_t layer, co
     };
     RopeArgs a{cache_of(cache), drafts_of(drafts), (int)layer, (int)q_heads, (int)rd, rotary->interleaved ? 1 : 0,
                rotary->inv_freq, rotary->amplitude, heads(q, has_q), heads(q_out, has_q), heads(k, has_k),
-               heads(v, has_k), {Over(1), Over(1), 0}, {Over(1), Over(1), 0}, Over(1), positions, status};
+               heads(v, has_k), {Over(1), Over(1), 0}, {Over(1), Over(1), 0}, Over(1), positions, mass, status};
     // 16-byte accesses where pointers, strides and the rotated part allow; else
     // element by element (odd strides or parts, which a view of a larger
     // projection can have)

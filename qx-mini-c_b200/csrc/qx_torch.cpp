@@ -138,10 +138,10 @@ qx_cuda_drafts drafts(const Handle& h, PyObject* slots, PyObject* lens, PyObject
             plain<int32_t>(lens, at::kInt, {seqs}, h.dev, "lens"), plain<int32_t>(nodes, at::kInt, {seqs}, h.dev, "nodes")};
 }
 
-// cache, layer, slots, lens, q, k, v, inv_freq, positions, nodes, interleaved, factor, q_out, status
+// cache, layer, slots, lens, q, k, v, inv_freq, positions, nodes, interleaved, factor, q_out, status, mass
 PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    arity(n, 14);
+    arity(n, 15);
     const Handle h = handle(a[0]);
     const at::Tensor *q = tensor(a[4], "q"), *k = tensor(a[5], "k"), *v = tensor(a[6], "v"), *qo = tensor(a[12], "q_out");
     const at::Tensor* x = q ? q : k;
@@ -165,9 +165,9 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const qx_cuda_heads hq = heads(q, st, x->sizes(), h.dev, "q"), ho = heads(qo, st, x->sizes(), h.dev, "q_out"),
                         hk = heads(k, st, kv_shape, h.dev, "k"), hv = heads(v, st, kv_shape, h.dev, "v");
     char err[256];
-    check(qx_cuda_rope_append(h.c, u32(a[1], "layer"), &d, &rot, type, q ? (uint32_t)q->size(2) : 0u, &hq, &ho, &hk, &hv,
-                              plain<int32_t>(a[8], at::kInt, {seqs, nodes}, h.dev, "positions"),
-                              plain<uint32_t>(a[13], at::kInt, {1}, h.dev, "status"), stream_of(h.dev), err, sizeof err),
+    check(qx_cuda_rope_append_mass(h.c, u32(a[1], "layer"), &d, &rot, type, q ? (uint32_t)q->size(2) : 0u, &hq, &ho, &hk, &hv,
+                                   plain<int32_t>(a[8], at::kInt, {seqs, nodes}, h.dev, "positions"), mass_of(a[14], h),
+                                   plain<uint32_t>(a[13], at::kInt, {1}, h.dev, "status"), stream_of(h.dev), err, sizeof err),
           err, "qx_cuda_rope_append");
     if (!q) Py_RETURN_NONE;
     return THPVariable_Wrap(*qo);

@@ -116,14 +116,15 @@ def rope_frequencies(rotary_dim, base=1e6, scheme="none", factor=1.0, original_c
 
 
 def rope_append(cache, layer, slots, lens, q, k, v, inv_freq, positions=None, nodes=None, interleaved=False, factor=1.0,
-                q_out=None, status=None):
+                q_out=None, status=None, mass=None):
     """Rotate drafted tokens and append their keys and values
-    (qx_cuda_rope_append).  q [seqs][nodes][q_heads][head_dim], k and v
+    (qx_cuda_rope_append_mass).  q [seqs][nodes][q_heads][head_dim], k and v
     [seqs][nodes][kv_heads][head_dim] of one float type (q, or k and v, may be
-    None); inv_freq float64 on the device, factor the amplitude.  Returns the
+    None); inv_freq float64 on the device, factor the amplitude; mass (like the
+    cache's scales) becomes 0 for the appended rows.  Returns the
     rotated queries (q_out; q itself rotates in place)."""
     return _native.rope_append(cache.handle, layer, slots, lens, q, k, v, inv_freq, positions, nodes, interleaved, factor, q_out,
-                               status)
+                               status, mass)
 
 
 def tree_attention(cache, layer, slots, lens, q, nodes=None, mask=None, scale=None, out=None, lse=None, mass=None,

@@ -841,6 +841,49 @@ def test_a_verify_step_and_its_captured_replay():
         assert all(torch.equal(x, y) for x, y in zip(d.results(), e.results())), lens
 
 
+def test_weights_of_rejected_nodes_do_not_reach_the_tokens_that_take_their_rows():
+    """Two verify steps, the first of which accepts none of its nodes (or one), on a cache whose mass behind the committed rows
+    is left over from something else: eviction goes by what each row's own token was given."""
+    g = gen(51)
+    n, ctx = 6, 120
+    c = make_cache(g, 3, 2, ctx, 2, 128)
+    slots, lens, mask = ints([2, 0, 1]), ints([100, 30, 57]), random_tree(3, n, 4)
+    inv = torch.from_numpy(qxops.rope_frequencies(128)[0]).to(DEV)
+    mass = 0.5 * torch.rand(c.k_scales.shape, generator=g, device=DEV)
+    other = mass[:, 0].clone()
+    want = mass.double()
+    tol = torch.zeros_like(want)
+    for accepted in ([0, 0, 1], None):
+        q, k, v = (torch.randn(3, n, h, 128, generator=g, device=DEV).bfloat16() for h in (8, 2, 2))
+        qo = qxops.rope_append(c, 1, slots, lens, q, k, v, inv, mass=mass)
+        for i in range(3):
+            rows = slice(int(lens[i]), int(lens[i]) + n)
+            want[int(slots[i]), 1, rows] = tol[int(slots[i]), 1, rows] = 0
+        qxops.tree_attention(c, 1, slots, lens, qo, mask=mask, mass=mass)
+        _, _, w, _, _, t = attention(c, 1, slots, lens, ints([n] * 3), qo, mask, 128 ** -0.5)
+        want, tol = want + w, tol + t + U32 * (want + w)
+        near(mass, want, tol, "mass")
+        lens = lens + ints(accepted) if accepted else lens + n
+    assert torch.equal(mass[:, 0], other)                        # the other layer's rows were not written
+    before, m0 = copies(c), mass.clone()
+    kept, new = qxops.evict(c, slots, lens, mass, 24, 2, 4)
+    e = evicted(before, m0, slots.tolist(), slots.tolist(), lens.tolist(), 24, 2, 4)
+    assert torch.equal(kept.cpu(), e[2]) and torch.equal(mass.cpu(), e[1])
+
+
+def test_rope_append_clears_the_mass_of_rows_it_writes_only():
+    g = gen(52)
+    c = make_cache(g, 4, 1, 12, 1, 64, layer_major=True)
+    inv = torch.from_numpy(qxops.rope_frequencies(64)[0]).to(DEV)
+    k, v = torch.randn(4, 3, 1, 64, generator=g, device=DEV), torch.randn(4, 3, 1, 64, generator=g, device=DEV)
+    mass = torch.ones_like(c.k_scales)
+    # sequence 0: two of three nodes; 1 and 2: one slot; 3: past the end
+    qxops.rope_append(c, 0, ints([3, 1, 1, 0]), ints([5, 0, 4, 11]), None, k, v, inv, nodes=ints([2, 3, 3, 3]), mass=mass)
+    want = torch.ones_like(mass)
+    want[3, 0, 5:7] = 0
+    assert torch.equal(mass, want)
+
+
 def test_verify_step_against_the_definitions():
     a = Loop(22)
     n = a.q.shape[1]

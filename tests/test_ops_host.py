@@ -254,3 +254,13 @@ def test_host_memory_is_refused():
 def test_view_refusals():
     ok, msg = said(opsabi.lib().qx_cuda_kv_view, None, 0, None)
     assert (ok, msg) == (0, "invalid cache view argument")
+
+
+def test_rope_append_mass_refusals():
+    fn = opsabi.lib().qx_cuda_rope_append_mass
+    P, U32 = C.c_void_p, C.c_uint32
+    fn.argtypes, fn.restype = [P, U32, P, P, U32, U32, P, P, P, P, P, P, P, P, C.c_char_p, C.c_uint64], C.c_int
+    c, d, r, h = cache(), drafts(), opsabi.Rotary(BASE, 1.0, 64, 0), heads()
+    call = lambda k, mass: said(fn, C.byref(c), 0, C.byref(d), C.byref(r), 0, 4, C.byref(h), C.byref(h), k, k, None, mass, None, None)  # noqa: E731
+    assert call(None, BASE) == (0, "mass goes with k and v")
+    assert call(C.byref(h), BASE + 2) == (0, "mass must be 4-byte aligned")
