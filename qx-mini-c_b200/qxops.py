@@ -19,7 +19,7 @@ qxlib.cuda()              # libqxcuda.so, or a message that says how to build it
 try:
     import _qxops as _native
 except ImportError as e:
-    raise RuntimeError("_qxops.so is not built (run make in %s)" % qxlib.HERE) from e
+    raise RuntimeError("_qxops.so is not built (run make all qxops in %s)" % qxlib.HERE) from e
 
 STATUS_RANGE = 0x1        # a sequence's slot, length or nodes lie outside the cache
 STATUS_SHARED = 0x2       # a slot written by a call is also another sequence's

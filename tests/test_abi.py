@@ -61,3 +61,12 @@ def test_create_from_image_rejects_corrupt_container(mini_image):
     ok = qxlib.cuda().qx_cuda_engine_create_from_image(bad.ctypes.data, bad.nbytes, C.byref(opt), C.byref(h), err,
                                                        len(err))
     assert ok == 0 and err.value == b"bad QXF magic"
+
+
+def test_the_engine_builds_without_python_or_torch():
+    """`make` alone plans the two C libraries; the torch module is a target of its own."""
+    plan = lambda *goal: subprocess.run(["make", "-C", os.path.join(ROOT, "qx-mini-c_b200"), "-n", "-B", "PYTHON=false", *goal],  # noqa: E731
+                                        capture_output=True, text=True, check=True).stdout
+    engine = plan()
+    assert "libqxcuda.so" in engine and "libqxhost.so" in engine and "torch" not in engine
+    assert "qx_torch.cpp" in plan("qxops")
