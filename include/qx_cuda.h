@@ -238,8 +238,9 @@ int qx_cuda_final_head_noalloc(const float *residual_dev, const float *norm_weig
  * with a message before anything is queued.  What only the device can see is
  * checked there: a sequence whose slot, length or node count does not fit the
  * cache, or which writes to a slot that another sequence of the call also
- * uses, is left out of the call (nothing is read or written for it) and a bit
- * is set in *status (device uint32, may be NULL; bits are only ever added).  */
+ * uses, is left out of the call (nothing is read or written for it; of mass,
+ * see qx_cuda_tree_attention) and a bit is set in *status (device uint32, may
+ * be NULL; bits are only ever added).  */
 #define QX_CUDA_F32  0u
 #define QX_CUDA_F16  1u
 #define QX_CUDA_BF16 2u
@@ -358,7 +359,9 @@ int qx_cuda_rope_append_mass(const qx_cuda_kv_cache *cache, uint32_t layer, cons
  *   NULL): adds, for each row, the weights that all nodes and heads of the
  *   call gave it, drafted rows included - what qx_cuda_kv_evict goes by.  Rows
  *   that are written anew have to start from 0 (qx_cuda_rope_append_mass).
- *   Sequences of one call then need distinct slots.
+ *   Sequences of one call then need distinct slots: those that share one add
+ *   nothing to mass (QX_CUDA_STATUS_SHARED); their out and lse, which are of
+ *   no slot, are written all the same.
  * Rows of out and lse past a sequence's nodes stay as they were.  Sequences
  * may share a slot when mass is NULL.  The same call gives the same bits every
  * time; how a sequence's rows are split over the GPU, and so its rounding,

@@ -467,6 +467,22 @@ def test_tree_attention_leaves_out_what_does_not_fit(n):
     assert int(status) == qxops.STATUS_SHARED and not mass[0].any() and bool((mass[1, 0, :20] > 0).all())
 
 
+@pytest.mark.parametrize("n", [1, 4, 20])
+def test_sequences_that_share_a_slot_attend_but_add_no_mass(n):
+    """In each kernel: out and lse are those of the call without mass, mass grows where a slot has one sequence."""
+    g = gen(14)
+    c = make_cache(g, 3, 1, 60, 2, 64)
+    q = torch.randn(4, n, 16, 64, generator=g, device=DEV)
+    args = (c, 0, ints([0, 2, 0, 1]), ints([20, 7, 33, 40]), q)
+    lse, lse_m, mass, status = (torch.zeros(4, n, 16, device=DEV), torch.zeros(4, n, 16, device=DEV), torch.zeros_like(c.k_scales), ints([0]))
+    out = qxops.tree_attention(*args, lse=lse, status=status)
+    assert int(status) == 0
+    got = qxops.tree_attention(*args, lse=lse_m, mass=mass, status=status)
+    assert int(status) == qxops.STATUS_SHARED
+    assert torch.equal(got, out) and torch.equal(lse_m, lse)
+    assert not mass[0].any() and bool((mass[1, 0, :40 + n] > 0).all()) and bool((mass[2, 0, :7 + n] > 0).all())
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,hd", [(3, 64), (4, 128)])
 def test_poison_in_trees_of_seventeen_to_thirty_two_rows(kind, n, hd):
