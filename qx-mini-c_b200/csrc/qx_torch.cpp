@@ -5,6 +5,7 @@
 // qx_cuda_rope_append, several times what its kernel takes for one token.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -46,10 +47,17 @@ uint32_t type_of(const at::Tensor& t) {
     }
 }
 
+// The operators have no backward pass: a result without its gradient is refused rather than given.
+void no_grad(const at::Tensor& t, const char* what) {
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+        bad(std::string(what) + " requires grad, and the operators have no backward pass: call them under torch.no_grad()");
+}
+
 void same(const at::Tensor& t, at::ScalarType type, at::IntArrayRef shape, c10::Device dev, const char* what, bool ok) {
     if (t.scalar_type() != type || t.device() != dev || t.sizes() != shape || !ok || t.is_conj() || t.is_neg())
         bad(std::string(what) + " must be a contiguous " + c10::toString(type) + " tensor of shape " + shape_of(shape) + " on " +
             dev.str());
+    no_grad(t, what);
 }
 
 // The address of a contiguous tensor of this type, shape and device; None: NULL.
@@ -78,6 +86,7 @@ Rows rows_of(const at::Tensor* t, at::ScalarType type, int64_t rows, c10::Device
         (t->size(1) > 1 && t->stride(1) != 1) || t->is_conj() || t->is_neg())
         bad(std::string(what) + " must be a " + c10::toString(type) + " tensor [" + std::to_string(rows) +
             "][...] on " + dev.str() + " with contiguous rows");
+    no_grad(*t, what);
     return {t->data_ptr(), t->size(1), t->stride(0)};
 }
 
@@ -114,6 +123,7 @@ float* mass_of(PyObject* o, const Handle& h) {
         t->size(1) != c.layers || t->size(2) != c.ctx_tokens || (c.slots > 1 && (uint64_t)t->stride(0) != c.slot_rows) ||
         (c.layers > 1 && (uint64_t)t->stride(1) != c.layer_rows) || (c.ctx_tokens > 1 && t->stride(2) != 1))
         bad("mass must be a float32 tensor like the scales");
+    no_grad(*t, "mass");
     return (float*)t->data_ptr();
 }
 
@@ -164,10 +174,13 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const qx_cuda_drafts d = drafts(h, a[2], a[3], a[9], seqs, nodes);
     const qx_cuda_heads hq = heads(q, st, x->sizes(), h.dev, "q"), ho = heads(qo, st, x->sizes(), h.dev, "q_out"),
                         hk = heads(k, st, kv_shape, h.dev, "k"), hv = heads(v, st, kv_shape, h.dev, "v");
+    const uint32_t layer = u32(a[1], "layer");
+    const int32_t* positions = plain<int32_t>(a[8], at::kInt, {seqs, nodes}, h.dev, "positions");
+    float* mass = mass_of(a[14], h);
+    uint32_t* status = plain<uint32_t>(a[13], at::kInt, {1}, h.dev, "status");
     char err[256];
-    check(qx_cuda_rope_append_mass(h.c, u32(a[1], "layer"), &d, &rot, type, q ? (uint32_t)q->size(2) : 0u, &hq, &ho, &hk, &hv,
-                                   plain<int32_t>(a[8], at::kInt, {seqs, nodes}, h.dev, "positions"), mass_of(a[14], h),
-                                   plain<uint32_t>(a[13], at::kInt, {1}, h.dev, "status"), stream_of(h.dev), err, sizeof err),
+    check(qx_cuda_rope_append_mass(h.c, layer, &d, &rot, type, q ? (uint32_t)q->size(2) : 0u, &hq, &ho, &hk, &hv, positions, mass,
+                                   status, stream_of(h.dev), err, sizeof err),
           err, "qx_cuda_rope_append");
     if (!q) Py_RETURN_NONE;
     return THPVariable_Wrap(*qo);
@@ -193,20 +206,21 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const qx_cuda_drafts d = drafts(h, a[2], a[3], a[5], seqs, nodes);
     const qx_cuda_heads hq = heads(&q, q.scalar_type(), q.sizes(), h.dev, "q"),
                         ho = heads(out, q.scalar_type(), q.sizes(), h.dev, "out");
+    const uint32_t layer = u32(a[1], "layer");
+    const uint64_t* mask = plain<uint64_t>(a[6], at::kLong, {seqs, nodes, (nodes + 63) / 64}, h.dev, "mask");
+    const float scale = a[7] == Py_None ? (float)(1.0 / std::sqrt((double)h.c->head_dim)) : (float)number(a[7]);
+    float *lse = plain<float>(a[9], at::kFloat, {seqs, nodes, qh}, h.dev, "lse"), *mass = mass_of(a[10], h);
+    uint32_t* status = plain<uint32_t>(a[11], at::kInt, {1}, h.dev, "status");
     char err[256];
     uint64_t bytes = 0;
     check(qx_cuda_tree_attention_workspace((uint32_t)seqs, (uint32_t)nodes, (uint32_t)qh, h.c->kv_heads, h.c->head_dim, type, &bytes,
                                            err, sizeof err),
           err, "qx_cuda_tree_attention");
     void* stream = stream_of(h.dev);
-    const float scale = a[7] == Py_None ? (float)(1.0 / std::sqrt((double)h.c->head_dim)) : (float)number(a[7]);
     // from torch's stream-ordered allocator, so each call and each captured graph has its own
     const at::Tensor work = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-    check(qx_cuda_tree_attention(h.c, u32(a[1], "layer"), &d, type, (uint32_t)qh, &hq, &ho,
-                                 plain<uint64_t>(a[6], at::kLong, {seqs, nodes, (nodes + 63) / 64}, h.dev, "mask"), scale,
-                                 plain<float>(a[9], at::kFloat, {seqs, nodes, qh}, h.dev, "lse"), mass_of(a[10], h),
-                                 work.data_ptr(), bytes, plain<uint32_t>(a[11], at::kInt, {1}, h.dev, "status"), stream, err,
-                                 sizeof err),
+    check(qx_cuda_tree_attention(h.c, layer, &d, type, (uint32_t)qh, &hq, &ho, mask, scale, lse, mass, work.data_ptr(), bytes,
+                                 status, stream, err, sizeof err),
           err, "qx_cuda_tree_attention");
     return THPVariable_Wrap(*out);
     END_HANDLE_TH_ERRORS
@@ -234,12 +248,14 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     same(*kept, at::kInt, {layers, seqs, (int64_t)budget}, h.dev, "kept", kept->is_contiguous());
     same(*fresh, at::kInt, {seqs}, h.dev, "new_lens", fresh->is_contiguous());
     if (seqs > 0xffffffffll) bad("too many sequences");
+    const int32_t *from = plain<int32_t>(a[1], at::kInt, {seqs}, h.dev, "slots"), *to = plain<int32_t>(a[7], at::kInt, {seqs}, h.dev, "dst_slots"),
+                  *lens = plain<int32_t>(a[2], at::kInt, {seqs}, h.dev, "lens");
+    float* mass = mass_of(a[3], h);
+    const uint32_t sink = u32(a[5], "sink"), recent = u32(a[6], "recent");
+    uint32_t* status = plain<uint32_t>(a[10], at::kInt, {1}, h.dev, "status");
     char err[256];
-    check(qx_cuda_kv_evict(h.c, (uint32_t)seqs, plain<int32_t>(a[1], at::kInt, {seqs}, h.dev, "slots"),
-                           plain<int32_t>(a[7], at::kInt, {seqs}, h.dev, "dst_slots"),
-                           plain<int32_t>(a[2], at::kInt, {seqs}, h.dev, "lens"), mass_of(a[3], h), budget, u32(a[5], "sink"),
-                           u32(a[6], "recent"), (int32_t*)kept->data_ptr(), (int32_t*)fresh->data_ptr(),
-                           plain<uint32_t>(a[10], at::kInt, {1}, h.dev, "status"), stream_of(h.dev), err, sizeof err),
+    check(qx_cuda_kv_evict(h.c, (uint32_t)seqs, from, to, lens, mass, budget, sink, recent, (int32_t*)kept->data_ptr(),
+                           (int32_t*)fresh->data_ptr(), status, stream_of(h.dev), err, sizeof err),
           err, "qx_cuda_kv_evict");
     return Py_BuildValue("(NN)", THPVariable_Wrap(*kept), THPVariable_Wrap(*fresh));
     END_HANDLE_TH_ERRORS
@@ -257,7 +273,6 @@ PyObject* pick_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
     qx_cuda_pick p{};
     p.dtype = type_of(x);
     if (rows > 0xffffffffll || vocab > 0xffffffffll) bad("too many rows or tokens");
-    void* stream = stream_of(dev);
     at::Tensor made_out, made_picked;
     if (!out) {
         made_out = at::empty({rows, vocab}, x.options());
@@ -298,7 +313,7 @@ PyObject* pick_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.allowed_stride = (uint64_t)m.stride;
     p.picked = (uint32_t*)picked->data_ptr();
     char err[256];
-    check(qx_cuda_pick_tokens(&p, stream, err, sizeof err), err, "qx_cuda_pick_tokens");
+    check(qx_cuda_pick_tokens(&p, stream_of(dev), err, sizeof err), err, "qx_cuda_pick_tokens");
     return Py_BuildValue("(NN)", THPVariable_Wrap(*out), THPVariable_Wrap(*picked));
     END_HANDLE_TH_ERRORS
 }

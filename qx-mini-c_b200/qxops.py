@@ -6,7 +6,8 @@ on their memory, queued on the current stream of their device.  Outputs that
 are not given are allocated (and outputs that a call may leave in part
 unwritten, zeroed); the scratch of a call comes from torch's allocator.  What
 the checks refuse raises ValueError, what the library refuses RuntimeError with
-its message.
+its message.  The operators have no backward pass: where gradients are recorded
+(outside torch.no_grad()), tensors that require one are refused.
 """
 import ctypes as C
 
