@@ -96,6 +96,11 @@ uint32_t u32(PyObject* o, const char* what) {
     if (v < 0 || v > 0xffffffffll) bad(std::string(what) + " must fit 32 bits");
     return (uint32_t)v;
 }
+bool truth(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v != 0;
+}
 double number(PyObject* o) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw python_error();
@@ -170,7 +175,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t kv_shape[4] = {seqs, nodes, (int64_t)h.c->kv_heads, (int64_t)h.c->head_dim};
     const at::Tensor& inv = needed(a[7], "inv_freq");
     same(inv, at::kDouble, {inv.numel()}, h.dev, "inv_freq", inv.is_contiguous());
-    qx_cuda_rotary rot{(const double*)inv.data_ptr(), number(a[11]), (uint32_t)(2 * inv.numel()), PyObject_IsTrue(a[10]) ? 1u : 0u};
+    qx_cuda_rotary rot{(const double*)inv.data_ptr(), number(a[11]), (uint32_t)(2 * inv.numel()), truth(a[10]) ? 1u : 0u};
     const qx_cuda_drafts d = drafts(h, a[2], a[3], a[9], seqs, nodes);
     const qx_cuda_heads hq = heads(q, st, x->sizes(), h.dev, "q"), ho = heads(qo, st, x->sizes(), h.dev, "q_out"),
                         hk = heads(k, st, kv_shape, h.dev, "k"), hv = heads(v, st, kv_shape, h.dev, "v");

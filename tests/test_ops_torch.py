@@ -151,6 +151,11 @@ def test_shapes_that_belong_together(dev):
 
 @pytest.mark.parametrize("dev", DEVICES)
 def test_errors_of_arguments_that_are_no_tensors_come_through(dev):
+    class Undecided:
+        def __bool__(self):
+            raise KeyError("undecided")
+    with pytest.raises(KeyError):
+        call("rope_append", dict(arguments("rope_append", dev), interleaved=Undecided()))
     with pytest.raises(TypeError):
         call("tree_attention", dict(arguments("tree_attention", dev), scale="half"))
     with pytest.raises(TypeError):
