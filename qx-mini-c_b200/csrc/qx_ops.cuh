@@ -16,7 +16,7 @@
 namespace qx {
 namespace ops {
 
-constexpr uint32_t kMaxSeqs = 4096, kMaxNodes = 4096, kMaxHeads = 1024;
+constexpr uint32_t kMaxSeqs = 4096, kMaxNodes = 4096, kMaxHeads = 1024, kMaxRow = 16384;
 
 inline int refuse(char* err, uint64_t n, const char* m) {
     if (err && n) snprintf(err, (size_t)n, "%s", m);
@@ -70,7 +70,7 @@ inline const char* check_cache(const qx_cuda_kv_cache* c) {
     if (c->slots > 1u << 20 || c->layers > 4096 || c->ctx_tokens > 1u << 24 || c->kv_heads > kMaxHeads || c->head_dim > 4096)
         return "the cache is larger than the operators support";
     const uint64_t row = (uint64_t)c->kv_heads * c->head_dim;
-    if (row % 16 || row > 16384) return "a cache row must be a multiple of 16 bytes and at most 16384";
+    if (row % 16 || row > kMaxRow) return "a cache row must be a multiple of 16 bytes and at most 16384";
     if (!aligned(c->k, 16) || !aligned(c->v, 16)) return "cache codes must be 16-byte aligned";
     if (!aligned(c->k_scales, 4) || !aligned(c->v_scales, 4)) return "cache scales must be 4-byte aligned";
     if (c->slot_rows > 1ull << 40 || c->layer_rows > 1ull << 40) return "cache strides are too large";

@@ -284,7 +284,8 @@ cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
     auto fn = a.interleaved ? (few ? k_rope_append<T, V, true, 256> : k_rope_append<T, V, true, 128>)
                             : (few ? k_rope_append<T, V, false, 256> : k_rope_append<T, V, false, 128>);
     cudaError_t e = cudaSuccess;
-    if (sm > 40 * 1024) e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+    // what the widest row needs, whatever this one does: the attribute is every thread's, and another may be about to launch
+    if (sm > 40 * 1024) e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxRow * 4);
     if (e != cudaSuccess) return e;
     fn<<<grid, few ? 256 : 128, sm, st>>>(a);
     return cudaGetLastError();

@@ -227,6 +227,44 @@ def test_rope_append_of_long_prompts(kind, interleaved):
     check_rope(c, before, 0, slots, lens, nodes, q, k, v, inv, pos, 1.0, 40, interleaved, out, torch.full_like(q, 5))
 
 
+def test_rope_append_from_threads_with_caches_of_different_width():
+    """Rows of 16384 and of 12288 bytes, each from a thread of its own through the C ABI: neither call sets what the other goes by."""
+    import threading
+    lib = opsabi.lib()
+    inv = torch.from_numpy(qxops.rope_frequencies(128)[0]).to(DEV)
+    said, out, keep = {}, {}, []
+
+    def calls(kvh, start):
+        c = make_cache(gen(kvh), 1, 1, 4, kvh, 128)
+        k = torch.randn(1, 2, kvh, 128, generator=gen(kvh), device=DEV)
+        slots, lens = ints([0]), ints([1])
+        keep.append((c, k, slots, lens))
+        h = opsabi.Heads(k.data_ptr(), 2 * kvh * 128, kvh * 128, 128)
+        d, r, none = opsabi.Drafts(1, 2, slots.data_ptr(), lens.data_ptr(), None), opsabi.Rotary(inv.data_ptr(), 1.0, 128, 0), opsabi.Heads()
+        stream = torch.cuda.Stream()
+        err = qxlib.err_buf()
+        torch.cuda.synchronize()
+        start.wait()
+        for i in range(4000):
+            if i % 64 == 0:
+                stream.synchronize()                             # a full queue would have the threads take turns
+            if not lib.qx_cuda_rope_append(C.byref(c.c), 0, C.byref(d), C.byref(r), 0, 0, C.byref(none), C.byref(none), C.byref(h),
+                                           C.byref(h), None, None, stream.cuda_stream, err, len(err)):
+                said[kvh] = err.value
+                break
+        stream.synchronize()
+        out[kvh] = (c.v[0, 0, 1:3].reshape(2, -1), codes_of(k.reshape(2, -1))[0])
+
+    start = threading.Barrier(6)
+    threads = [threading.Thread(target=calls, args=(kvh, start)) for kvh in (128, 96) * 3]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not said
+    assert all(torch.equal(*out[kvh]) for kvh in (128, 96))
+
+
 def test_rope_append_leaves_out_what_does_not_fit():
     g = gen(8)
     c = make_cache(g, 3, 1, 6, 1, 64)
