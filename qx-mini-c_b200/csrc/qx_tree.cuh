@@ -16,6 +16,11 @@
 // multiplied by a power of two that puts its largest value in [2^13, 2^14)
 // (BF16 values more than 2^38 below it lose bits).  F32 queries, and P_t then
 // too, are two F16 terms (hi + the rest, 22 bits).  Everything else is F32.
+// That P_t is one F16 term for half types is a choice: its 2^-11 is the size of
+// an F16 output's own rounding (16 nodes over 4096 random rows: error 2.9e-4
+// against 2.1e-4 with P_t in F32) and an eighth of a BF16 output's (1.68e-3
+// against 1.66e-3), while a second term takes as long as F32 queries do (64 x 16
+// nodes 173 against 151 us).
 //
 // Work is cut into units (sequence, KV head, block of rows) and those into
 // tiles of 64 cache rows; the tiles of all units, laid end to end, are shared

@@ -416,7 +416,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                         const bool raise = big > m + kSlack || (m == -INFINITY && big > -INFINITY);
                         if (__any_sync(~0u, raise)) {
                             // Every row of the warp goes up to the largest score it has seen, so that this is rare from then on;
-                            // by a whole number of powers of two, so that what is rescaled loses no bits.
+                            // by a whole number of powers of two, so that what is rescaled loses no bits: m1's own rounding,
+                            // 2^-24 of it, is far below half a step of the F16 weights, whose second rounding takes it back.
+                            // (Weights that are subnormal by then, 2^-22 of the largest and less, do lose bits.)
                             const float m1 = m == -INFINITY ? top : m + fmaxf(ceilf(top - m), 0.f);
                             const float f = m == -INFINITY ? 0.f : exp2_fast(m - m1);
                             m = m1;
