@@ -240,7 +240,8 @@ int qx_cuda_final_head_noalloc(const float *residual_dev, const float *norm_weig
  * cache, or which writes to a slot that another sequence of the call also
  * uses, is left out of the call (nothing is read or written for it; of mass,
  * see qx_cuda_tree_attention) and a bit is set in *status (device uint32, may
- * be NULL; bits are only ever added).  */
+ * be NULL; bits are only ever added).  What a call writes may overlap nothing
+ * that it reads, but for what its comment allows.  */
 #define QX_CUDA_F32  0u
 #define QX_CUDA_F16  1u
 #define QX_CUDA_BF16 2u
@@ -371,6 +372,7 @@ int qx_cuda_rope_append_mass(const qx_cuda_kv_cache *cache, uint32_t layer, cons
  *   Sequences of one call then need distinct slots: those that share one add
  *   nothing to mass (QX_CUDA_STATUS_SHARED); their out and lse, which are of
  *   no slot, are written all the same.
+ * out may be q itself (same pointer and strides) where mass is NULL.
  * Rows of out and lse past a sequence's nodes stay as they were.  Sequences
  * may share a slot when mass is NULL.  The same call gives the same bits every
  * time; how a sequence's rows are split over the GPU, and so its rounding,

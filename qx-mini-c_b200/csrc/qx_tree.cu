@@ -878,6 +878,13 @@ QX_API int qx_cuda_tree_attention(const qx_cuda_kv_cache* cache, uint32_t layer,
         (mass && drafts->seqs * tiles * (kTile / 16) > 0x7fffffffull))
         return refuse(err, n, "more rows and cache than one call can take");
     if (cache_rows(cache_of(cache)) > 0x7fffffffull - kTile) return refuse(err, n, "the cache has more rows than the operator supports");
+    if (q->data == out->data) {
+        // each block of rows is read by the CTA that writes it, or by all before the join; the mass reads q after that
+        if (mass) return refuse(err, n, "out may not be q itself where mass is collected");
+        if ((drafts->seqs > 1 && q->seq_stride != out->seq_stride) || (drafts->max_nodes > 1 && q->node_stride != out->node_stride) ||
+            (q_heads > 1 && q->head_stride != out->head_stride))
+            return refuse(err, n, "out in place of q must have its strides");
+    }
     DeviceOf dev(cache->k, err, n);
     if (!dev.ok) return 0;
     TreeArgs a{};

@@ -134,7 +134,8 @@ def tree_attention(cache, layer, slots, lens, q, nodes=None, mask=None, scale=No
     q [seqs][nodes][q_heads][head_dim]; mask int64 [seqs][nodes][words] of
     visibility bits, None for a chain; scale None: head_dim ** -0.5; lse
     float32 [seqs][nodes][q_heads] and mass (like the cache's scales) are
-    written where given.  Returns out (like q)."""
+    written where given.  out may be q itself where mass is not given.  Returns
+    out (like q)."""
     return _native.tree_attention(cache.handle, layer, slots, lens, q, nodes, mask, scale, out, lse, mass, status)
 
 

@@ -552,6 +552,22 @@ def test_mass_of_more_queries_than_one_pass_holds(kind, heads, hd, n):
     check_tree(c, 0, ints([2, 0, 3, 1]), ints([200, 0, 17, 400 - n]), ints([n, n, 0, n - 1]), q, random_tree(4, n, 5), hd ** -0.5)
 
 
+@pytest.mark.parametrize("kind,n", [("bf16", 1), ("f16", 4), ("f32", 20)])
+def test_output_in_place_of_the_queries(kind, n):
+    """Without mass out may be q itself; with mass, whose weights are taken from q after out is written, it is refused."""
+    g = gen(17)
+    c = make_cache(g, 3, 1, 700, 2, 64)
+    q = torch.randn(3, n, 16, 64, generator=g, device=DEV).to(TYPES[kind])
+    args = (c, 0, ints([0, 2, 1]), ints([640, 7, 300]))
+    want = qxops.tree_attention(*args, q)
+    here = q.clone()
+    mass = torch.zeros_like(c.k_scales)
+    with pytest.raises(RuntimeError, match="out may not be q itself where mass is collected"):
+        qxops.tree_attention(*args, here, out=here, mass=mass)
+    assert torch.equal(here, q) and not mass.any()
+    assert qxops.tree_attention(*args, here, out=here) is here and torch.equal(here, want)
+
+
 def test_calls_on_two_streams_at_once():
     """Each call has scratch of its own: the bits are those of the calls alone."""
     g = gen(23)

@@ -264,3 +264,10 @@ def test_rope_append_mass_refusals():
     call = lambda k, mass: said(fn, C.byref(c), 0, C.byref(d), C.byref(r), 0, 4, C.byref(h), C.byref(h), k, k, None, mass, None, None)  # noqa: E731
     assert call(None, BASE) == (0, "mass goes with k and v")
     assert call(C.byref(h), BASE + 2) == (0, "mass must be 4-byte aligned")
+
+
+def test_tree_attention_in_place_refusals():
+    assert tree(mass=BASE) == (0, "out may not be q itself where mass is collected")
+    assert tree(q=heads(), out=heads(seq=8 * 4 * 64)) == (0, "out in place of q must have its strides")
+    for apart in (dict(mass=BASE, out=heads(data=1 << 21)), dict()):
+        assert tree(**apart)[1] not in ("", "out may not be q itself where mass is collected")       # refused later, for its made-up addresses
