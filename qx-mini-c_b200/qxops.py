@@ -59,6 +59,15 @@ def _call(fn, *args):
         raise RuntimeError("%s failed: %s" % (fn.__name__, err.value.decode(errors="replace")))
 
 
+def _device_of(address):
+    """The CUDA ordinal of the device that holds an address."""
+    n = C.c_int()
+    code = C.CDLL("libcuda.so.1").cuPointerGetAttribute(C.byref(n), 9, C.c_uint64(address))      # CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL
+    if code:
+        raise RuntimeError("cuPointerGetAttribute failed: %d" % code)
+    return n.value
+
+
 class KvCache:
     """A handle on an INT8 cache (qx_cuda_kv_cache): k, v int8
     [slots][layers][ctx][kv_heads][head_dim] and k_scales, v_scales float32
@@ -93,17 +102,27 @@ class KvCache:
 class EngineCache:
     """The same handle on an engine's own cache (qx_cuda_kv_view): its
     single-sequence cache, or with batch=True the slots of decode_batch.
-    Valid while the engine is open; order calls after the engine's own work
-    (Engine.stream())."""
+    Calls are refused once the engine is closed; order them after the engine's own work
+    (Engine.stream()).  device, if given, must be the engine's."""
 
     def __init__(self, engine, batch=False, device=None):
+        if not engine.h:
+            raise ValueError("the engine is closed")
         self.c = _Cache()
         _call(_cuda().qx_cuda_kv_view, engine.h, 1 if batch else 0, C.byref(self.c))
         self.engine = engine
-        self.device = torch.device("cuda", torch.cuda.current_device() if device is None else device)
-        self.handle = (C.addressof(self.c), self.device.index)
+        self.device = torch.device("cuda", _device_of(self.c.k))
+        if device is not None and torch.device("cuda", device) != self.device:
+            raise ValueError("the engine's cache is on %s" % self.device)
+        self._handle = (C.addressof(self.c), self.device.index)
         self.slots, self.layers, self.ctx = self.c.slots, self.c.layers, self.c.ctx_tokens
         self.kv_heads, self.head_dim = self.c.kv_heads, self.c.head_dim
+
+    @property
+    def handle(self):
+        if not self.engine.h:
+            raise ValueError("the engine of this cache is closed")
+        return self._handle
 
 
 def rope_frequencies(rotary_dim, base=1e6, scheme="none", factor=1.0, original_ctx=4096, low=1.0, high=32.0):

@@ -1000,6 +1000,22 @@ def test_operators_over_an_engines_cache(mini_image):
         eng.close()
 
 
+def test_a_view_ends_with_its_engine_and_knows_its_device(mini_image):
+    """The engine's memory is gone once it is closed: calls with a view of it are refused, before anything is queued."""
+    eng = qxlib.Engine(mini_image, ctx=64, device=0)
+    try:
+        with pytest.raises(ValueError, match="the engine's cache is on cuda:0"):
+            qxops.EngineCache(eng, device=1)
+        view = qxops.EngineCache(eng, device=0)
+        assert view.device == torch.device("cuda", 0) == qxops.EngineCache(eng).device
+    finally:
+        eng.close()
+    q = torch.randn(1, 1, 8, 128, device=DEV)
+    for call in (lambda: qxops.tree_attention(view, 0, ints([0]), ints([0]), q), lambda: qxops.EngineCache(eng)):
+        with pytest.raises(ValueError, match="closed"):
+            call()
+
+
 def test_offsets_past_32_bits():
     """A cache whose last slot starts more than 2^32 bytes in."""
     kvh, hd, ctx, slots = 4, 128, 4096, 2200

@@ -271,3 +271,14 @@ def test_tree_attention_in_place_refusals():
     assert tree(q=heads(), out=heads(seq=8 * 4 * 64)) == (0, "out in place of q must have its strides")
     for apart in (dict(mass=BASE, out=heads(data=1 << 21)), dict()):
         assert tree(**apart)[1] not in ("", "out may not be q itself where mass is collected")       # refused later, for its made-up addresses
+
+
+def test_a_closed_engine_gives_no_view():
+    class Closed:
+        h = None
+    with pytest.raises(ValueError, match="the engine is closed"):
+        qxops.EngineCache(Closed())
+    view = object.__new__(qxops.EngineCache)
+    view.engine = Closed()
+    with pytest.raises(ValueError, match="the engine of this cache is closed"):
+        view.handle
