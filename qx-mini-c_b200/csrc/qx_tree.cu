@@ -699,6 +699,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_tree_mass(const __grid_cons
                         for (int i = 0; i < 4; ++i)
                             if (!(seen >> i & 1u)) e[u][i] = 0.f;
                     }
+                    __syncwarp();                          // the next products are the whole warp's
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) got[i] += e[0][i] + e[1][i];

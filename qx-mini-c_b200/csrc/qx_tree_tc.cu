@@ -384,8 +384,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                     const int t0 = (p.tile0 + j) * kTile;
                     const bool edge = t0 + kTile > p.len;
                     unsigned long long see = 0ull;
-                    if (edge && node >= 0)
-                        see = sees64(a.mask ? a.mask + ((size_t)p.s * a.d.max_nodes + node) * a.words : nullptr, a.words, node, t0, p.len, p.n);
+                    if (edge) {
+                        if (node >= 0)
+                            see = sees64(a.mask ? a.mask + ((size_t)p.s * a.d.max_nodes + node) * a.words : nullptr, a.words, node, t0, p.len, p.n);
+                        __syncwarp();                            // the loads below are the whole warp's
+                    }
                     // 32 columns at a time, in a loop: half the registers, and half the code to fetch
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
@@ -519,6 +522,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
 #pragma unroll 1
                     for (int c = w * (HD / 2); c < (w + 1) * (HD / 2); c += 16) {
                         float2 oa[8] = {}, ob[8] = {};
+                        __syncwarp();                            // lanes without a row went on early
                         if (has_a) tmem_ld16(lanes + S::kO + c, reinterpret_cast<uint32_t*>(oa));
                         if (has_b) tmem_ld16(lanes + S::kO + HD + c, reinterpret_cast<uint32_t*>(ob));
                         wait_ld();
