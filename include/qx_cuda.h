@@ -354,7 +354,10 @@ int qx_cuda_rope_append_mass(const qx_cuda_kv_cache *cache, uint32_t layer, cons
  * nothing gets zeros (and lse -infinity).  What a node does not see does not
  * touch it, whatever it holds.  head_dim 64 or 128; q and out share `dtype`.
  * The value scales of rows that are seen must not be negative; ones below
- * 2^-90 count as 2^-90.
+ * 2^-90 count as 2^-90, and those that one node sees may lie 2^100 apart (rows
+ * further below the largest can lose their share of the softmax's sum).  A row
+ * whose weight times value scale is 2^-32 of the largest and less adds nothing
+ * to out.
  *   What is held in how many bits: scores, the softmax's reference and sum,
  * lse, mass and the sums of both products F32.  The products' operands are
  * F16 numbers.  Codes are exact in them; a value of an F16 or BF16 query is

@@ -9,7 +9,11 @@
 //     o = sum_t P_t v_t / sum_t (P_t / vs_t):
 // what meets the codes v_t in the second product is one F16 number in
 // (0, 2^15] per (row, t) whatever the scales are, and the running reference m
-// is the only thing the accumulators are ever rescaled by.
+// is the only thing the accumulators are ever rescaled by.  The price: P_t / vs_t
+// is lost where P_t is below 2^-126, x_t more than 133 below the largest, so
+// value scales may lie 2^100 apart (what is lost then has a share of 2^-33).
+// And P_t below 2^-25, 2^-32 of the largest, rounds to 0 in F16: such rows add
+// nothing to o, which shows only in dims where all larger rows hold zeros.
 //
 // INT8 codes are exact in F16, so both products run on the tensor cores as F16
 // with F32 accumulation.  F16 and BF16 queries are one F16 term: a row is

@@ -469,6 +469,29 @@ def test_scales_and_queries_of_far_apart_sizes(kind):
     check_tree(c, 0, ints([0, 1, 2, 3]), ints([290, 290, 290, 290]), None, q.to(TYPES[kind]), None, 0.05)
 
 
+@pytest.mark.parametrize("kind,n", [("bf16", 1), ("f16", 4), ("f32", 20), ("bf16", 20)])
+def test_value_scales_as_far_apart_as_they_may_lie(kind, n):
+    """One row's value scale 2^100 times the others', with scores that are equal, and a little apart: none loses its share."""
+    g = gen(18)
+    c = make_cache(g, 2, 1, 300, 2, 64)
+    c.v_scales[:] = 2.0 ** -84
+    c.v_scales[:, 0, 77] = 2.0 ** 16
+    c.k_scales[0] = 0
+    q = torch.randn(2, n, 16, 64, generator=g, device=DEV).to(TYPES[kind])
+    slots, lens, status = ints([0, 1]), ints([270, 270]), ints([0])
+    lse, mass = torch.zeros(2, n, 16, device=DEV), torch.zeros_like(c.k_scales)
+    out = qxops.tree_attention(c, 0, slots, lens, q, scale=0.05, lse=lse, mass=mass, status=status)
+    assert int(status) == 0
+    w_out, w_lse, w_mass, tol, tol_lse, tol_mass = attention(c, 0, slots, lens, ints([n, n]), q, None, 0.05)
+    # On top of attention()'s tolerances: a row meets the codes (127 at most) with P_t = 2^(x_t - m + 8) as F16 numbers, which are
+    # off by up to 2^-25 below 2^-14 (half a subnormal step; two terms too: the rest of such a number is 0).  The reference m is at
+    # most 1 above the largest x, that of the row of scale 2^16, so the sum that divides is at least 2^7 / 2^16:
+    # T rows are off by T 127 2^-25 2^9 together, in dims where that row's code is 0 all there is to see.
+    near(out, w_out, tol + (270 + n) * 127 * 2.0 ** -16, "out")
+    near(lse, w_lse, tol_lse, "lse")
+    near(mass, w_mass, tol_mass + U32 * w_mass, "mass")
+
+
 def test_shared_slots_broadcast_queries_and_strides():
     g = gen(11)
     c = make_cache(g, 2, 3, 120, 2, 128, layer_major=True)
