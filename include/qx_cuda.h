@@ -359,8 +359,9 @@ int qx_cuda_rope_append_mass(const qx_cuda_kv_cache *cache, uint32_t layer, cons
  * whose weight times value scale is 2^-32 of the largest and less adds nothing
  * to out.
  *   What is held in how many bits: scores, the softmax's reference and sum,
- * lse, mass and the sums of both products F32.  The products' operands are
- * F16 numbers.  Codes are exact in them; a value of an F16 or BF16 query is
+ * lse, mass and the sums of both products F32 (these cut off rather than
+ * rounded: F32 outputs over long rows are small by up to 4e-6 of themselves).
+ * The products' operands are F16 numbers.  Codes are exact in them; a value of an F16 or BF16 query is
  * one, exact but for BF16 values 2^38 below their row's largest, which lose
  * bits; and with such queries the weight of a row is one, 11 bits, where a
  * softmax in F32 has 24: with random values the error of F16 outputs grows

@@ -148,10 +148,11 @@ __device__ __forceinline__ void key_halves(const uint4& k, uint32_t* b) {
     }
 }
 // acc[h] += q . k of a staged block and key tile h, dims 64 c to 64 c + 63 (b: their key_halves).
+// The smaller term first: the tensor cores cut what they add to a sum off at its last bit, and what comes first meets small sums.
 template <int HD, int NT>
 __device__ __forceinline__ void dot_block(const uint8_t* block, int c, const uint32_t* b0, const uint32_t* b1, float (&acc)[2][4]) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = NT - 1; t >= 0; --t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint4 q = *reinterpret_cast<const uint4*>(block + t * QBlock<HD, NT>::kTerm + (4 * c + i) * QBlock<HD, NT>::kFrag +

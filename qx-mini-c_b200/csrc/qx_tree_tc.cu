@@ -701,11 +701,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_tree_tc(const __grid_constant
                         if (issues) {
                             const uint64_t k0 = kd + ks * (S::kTileBytes / 16);
                             const uint32_t d = tmem + kTile * sb;
+                            // the smaller term first (qx_tree.cuh)
 #pragma unroll
-                            for (int q = 0; q < NT; ++q)
+                            for (int q = NT - 1; q >= 0; --q)
 #pragma unroll
                                 for (int k = 0; k < HD / 16; ++k)
-                                    mma_ss(d, q0 + q * (S::kQBytes / 16) + k * 16, k0 + k * 16, id, q + k > 0);
+                                    mma_ss(d, q0 + q * (S::kQBytes / 16) + k * 16, k0 + k * 16, id, q < NT - 1 || k > 0);
                             mma_commit(&bars.s_ready[sb]);
                             mma_commit(&bars.k_free[ks]);
                             if (left == 1) mma_commit(&bars.q_free[pc % S::kQs]);

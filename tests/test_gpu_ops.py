@@ -492,6 +492,23 @@ def test_value_scales_as_far_apart_as_they_may_lie(kind, n):
     near(mass, w_mass, tol_mass + U32 * w_mass, "mass")
 
 
+def test_the_smaller_term_of_f32_queries_reaches_the_scores():
+    """128 values of 8192 + 7 2^-10 against codes of 64: the first F16 terms give 2^26, whose last bit is 8, the rest 7 in each of
+    the eight steps of 16 products.  Added to 2^26 one by one, by a unit that cuts sums off, they would all be lost.
+
+    lse of one row is its score, here 2^26 2^-20 and 92 in base 2.  Queries with and without the rest go through the same steps:
+    the product with the row's factor, the reference less 8 and its sum with the logarithm, the product with ln 2, a rounding
+    of 2^-24 each; the sum itself is exact where the rests come first (56 is a multiple of every partial sum's last bit)."""
+    c = qxops.KvCache(*(torch.full((1, 1, 8, 1, 128), 64, dtype=torch.int8, device=DEV) for _ in range(2)),
+                      *(torch.ones(1, 1, 8, device=DEV) for _ in range(2)))
+    q = torch.full((1, 5, 8, 128), 8192.0, device=DEV)
+    q[:, :, ::2] += 7 * 2.0 ** -10
+    lse = torch.zeros(1, 5, 8, device=DEV)
+    qxops.tree_attention(c, 0, ints([0]), ints([1]), q, mask=torch.zeros(1, 5, 1, dtype=torch.int64, device=DEV), scale=2.0 ** -20, lse=lse)
+    more = (lse[:, :, ::2].double() - lse[:, :, 1::2].double()) / 64
+    assert bool(((more - 56 * 2.0 ** -26).abs() <= 8 * 2.0 ** -24).all()), more
+
+
 def test_shared_slots_broadcast_queries_and_strides():
     g = gen(11)
     c = make_cache(g, 2, 3, 120, 2, 128, layer_major=True)
