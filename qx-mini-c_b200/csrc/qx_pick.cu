@@ -327,7 +327,7 @@ cudaError_t run_pick(const PickArgs& a, cudaStream_t st) {
     if (a.rows * 8 <= 148) return launch_pick<T, 1024, 8>(a, st);
     // More rows than there are clusters: smaller ones read the histories less often and wait for fewer, if two of their
     // larger slices fit an SM (256 rows of 32000 took 33 us by clusters of four, take 25 by two; 64 rows of 50257 took
-    // 17 us by eight, take 11 by four; one CTA of 1024 threads with a slice of a quarter was no faster for rows of 151936).
+    // 17 us by eight, take 12 by four; one CTA of 1024 threads with a slice of a quarter was no faster for rows of 151936).
     if (a.rows * 4 > 2 * 148 && slice_of(a.vocab, 2) * 4 <= 100 * 1024) return launch_pick<T, 512, 2>(a, st);
     if (a.rows * 8 > 2 * 148 && slice_of(a.vocab, 4) * 4 <= 100 * 1024) return launch_pick<T, 512, 4>(a, st);
     return launch_pick<T, 512, 8>(a, st);

@@ -84,8 +84,9 @@ __device__ __forceinline__ int code_of(float x, float scale, float inv) {
 // need their row's largest magnitude before they can be quantized).
 //
 // A prompt of 4096 tokens moves 76 MB, 12 us at the memory's rate, and takes
-// 28 us fully rotated, 24 us with half of each head rotated in pairs.  What is left are instructions: the
-// scheduler issues in 62 of 100 cycles, a quarter of them sines and keys in
+// 28 us fully rotated, 24 us with half of each head rotated in pairs.  What is left is a token's chain: the
+// scheduler issues in 48 and 52 of 100 cycles, and warps wait most for loads and
+// at the barrier behind the sines, which a part of the threads works out in
 // double.  8 CTAs to an SM and one item ahead did best: 2 items 33 us, 3 items
 // and 5 CTAs 40 us.
 template <class T, int V, bool IL, int THREADS>
@@ -278,7 +279,7 @@ cudaError_t launch_rope(RopeArgs a, cudaStream_t st) {
     a.v_packs = Over((uint32_t)a.c.head_dim / V);
     const dim3 grid((unsigned)a.d.max_nodes, (unsigned)a.d.seqs);
     const size_t sm = a.k.p ? (size_t)2 * a.c.kv_heads * a.c.head_dim * 4 : 0;
-    // 256 threads a token while all of them run at once (one token 5.6 -> 5.0 us, 64 trees of 16 nodes 7.5 -> 6.9 us; a
+    // 256 threads a token while all of them run at once (one token 5.6 -> 4.8 us, 64 trees of 16 nodes 7.5 -> 6.9 us; a
     // prompt of 4096 tokens 28 -> 37 us)
     const bool few = (uint64_t)a.d.max_nodes * a.d.seqs <= 148 * 8;
     auto fn = a.interleaved ? (few ? k_rope_append<T, V, true, 256> : k_rope_append<T, V, true, 128>)

@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) k_tree_join(const __grid_cons
 //
 // For 64 ragged sequences of one token over up to 4096 rows it is 25 us of the
 // call's 61, bound by instructions and by steps that come out uneven (25 for 16 warps); for 64 trees of 16 nodes (512
-// query rows) over 4096 rows 183 of 334, bound by mma.sync, whose pipe 16 products of 16 x 8 x 16 a block keep busy
+// query rows) over 4096 rows 183 of 333, bound by mma.sync, whose pipe 16 products of 16 x 8 x 16 a block keep busy
 // (staging the queries anew for every tile and block took 1150 us).
 constexpr int kMassWarps = 16, kMassThreads = kMassWarps * 32;
 template <int HD, int NT>

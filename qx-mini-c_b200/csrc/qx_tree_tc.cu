@@ -17,8 +17,8 @@
 // 64 sequences with trees of 16 nodes over 4096 rows (BF16, 4 KV heads of 128:
 // 128 query rows to a KV head, 16640 tiles, 69 GFLOP and 288 MB, 44 us at the memory's rate) take 151
 // us, F32 173 us; one sequence with 13 nodes over 32768 rows (F32) takes 45.  That is
-// 0.9 us a tile and SM, with no unit above half of what it can do (issue slots 44 %, shared memory 44 %,
-// tensor cores 20 %): a tile's chain of product, softmax and product is what takes the time, so two
+// 0.9 us a tile and SM, with no unit above half of what it can do (issue slots 45 %, shared memory 45 %,
+// tensor cores 23 %): a tile's chain of product, softmax and product is what takes the time, so two
 // groups of softmax warps take turns, S runs four tiles ahead, and codes come two or three tiles
 // ahead.  A call with one tile a CTA costs about 20 us: instruction fetch,
 // queries, and the length of that chain.
